@@ -332,6 +332,56 @@ LITHE_API int32_t lithe_pack_raw_batch(const uint16_t* raw, int64_t raw_stride, 
                              uint64_t* bank, int64_t slot_stride, int64_t n_slots, const int32_t* slot_ids,
                              int64_t n_words, int32_t* err_flag, void* stream);
 
+/* Where one operand of lithe_rotate_axes / lithe_qk_norm_rotate sits: element (b, s, h, d) of a
+ * (batch, tokens, heads, dim) tensor is base[b*sample_stride + s*token_stride + h*head_stride + d]
+ * (strides in elements, none negative). */
+typedef struct lithe_heads_view {
+    const void* base;          /* device (an output is written through it) */
+    int64_t sample_stride, token_stride, head_stride;
+    int32_t heads;
+} lithe_heads_view;
+
+#define LITHE_MAX_HEAD_DIM 256
+#define LITHE_MAX_AXES 8
+#define LITHE_POS_I32 0
+#define LITHE_POS_I64 1
+#define LITHE_POS_F32 2
+#define LITHE_PAIR_INTERLEAVED 0    /* pair p = values 2p and 2p + 1 */
+#define LITHE_PAIR_HALVES 1         /* pair p = values p and p + R/2, R = sum of axis_dims */
+
+/*
+ * Rotary positions with several axes (time, row, column): out = x with every head's pairs turned.
+ * It has no counterpart in the reference, whose pipelines take the rotation from diffusers.
+ *   pair p of the axis-a slice (axis_dims[a] / 2 pairs, slices in order) turns by
+ *   positions[token][a] * theta^(-2 i / axis_dims[a]), i = p's index inside the slice:
+ *   (u, v) -> (u cos - v sin, v cos + u sin), in fp32 with the revolution count in fp64, rounded
+ *   once.  The values from R = sum(axis_dims) on are copied.
+ *   dtype      LITHE_DTYPE_BF16, _F16 or _F32 of x and out; out may be x itself (the same view),
+ *              any other overlap of the two is undefined
+ *   positions  device (tokens, n_axes), or (batch, tokens, n_axes) when per_sample != 0, contiguous,
+ *              of pos_type; integers beyond 2^53 are rounded
+ *   axis_dims  HOST (n_axes) even, >= 0, sum at most dim; n_axes 1..LITHE_MAX_AXES
+ * dim even, at most LITHE_MAX_HEAD_DIM (LITHE_ERR_UNSUPPORTED above).  batch or tokens 0: no-op.
+ */
+LITHE_API int32_t lithe_rotate_axes(const lithe_heads_view* x, const lithe_heads_view* out, int32_t dtype,
+                        int32_t batch, int32_t tokens, int32_t dim, const void* positions, int32_t pos_type,
+                        int32_t per_sample, const int32_t* axis_dims, int32_t n_axes, double theta,
+                        int32_t pairing, void* stream);
+
+/*
+ * RMS norm of every head of q and k, then the rotation of lithe_rotate_axes, in one pass:
+ *   n = x * rsqrt(mean(x^2) + eps) * weight   over the head's dim, in fp32; then turned; one rounding.
+ * q and k may have different head counts (grouped heads); out_q / out_k may be slices of larger
+ * buffers (a joint [text; image] sequence) or q / k themselves; any other overlap of an output
+ * with an input or the other output is undefined.
+ *   weight_q, weight_k   device (dim) of weight_dtype (dtype or LITHE_DTYPE_F32), or NULL for ones
+ */
+LITHE_API int32_t lithe_qk_norm_rotate(const lithe_heads_view* q, const lithe_heads_view* k,
+                        const lithe_heads_view* out_q, const lithe_heads_view* out_k, const void* weight_q,
+                        const void* weight_k, int32_t weight_dtype, float eps, int32_t dtype, int32_t batch,
+                        int32_t tokens, int32_t dim, const void* positions, int32_t pos_type, int32_t per_sample,
+                        const int32_t* axis_dims, int32_t n_axes, double theta, int32_t pairing, void* stream);
+
 /*
  * Self-test of the bounded pipeline wait (no counterpart in the reference): one warp waits on
  * an mbarrier that nothing arrives at.  After the wait's time limit (4 s) it ORs

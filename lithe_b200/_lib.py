@@ -29,6 +29,14 @@ DTYPE_BF16 = 0
 DTYPE_F32 = 1
 DTYPE_F16 = 2
 
+POS_I32 = 0
+POS_I64 = 1
+POS_F32 = 2
+PAIR_INTERLEAVED = 0
+PAIR_HALVES = 1
+MAX_HEAD_DIM = 256
+MAX_AXES = 8
+
 MAX_LEVELS = 4
 NOALLOC_WS_BYTES = 4 << 20       # LITHE_NOALLOC_WS_BYTES
 ABI_VERSION = 1
@@ -59,7 +67,20 @@ class PackSegment(ctypes.Structure):
     _fields_ = [("raw_offset", ctypes.c_int64), ("first_block", ctypes.c_int64), ("n_blocks", ctypes.c_int64)]
 
 
+class HeadsView(ctypes.Structure):
+    """``lithe_heads_view``: a (batch, tokens, heads, dim) operand of the rotation kernels."""
+    _fields_ = [("base", ctypes.c_void_p), ("sample_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int32)]
+
+
 _SIGNATURES.update({
+    "lithe_rotate_axes": (_c.c_int32, [
+        _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p,
+        _c.c_int32, _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),
+    "lithe_qk_norm_rotate": (_c.c_int32, [
+        _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.c_void_p,
+        _c.c_void_p, _c.c_int32, _c.c_float, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_int32,
+        _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),
     "lithe_sgmv_index": (_c.c_int32, [
         _c.c_void_p, _c.c_void_p, _c.c_int32, _c.POINTER(IndexView), _c.POINTER(IndexView), _c.c_int64,
         _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32,

@@ -4,6 +4,7 @@
               the whole-adapter decode kernel.
 * ``shared``  index-resident per-sample LoRA delta with the decode fused into the
               shrink / expand tiles (one launch per linear).
+* ``rotary``  rotary positions with several axes, alone or with the per-head norm of q and k.
 * ``layers``  nn.Module wrappers that route each sample of a batch to its own adapter.
 """
 from ._launch import device_errors, raise_device_errors
@@ -11,6 +12,7 @@ from .layers import (IndexLoRALinear, PackedLoRALinear, PerSampleLoRALinear, Sha
                      wrap_linears, wrap_packed)
 from .packed import (PackedBank, PackedLayout, SlotLoader, decode_packed, flat_indices, pack_adapter,
                      pack_indices, split_decoded, unpack_indices)
+from .rotary import qk_norm_rotate, rotate_axes
 from .shared import packed_codebook_lora_delta_, shared_codebook_lora_delta, shared_codebook_lora_delta_
 
 __all__ = [
@@ -19,5 +21,6 @@ __all__ = [
     "PackedBank", "PackedLayout", "SlotLoader", "decode_packed", "flat_indices", "pack_adapter", "pack_indices",
     "split_decoded", "unpack_indices",
     "shared_codebook_lora_delta", "shared_codebook_lora_delta_", "packed_codebook_lora_delta_",
+    "rotate_axes", "qk_norm_rotate",
     "device_errors", "raise_device_errors",
 ]

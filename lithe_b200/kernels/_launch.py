@@ -7,6 +7,7 @@ kernels' device-side error word is read only by ``device_errors``.
 from __future__ import annotations
 
 import ctypes
+import functools
 import threading
 from typing import Optional, Sequence
 
@@ -443,3 +444,164 @@ def pack_raw_batch_(raw: torch.Tensor, segments: torch.Tensor, levels: int, bank
             stream_handle(raw.device))
     _lib.check(rc, "lithe_pack_raw_batch")
     return bank
+
+
+# ------------------------------------------------------------------------------------------
+# Rotation and per-head norm
+# ------------------------------------------------------------------------------------------
+_POS_CODE = {torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64, torch.float32: _lib.POS_F32}
+PAIRINGS = {"interleaved": _lib.PAIR_INTERLEAVED, "halves": _lib.PAIR_HALVES}
+
+
+@functools.lru_cache(maxsize=256)
+def _axis_array(axes: tuple) -> ctypes.Array:
+    return (ctypes.c_int32 * max(1, len(axes)))(*axes)
+
+
+def _heads_strides(t: torch.Tensor) -> tuple:
+    """(sample, token, head) strides; a dimension of one element has none that matters."""
+    return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
+
+
+def _heads_view(t: torch.Tensor) -> _lib.HeadsView:
+    return _lib.HeadsView(t.data_ptr(), *_heads_strides(t), t.shape[2])
+
+
+def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
+    _require_cuda(t, name)
+    if t.dtype not in _DTYPE_CODE:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
+    if t.dim() != 4:
+        raise ValueError(f"{name} must be (batch, tokens, heads, dim), got {tuple(t.shape)}")
+    if t.shape[3] > 1 and t.stride(3) != 1:
+        raise ValueError(f"{name}: the values of a head must be contiguous (stride 1), got stride {t.stride(3)}")
+    if like is not None:
+        if t.dtype != like.dtype or t.device != like.device:
+            raise ValueError(f"{name} must have the inputs' type and device ({like.dtype}, {like.device}), got "
+                             f"{t.dtype}, {t.device}")
+
+
+def _byte_span(t: torch.Tensor) -> tuple:
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _has_own_elements(t: torch.Tensor) -> bool:
+    """Whether no two of ``t``'s elements share an address (an expanded tensor's do)."""
+    reach = 0
+    for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if s <= reach:
+            return False
+        reach += (n - 1) * s
+    return True
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two (batch, tokens, heads, dim) tensors certainly share no element: their bytes do
+    not meet, or they are slices of one buffer that leave each other's part of every token alone."""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    a0, a1 = _byte_span(a)
+    b0, b1 = _byte_span(b)
+    if a1 <= b0 or b1 <= a0:
+        return True
+    sa, sb = _heads_strides(a), _heads_strides(b)
+    if a.shape[:2] != b.shape[:2] or sa[:2] != sb[:2]:
+        return False
+    size = a.element_size()
+    # the period that both repeat with: a token, or (tokens of one sample only) a sample
+    period = sa[1] if a.shape[1] > 1 else sa[0]
+    if period <= 0 or (a.shape[0] > 1 and sa[0] % period) or (b0 - a0) % size:
+        return False
+    inner_a = (a.shape[2] - 1) * sa[2] + a.shape[3]
+    inner_b = (b.shape[2] - 1) * sb[2] + b.shape[3]
+    d = ((b0 - a0) // size) % period
+    return d >= inner_a and d + inner_b <= period
+
+
+def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and a.shape == b.shape and _heads_strides(a) == _heads_strides(b)
+
+
+def _check_outputs(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], names: Sequence[str]) -> None:
+    """Every output is its own input (in place) or shares no element with an input or another output."""
+    for i, (o, name) in enumerate(zip(outs, names)):
+        if not _has_own_elements(o):
+            raise ValueError(f"{name} has elements that share an address")
+        for j, x in enumerate(ins):
+            if not (i == j and _same_view(o, x)) and not _apart(o, x):
+                raise ValueError(f"{name} overlaps an input (it may be its own input's very view)")
+        for j in range(i):
+            if not _apart(o, outs[j]):
+                raise ValueError(f"{name} overlaps {names[j]}")
+
+
+def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta: float, pairing: int) -> tuple:
+    if positions.dtype not in _POS_CODE:
+        raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
+    if positions.device != x.device:
+        raise ValueError("positions must be on the inputs' device")
+    b, s = x.shape[:2]
+    if tuple(positions.shape) not in ((s, len(axes)), (b, s, len(axes))):
+        raise ValueError(f"positions must be ({s}, {len(axes)}) or ({b}, {s}, {len(axes)}), got "
+                         f"{tuple(positions.shape)}")
+    if not positions.is_contiguous():
+        raise ValueError("positions must be contiguous")
+    return (positions.data_ptr(), _POS_CODE[positions.dtype], int(positions.dim() == 3), _axis_array(axes), len(axes),
+            theta, pairing, stream_handle(x.device))
+
+
+def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], theta: float,
+                 pairing: int) -> torch.Tensor:
+    """lithe_rotate_axes on torch tensors: ``out`` (batch, tokens, heads, dim) is written."""
+    _check_heads(x, "x")
+    if out is not x:
+        _check_heads(out, "out", x)
+        if out.shape != x.shape:
+            raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
+        _check_outputs((x,), (out,), ("out",))
+    else:
+        _check_outputs((), (out,), ("x, written in place,",))
+    axes = tuple(axes)
+    with device_ctx(x.device):
+        rc = _lib.lib().lithe_rotate_axes(ctypes.byref(_heads_view(x)), ctypes.byref(_heads_view(out)),
+                                          _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1], x.shape[3],
+                                          *_rotation_args(x, positions, axes, theta, pairing))
+    _lib.check(rc, "lithe_rotate_axes")
+    return out
+
+
+def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k: torch.Tensor,
+                    weight_q: Optional[torch.Tensor], weight_k: Optional[torch.Tensor], positions: torch.Tensor,
+                    axes: Sequence[int], theta: float, eps: float, pairing: int) -> None:
+    """lithe_qk_norm_rotate on torch tensors: ``out_q`` and ``out_k`` are written."""
+    _check_heads(q, "q")
+    _check_heads(k, "k", q)
+    _check_heads(out_q, "out_q", q)
+    _check_heads(out_k, "out_k", q)
+    if k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch, tokens and dim")
+    if out_q.shape != q.shape or out_k.shape != k.shape:
+        raise ValueError(f"out_q and out_k must be {tuple(q.shape)} and {tuple(k.shape)}, got {tuple(out_q.shape)} "
+                         f"and {tuple(out_k.shape)}")
+    weight_dtype = q.dtype
+    for w, name in ((weight_q, "weight_q"), (weight_k, "weight_k")):
+        if w is None:
+            continue
+        if w.dtype not in (q.dtype, torch.float32):
+            raise TypeError(f"{name} must be {q.dtype} or float32, got {w.dtype}")
+        if tuple(w.shape) != (q.shape[3],) or w.device != q.device or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous ({q.shape[3]},) tensor on q's device")
+        weight_dtype = w.dtype
+    if weight_q is not None and weight_k is not None and weight_q.dtype != weight_k.dtype:
+        raise TypeError(f"weight_q and weight_k must have one type, got {weight_q.dtype} and {weight_k.dtype}")
+    _check_outputs((q, k), (out_q, out_k), ("out_q", "out_k"))
+    axes = tuple(axes)
+    with device_ctx(q.device):
+        rc = _lib.lib().lithe_qk_norm_rotate(
+            ctypes.byref(_heads_view(q)), ctypes.byref(_heads_view(k)), ctypes.byref(_heads_view(out_q)),
+            ctypes.byref(_heads_view(out_k)), weight_q.data_ptr() if weight_q is not None else None,
+            weight_k.data_ptr() if weight_k is not None else None, _DTYPE_CODE[weight_dtype], eps,
+            _DTYPE_CODE[q.dtype], q.shape[0], q.shape[1], q.shape[3],
+            *_rotation_args(q, positions, axes, theta, pairing))
+    _lib.check(rc, "lithe_qk_norm_rotate")

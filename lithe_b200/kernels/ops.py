@@ -24,6 +24,9 @@ ABI as a flat list of 2 * levels * 10 floats.
                                                          lithe_lora_prep_multi (linears sharing x;
                                                          one bank tensor pair per target)
   lora_gemm(x, weight, bias, h, b_dec, rows_per_sample) -> out       lithe_lora_gemm
+  rotate_axes_(out!, x, positions, axes, theta, pairing)             lithe_rotate_axes
+  qk_norm_rotate_(out_q!, out_k!, q, k, weight_q, weight_k, positions, axes, theta, eps, pairing)
+                                                         lithe_qk_norm_rotate
   decode_packed(words, n_blocks, levels, sides, lut, fp32) -> out    lithe_decode_packed
 """
 from __future__ import annotations
@@ -153,3 +156,26 @@ def decode_packed(words: torch.Tensor, n_blocks: int, levels: int, sides: Option
 @decode_packed.register_fake
 def _decode_packed_fake(words, n_blocks, levels, sides, lut, fp32):
     return words.new_empty(n_blocks, 64, dtype=torch.float32 if fp32 else torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_NS}::rotate_axes_", mutates_args=("out",), device_types="cuda")
+def rotate_axes_(out: torch.Tensor, x: torch.Tensor, positions: torch.Tensor, axes: List[int], theta: float,
+                 pairing: int) -> None:
+    _launch.rotate_axes_(x, out, positions, axes, theta, pairing)
+
+
+@rotate_axes_.register_fake
+def _rotate_axes_fake(out, x, positions, axes, theta, pairing):
+    return None
+
+
+@torch.library.custom_op(f"{_NS}::qk_norm_rotate_", mutates_args=("out_q", "out_k"), device_types="cuda")
+def qk_norm_rotate_(out_q: torch.Tensor, out_k: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                    weight_q: Optional[torch.Tensor], weight_k: Optional[torch.Tensor], positions: torch.Tensor,
+                    axes: List[int], theta: float, eps: float, pairing: int) -> None:
+    _launch.qk_norm_rotate_(q, k, out_q, out_k, weight_q, weight_k, positions, axes, theta, eps, pairing)
+
+
+@qk_norm_rotate_.register_fake
+def _qk_norm_rotate_fake(out_q, out_k, q, k, weight_q, weight_k, positions, axes, theta, eps, pairing):
+    return None

@@ -1,0 +1,105 @@
+"""Rotary positions with several axes, and the per-head RMS norm of q and k in the same pass.
+
+The step between the q / k projections of an attention block and its attention: images and
+video give every token one position per axis (time, row, column), each axis turns its own slice
+of a head's value pairs, and models of this kind normalise each head of q and k first.
+
+    angle(token, pair) = positions[token, axis] * theta ** (-2 i / axes[axis])
+
+with i the pair's index inside its axis's slice of axes[axis] / 2 pairs (slices in order).
+``pairing`` "interleaved" turns neighbours (2p, 2p + 1), "halves" turns p with p + sum(axes) / 2;
+values from sum(axes) on are left as they are.  Everything is computed in fp32 (the angle's
+revolutions in fp64) and rounded once.
+
+The reference's pipelines take both steps from diffusers; they have no counterpart in it.
+Inference only, like the layers.  Both calls run on the current stream of their inputs' device,
+allocate nothing but their results, and can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from .. import _lib
+from . import _launch
+
+
+def _inference_only(*tensors: Optional[torch.Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
+
+
+def _rotation(dim: int, axes: Sequence[int], theta: float, pairing: str) -> Tuple[Tuple[int, ...], float, int]:
+    axes = tuple(int(a) for a in axes)
+    if pairing not in _launch.PAIRINGS:
+        raise ValueError(f"pairing must be one of {tuple(_launch.PAIRINGS)}, got {pairing!r}")
+    if not 1 <= len(axes) <= _lib.MAX_AXES:
+        raise ValueError(f"1 to {_lib.MAX_AXES} axes, got {len(axes)}")
+    if any(a < 0 or a % 2 for a in axes) or sum(axes) > dim:
+        raise ValueError(f"the axes' dims {axes} must be even, not negative and sum to at most the head dim {dim}")
+    theta = float(theta)
+    if not (theta > 0.0 and math.isfinite(theta)):
+        raise ValueError(f"theta must be positive and finite, got {theta}")
+    return axes, theta, _launch.PAIRINGS[pairing]
+
+
+def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *, theta: float = 10000.0,
+                pairing: str = "interleaved", out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x (batch, tokens, heads, dim) with every head turned by its token's positions.
+
+    ``positions`` (tokens, len(axes)), or (batch, tokens, len(axes)) for positions of each
+    sample's own; int32, int64 or float32, on x's device.  ``axes``: the head's values each axis
+    turns (even, summing to at most dim); dim even, at most 256.  x is bfloat16, float16 or
+    float32, with any strides over samples, tokens and heads (a slice of a fused q / k / v
+    projection).  The result is a new tensor, or ``out`` (x itself to rotate in place).
+    """
+    _launch._check_heads(x, "x")
+    _inference_only(x)
+    axes, theta, code = _rotation(x.shape[3], axes, theta, pairing)
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    positions = positions.contiguous()
+    if torch.compiler.is_compiling():
+        if out is x:
+            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            torch.ops.lithe_b200.rotate_axes_(out, x, positions, list(axes), theta, code)
+            return x.copy_(out)
+        torch.ops.lithe_b200.rotate_axes_(out, x, positions, list(axes), theta, code)
+        return out
+    return _launch.rotate_axes_(x, out, positions, axes, theta, code)
+
+
+def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Tensor],
+                   weight_k: Optional[torch.Tensor], positions: torch.Tensor, axes: Sequence[int], *,
+                   theta: float = 10000.0, eps: float = 1e-6, pairing: str = "interleaved",
+                   out_q: Optional[torch.Tensor] = None,
+                   out_k: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, k) with every head RMS-normalised, weighted and turned by its token's positions.
+
+    q (batch, tokens, heads, dim) and k (batch, tokens, kv_heads, dim), any strides over the
+    first three dimensions.  ``weight_q`` / ``weight_k`` (dim,) of q's type or float32, or None
+    for a norm without weights.  ``positions``, ``axes``, ``theta`` and ``pairing`` as in
+    ``rotate_axes``.  The results are new tensors, or ``out_q`` / ``out_k``: slices of a joint
+    [text; image] buffer, or q and k themselves.
+    """
+    _launch._check_heads(q, "q")
+    _launch._check_heads(k, "k", q)
+    _inference_only(q, k, weight_q, weight_k)
+    eps = float(eps)
+    if not (eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and not negative, got {eps}")
+    axes, theta, code = _rotation(q.shape[3], axes, theta, pairing)
+    if out_q is None:
+        out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out_k is None:
+        out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    positions = positions.contiguous()
+    if torch.compiler.is_compiling():
+        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is q else out_q
+        ok = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is k else out_k
+        torch.ops.lithe_b200.qk_norm_rotate_(oq, ok, q, k, weight_q, weight_k, positions, list(axes), theta, eps, code)
+        return (q.copy_(oq) if out_q is q else oq), (k.copy_(ok) if out_k is k else ok)
+    _launch.qk_norm_rotate_(q, k, out_q, out_k, weight_q, weight_k, positions, axes, theta, eps, code)
+    return out_q, out_k
