@@ -383,6 +383,36 @@ LITHE_API int32_t lithe_qk_norm_rotate(const lithe_heads_view* q, const lithe_he
                         const int32_t* axis_dims, int32_t n_axes, double theta, int32_t pairing, void* stream);
 
 /*
+ * Rows to 8-bit integers, one scale a row (activations per token, weights per output channel):
+ *   scale[r] = max_k |x[r, k]| / 127                                              (fp32)
+ *   q[r, k]  = x[r, k] * 127 / max_k |x[r, k]|, the exact quotient to the nearest whole number,
+ *              ties to even; 0 in a row of zeros (scale 0)
+ * A row that holds an infinity or a NaN gets scale NaN and zeros.  No counterpart in the reference.
+ *   x      device (rows, k) of dtype LITHE_DTYPE_BF16 or _F16, rows x_stride elements apart
+ *   q      device int8 (rows, k), 16-byte aligned, rows q_stride bytes apart (a multiple of 16, at
+ *          least k); the bytes behind a row's k values are left as they are
+ */
+LITHE_API int32_t lithe_quantize_rows(const void* x, int32_t dtype, int32_t rows, int32_t k, int64_t x_stride,
+                        void* q, int64_t q_stride, float* scale, void* stream);
+
+/*
+ * Linear on 8-bit integers, with the adapters' expand of lithe_lora_gemm added before the rounding:
+ *   out[r, :] = (q[r, :] . w^T) * x_scale[r] * w_scale + bias + h[r, :] . b_dec[r / rows_per_sample]^T
+ * The products are summed exactly in int32, the rest in fp32, one rounding to dtype.  It is the
+ * base linear of lithe_lora_gemm with the weights in half the bytes; no counterpart in the reference.
+ *   q, x_scale   what lithe_quantize_rows gives for the activations
+ *   w            device int8 (n, k), 16-byte aligned, rows w_stride bytes apart (a multiple of 16)
+ *   w_scale      device fp32 (n)          bias  device (n) of dtype, or NULL
+ *   out          device (rows, n) of dtype (LITHE_DTYPE_BF16 or _F16), contiguous, written
+ *   h, b_dec     as in lithe_lora_gemm (bf16, rank 16), or NULL; rows_per_sample divides rows
+ * Any rows, n >= 1 and k in 1..131072 (above: LITHE_ERR_UNSUPPORTED, the sums could overflow).
+ */
+LITHE_API int32_t lithe_int8_linear(const void* q, int64_t q_stride, const float* x_scale, const void* w,
+                        int64_t w_stride, const float* w_scale, const void* bias, void* out, int32_t dtype,
+                        int32_t rows, int32_t n, int32_t k, const void* h, const void* b_dec,
+                        int32_t rows_per_sample, int32_t rank, int32_t* err_flag, void* stream);
+
+/*
  * Self-test of the bounded pipeline wait (no counterpart in the reference): one warp waits on
  * an mbarrier that nothing arrives at.  After the wait's time limit (4 s) it ORs
  * LITHE_DEVERR_TIMEOUT into *err_flag, writes 0 to *waited_ok (device int32, may be NULL) and

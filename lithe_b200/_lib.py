@@ -74,6 +74,13 @@ class HeadsView(ctypes.Structure):
 
 
 _SIGNATURES.update({
+    "lithe_quantize_rows": (_c.c_int32, [
+        _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p,
+        _c.c_void_p]),
+    "lithe_int8_linear": (_c.c_int32, [
+        _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+        _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32,
+        _c.c_void_p, _c.c_void_p]),
     "lithe_rotate_axes": (_c.c_int32, [
         _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p,
         _c.c_int32, _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),

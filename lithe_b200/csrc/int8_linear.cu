@@ -1,0 +1,357 @@
+// 8-bit integer linear: activations quantised per token, weights per output channel, the
+// adapters' rank-16 expand added before the one rounding.
+//
+//   s_r = max_k |x[r, k]| / 127,  q[r, k] = x[r, k] * 127 / max_k |x[r, k]| to the nearest whole
+//   number, ties to even                                              (lithe_quantize_rows)
+//   out[r, n] = (sum_k q[r, k] w[n, k]) s_r s_n + bias[n] + sum_j h[r, j] b_dec[sample(r), n, j]
+//                                                                     (lithe_int8_linear)
+//   The products are summed exactly in int32 (k <= 131072), everything after in fp32.
+#include "device_common.cuh"
+#include "host_common.h"
+
+namespace lithe {
+namespace i8 {
+
+constexpr int kRank = 16;              // rank of the fused expand
+constexpr int kMaxK = 131072;          // 127 * 127 * kMaxK < 2^31
+
+// ------------------------------------------------------------------------------------------
+// lithe_quantize_rows
+//
+// q is the exact quotient's rounding: with r = 127 / max and t = x r in fp32, t is within
+// 2^-23 |t| of x 127 / max.  The quotient of two values of at most 11 bits is either exactly
+// halfway between two whole numbers or at least 2^-19 |t| away from it (its distance is a whole
+// number over 2 max's mantissa, 254 of x's mantissa times smaller than |t| at most).  So a t
+// within 2^-21 |t| of halfway is a tie, which goes to the even number, and any other t rounds
+// as the quotient does.
+//
+// Bound: HBM (x read once, a byte a value written).  One CTA a row; a row of up to
+// 8 * kThreadsQ * kChunks values stays in registers between the maximum and the rounding, a
+// longer or unaligned one is read twice (the second time from L2).
+// ------------------------------------------------------------------------------------------
+constexpr int kThreadsQ = 128;
+
+template <bool kF16>
+__device__ __forceinline__ float value_of(uint32_t bits) {
+    if (kF16) return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+    return __uint_as_float(bits << 16);
+}
+
+// Low byte: q of the value x of a row with r = 127 / max (x and r both scaled to keep r finite).
+__device__ __forceinline__ uint32_t quantize(float x, float r) {
+    constexpr float kMagic = 12582912.0f;      // 1.5 * 2^23: adding it rounds to a whole number, ties to even
+    const float t = x * r;
+    const float s = t + kMagic;
+    const float d = fabsf(t - (s - kMagic));
+    if (d > fmaf(fabsf(t), -0x1p-21f, 0.5f)) return 2u * __float_as_uint(fmaf(t, 0.5f, kMagic));
+    return __float_as_uint(s);
+}
+
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+    __shared__ uint32_t part[kThreadsQ / 32];
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    uint32_t m = part[0];
+#pragma unroll
+    for (int i = 1; i < kThreadsQ / 32; ++i) m = max(m, part[i]);
+    return m;
+}
+
+// The row's scale (written by one thread) and the two factors of a value's quotient.  A row with
+// an infinity or NaN gets scale NaN (its outputs are NaN) and zeros.
+template <bool kF16>
+__device__ __forceinline__ void row_factors(uint32_t max_bits, float* scale, float& pre, float& r) {
+    const float most = value_of<kF16>(max_bits);
+    const bool finite = max_bits < (kF16 ? 0x7c00u : 0x7f80u);
+    pre = 1.0f;
+    r = 0.0f;
+    if (finite && most > 0.0f) {
+        if (most < 0x1p-64f) pre = 0x1p+64f;          // keeps 127 / max finite
+        r = __fdiv_rn(127.0f, most * pre);
+    }
+    if (threadIdx.x == 0) *scale = finite ? __fdiv_rn(most, 127.0f) : __uint_as_float(0x7fffffffu);
+    if (!finite) pre = 0.0f;
+}
+
+struct QuantParams {
+    const uint16_t* x;
+    int8_t* q;
+    float* scale;
+    int64_t x_stride, q_stride;
+    int32_t rows, k;
+};
+
+// Eight values to eight bytes.
+template <bool kF16>
+__device__ __forceinline__ uint2 quantize8(const uint4& v, float pre, float r) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        b[2 * i] = quantize(value_of<kF16>(w[i] & 0xffffu) * pre, r);
+        b[2 * i + 1] = quantize(value_of<kF16>(w[i] >> 16) * pre, r);
+    }
+    const uint32_t a0 = __byte_perm(b[0], b[1], 0x0040), a1 = __byte_perm(b[2], b[3], 0x0040);
+    const uint32_t a2 = __byte_perm(b[4], b[5], 0x0040), a3 = __byte_perm(b[6], b[7], 0x0040);
+    return make_uint2(__byte_perm(a0, a1, 0x5410), __byte_perm(a2, a3, 0x5410));
+}
+
+template <bool kF16, int kChunks>
+__global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p) {
+    const int64_t row = blockIdx.x;
+    const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_stride);
+    uint2* q = reinterpret_cast<uint2*>(p.q + row * p.q_stride);
+    const int chunks = p.k >> 3;
+    uint4 v[kChunks];
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int at = c * kThreadsQ + threadIdx.x;
+        v[c] = at < chunks ? __ldg(x + at) : make_uint4(0, 0, 0, 0);
+    }
+    uint32_t m = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c)
+        m = __vmaxu2(__vmaxu2(m, __vmaxu2(v[c].x & 0x7fff7fffu, v[c].y & 0x7fff7fffu)),
+                     __vmaxu2(v[c].z & 0x7fff7fffu, v[c].w & 0x7fff7fffu));
+    m = block_max(max(m & 0xffffu, m >> 16));
+    float pre, r;
+    row_factors<kF16>(m, p.scale + row, pre, r);
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+        const int at = c * kThreadsQ + threadIdx.x;
+        if (at < chunks) q[at] = pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r);
+    }
+}
+
+template <bool kF16>
+__global__ void __launch_bounds__(kThreadsQ) quantize_any_kernel(const QuantParams p) {
+    const int64_t row = blockIdx.x;
+    const uint16_t* x = p.x + row * p.x_stride;
+    int8_t* q = p.q + row * p.q_stride;
+    uint32_t m = 0;
+    for (int i = threadIdx.x; i < p.k; i += kThreadsQ) m = max(m, static_cast<uint32_t>(__ldg(x + i)) & 0x7fffu);
+    m = block_max(m);
+    float pre, r;
+    row_factors<kF16>(m, p.scale + row, pre, r);
+    for (int i = threadIdx.x; i < p.k; i += kThreadsQ)
+        q[i] = pre == 0.0f ? 0 : static_cast<int8_t>(quantize(value_of<kF16>(__ldg(x + i)) * pre, r) & 0xffu);
+}
+
+// ------------------------------------------------------------------------------------------
+// lithe_int8_linear
+// ------------------------------------------------------------------------------------------
+struct Params {
+    const int8_t* q;               // (rows, k), row stride q_stride
+    const int8_t* w;               // (n, k), row stride w_stride
+    const float* x_scale;          // (rows)
+    const float* w_scale;          // (n)
+    const uint16_t* bias;          // (n) or nullptr
+    uint16_t* out;                 // (rows, n)
+    const __nv_bfloat16* h;        // (rows, 16) or nullptr
+    const __nv_bfloat16* b_dec;    // (rows / rows_per_sample, n, 16)
+    int32_t* err;
+    int64_t q_stride, w_stride;
+    int32_t rows, n, k;
+    int32_t rows_per_sample;
+};
+
+// D(16 x 8, int32) += A(16 x 32, int8, row) * B(32 x 8, int8, col)
+__device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 bytes of a row at k0; bytes from k on are zeros.
+__device__ __forceinline__ uint4 load16(const int8_t* row, int k0, int k) {
+    if (k0 + 16 <= k) return __ldg(reinterpret_cast<const uint4*>(row + k0));
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int i = 0; k0 + i < k && i < 16; ++i)
+        w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k0 + i])) << (8 * (i & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Few rows: the weights' bytes are the work.  A CTA takes 16 output channels and 8 kTiles rows;
+// its 8 warps take every 8th piece of 64 k's, so that the channels' rows are read by many warps
+// at once, and add their int32 sums at the end.  Inside a piece a lane reads 16 contiguous bytes
+// of a row and uses its four words as the k's of two MMAs: the same bijection of k for weights
+// and activations, so the sums stand.
+constexpr int kWarpsR = 8;
+constexpr int kUnroll = 4;         // pieces a warp loads before it uses the first
+
+template <bool kF16, int kTiles>
+__global__ void __launch_bounds__(32 * kWarpsR) int8_rows_kernel(const Params p) {
+    __shared__ int part[kWarpsR][8 * kTiles][17];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, kq = 16 * (lane & 3);
+    const int n0 = blockIdx.x * 16, r0 = blockIdx.y * 8 * kTiles;
+    const int8_t* w0 = p.w + static_cast<int64_t>(n0 + g) * p.w_stride;
+    const int8_t* w1 = w0 + 8 * p.w_stride;
+    const bool in0 = n0 + g < p.n, in1 = n0 + g + 8 < p.n;
+    int acc[kTiles][4] = {};
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int k0 = 64 * warp; k0 < p.k; k0 += 64 * kWarpsR * kUnroll) {
+        uint4 a0[kUnroll], a1[kUnroll], b[kUnroll][kTiles];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int k = k0 + 64 * kWarpsR * u + kq;
+            a0[u] = in0 && k < p.k ? load16(w0, k, p.k) : zero;
+            a1[u] = in1 && k < p.k ? load16(w1, k, p.k) : zero;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                const int r = r0 + 8 * t + g;
+                b[u][t] = r < p.rows && k < p.k ? load16(p.q + r * p.q_stride, k, p.k) : zero;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) {
+                mma_s8(acc[t], a0[u].x, a1[u].x, a0[u].y, a1[u].y, b[u][t].x, b[u][t].y);
+                mma_s8(acc[t], a0[u].z, a1[u].z, a0[u].w, a1[u].w, b[u][t].z, b[u][t].w);
+            }
+    }
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)        // element i: channel g + 8 (i / 2), row 2 (lane % 4) + i % 2
+            part[warp][8 * t + 2 * (lane & 3) + (i & 1)][g + 8 * (i >> 1)] = acc[t][i];
+    __syncthreads();
+    for (int e = threadIdx.x; e < 16 * 8 * kTiles; e += 32 * kWarpsR) {
+        const int r = r0 + (e >> 4), n = n0 + (e & 15);
+        if (r >= p.rows || n >= p.n) continue;
+        int sum = 0;
+#pragma unroll
+        for (int i = 0; i < kWarpsR; ++i) sum += part[i][e >> 4][e & 15];
+        float y = static_cast<float>(sum) * p.x_scale[r] * p.w_scale[n];
+        if (p.bias) y += value_of<kF16>(p.bias[n]);
+        if (p.h) {
+            const uint32_t* hr = reinterpret_cast<const uint32_t*>(p.h + static_cast<int64_t>(r) * kRank);
+            const int64_t at = static_cast<int64_t>(r / p.rows_per_sample) * p.n + n;
+            const uint32_t* br = reinterpret_cast<const uint32_t*>(p.b_dec + at * kRank);
+#pragma unroll
+            for (int j = 0; j < kRank / 2; ++j) {
+                const uint32_t hv = __ldg(hr + j), bv = __ldg(br + j);
+                y = fmaf(bf16lo_to_f32(hv), bf16lo_to_f32(bv), y);
+                y = fmaf(bf16hi_to_f32(hv), bf16hi_to_f32(bv), y);
+            }
+        }
+        p.out[static_cast<int64_t>(r) * p.n + n] = static_cast<uint16_t>(Act<kF16>::pack(y, 0.0f) & 0xffffu);
+    }
+}
+
+template <bool kF16, int kTiles>
+int32_t launch_rows(const Params& p, cudaStream_t st) {
+    const dim3 grid((p.n + 15) / 16, (p.rows + 8 * kTiles - 1) / (8 * kTiles));
+    int8_rows_kernel<kF16, kTiles><<<grid, 32 * kWarpsR, 0, st>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "int8_rows_kernel launch");
+}
+
+template <bool kF16>
+int32_t launch_linear(const Params& p, cudaStream_t st) {
+    if (p.rows <= 8) return launch_rows<kF16, 1>(p, st);
+    if (p.rows <= 16) return launch_rows<kF16, 2>(p, st);
+    return launch_rows<kF16, 4>(p, st);
+}
+
+template <bool kF16>
+int32_t launch_quantize(const QuantParams& p, cudaStream_t st) {
+    // whole 16-byte pieces of x to whole 8-byte pieces of q
+    const bool vec = p.k % 8 == 0 && p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+    const int chunks = (p.k / 8 + kThreadsQ - 1) / kThreadsQ;
+    if (vec && chunks <= 2) quantize_kernel<kF16, 2><<<p.rows, kThreadsQ, 0, st>>>(p);
+    else if (vec && chunks <= 4) quantize_kernel<kF16, 4><<<p.rows, kThreadsQ, 0, st>>>(p);
+    else if (vec && chunks <= 8) quantize_kernel<kF16, 8><<<p.rows, kThreadsQ, 0, st>>>(p);
+    else if (vec && chunks <= 16) quantize_kernel<kF16, 16><<<p.rows, kThreadsQ, 0, st>>>(p);
+    else quantize_any_kernel<kF16><<<p.rows, kThreadsQ, 0, st>>>(p);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "quantize_kernel launch");
+}
+
+int32_t check_size(int32_t rows, int32_t n, int32_t k) {
+    if (rows < 0 || n <= 0 || k <= 0) return fail_arg("rows must be >= 0 and n, k > 0 (rows %d, n %d, k %d)", rows, n, k);
+    if (k > kMaxK) return fail_unsupported("k %d above %d: the int32 sums could overflow", k, kMaxK);
+    return LITHE_OK;
+}
+
+int32_t check_bytes(const void* base, int64_t stride, int32_t k, const char* name) {
+    if (!base) return fail_arg("%s must be non-NULL", name);
+    if (reinterpret_cast<uintptr_t>(base) % 16 || stride % 16 || stride < k)
+        return fail_arg("%s: rows must start on 16-byte boundaries, a stride of at least k apart (stride %lld, k %d)",
+                        name, static_cast<long long>(stride), k);
+    return LITHE_OK;
+}
+
+}  // namespace i8
+}  // namespace lithe
+
+extern "C" int32_t lithe_quantize_rows(const void* x, int32_t dtype, int32_t rows, int32_t k, int64_t x_stride,
+                                       void* q, int64_t q_stride, float* scale, void* stream) {
+    using namespace lithe;
+    using namespace lithe::i8;
+    clear_error();
+    if (dtype != LITHE_DTYPE_BF16 && dtype != LITHE_DTYPE_F16)
+        return fail_arg("dtype must be LITHE_DTYPE_BF16 or _F16, got %d", dtype);
+    int32_t rc = check_size(rows, 1, k);
+    if (rc != LITHE_OK) return rc;
+    if (rows == 0) return LITHE_OK;
+    if (!x || !scale) return fail_arg("x and scale must be non-NULL");
+    if (reinterpret_cast<uintptr_t>(x) % 2 || reinterpret_cast<uintptr_t>(scale) % 4)
+        return fail_arg("x and scale must be aligned to their elements");
+    if (x_stride < 0) return fail_arg("x_stride must be >= 0");
+    if ((rc = check_bytes(q, q_stride, k, "q")) != LITHE_OK) return rc;
+    QuantParams p{static_cast<const uint16_t*>(x), static_cast<int8_t*>(q), scale, x_stride, q_stride, rows, k};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == LITHE_DTYPE_F16 ? launch_quantize<true>(p, st) : launch_quantize<false>(p, st);
+}
+
+extern "C" int32_t lithe_int8_linear(const void* q, int64_t q_stride, const float* x_scale, const void* w,
+                                     int64_t w_stride, const float* w_scale, const void* bias, void* out,
+                                     int32_t dtype, int32_t rows, int32_t n, int32_t k, const void* h,
+                                     const void* b_dec, int32_t rows_per_sample, int32_t rank, int32_t* err_flag,
+                                     void* stream) {
+    using namespace lithe;
+    using namespace lithe::i8;
+    clear_error();
+    if (dtype != LITHE_DTYPE_BF16 && dtype != LITHE_DTYPE_F16)
+        return fail_arg("dtype must be LITHE_DTYPE_BF16 or _F16, got %d", dtype);
+    int32_t rc = check_size(rows, n, k);
+    if (rc != LITHE_OK) return rc;
+    if (h) {
+        if (!b_dec) return fail_arg("b_dec is NULL while h is given");
+        if (dtype != LITHE_DTYPE_BF16) return fail_unsupported("the fused expand is bf16");
+        if (rank != kRank) return fail_unsupported("the fused expand supports rank %d, got %d", kRank, rank);
+        if (rows_per_sample <= 0 || rows % rows_per_sample)
+            return fail_arg("rows per sample (%d) must be positive and divide rows (%d)", rows_per_sample, rows);
+        if (reinterpret_cast<uintptr_t>(h) % 16 || reinterpret_cast<uintptr_t>(b_dec) % 16)
+            return fail_arg("h and b_dec must be 16-byte aligned");
+    }
+    if (rows == 0) return LITHE_OK;
+    if ((rc = check_bytes(q, q_stride, k, "q")) != LITHE_OK) return rc;
+    if ((rc = check_bytes(w, w_stride, k, "w")) != LITHE_OK) return rc;
+    if (!x_scale || !w_scale || !out) return fail_arg("x_scale, w_scale and out must be non-NULL");
+    if (reinterpret_cast<uintptr_t>(x_scale) % 4 || reinterpret_cast<uintptr_t>(w_scale) % 4 ||
+        reinterpret_cast<uintptr_t>(out) % 2 || reinterpret_cast<uintptr_t>(bias) % 2)
+        return fail_arg("x_scale, w_scale, bias and out must be aligned to their elements");
+    Params p{};
+    p.q = static_cast<const int8_t*>(q);
+    p.w = static_cast<const int8_t*>(w);
+    p.x_scale = x_scale;
+    p.w_scale = w_scale;
+    p.bias = static_cast<const uint16_t*>(bias);
+    p.out = static_cast<uint16_t*>(out);
+    p.h = static_cast<const __nv_bfloat16*>(h);
+    p.b_dec = static_cast<const __nv_bfloat16*>(b_dec);
+    p.err = err_flag;
+    p.q_stride = q_stride;
+    p.w_stride = w_stride;
+    p.rows = rows;
+    p.n = n;
+    p.k = k;
+    p.rows_per_sample = rows_per_sample;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return dtype == LITHE_DTYPE_F16 ? launch_linear<true>(p, st) : launch_linear<false>(p, st);
+}

@@ -509,14 +509,22 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     if a.shape[:2] != b.shape[:2] or sa[:2] != sb[:2]:
         return False
     size = a.element_size()
-    # the period that both repeat with: a token, or (tokens of one sample only) a sample
-    period = sa[1] if a.shape[1] > 1 else sa[0]
-    if period <= 0 or (a.shape[0] > 1 and sa[0] % period) or (b0 - a0) % size:
+    if (b0 - a0) % size:
         return False
     inner_a = (a.shape[2] - 1) * sa[2] + a.shape[3]
     inner_b = (b.shape[2] - 1) * sb[2] + b.shape[3]
-    d = ((b0 - a0) // size) % period
-    return d >= inner_a and d + inner_b <= period
+    spans = []                      # (period both repeat with, what each covers of one period)
+    if a.shape[1] > 1:
+        if a.shape[0] == 1 or sa[0] % sa[1] == 0:
+            spans.append((sa[1], inner_a, inner_b))
+        inner_a, inner_b = inner_a + (a.shape[1] - 1) * sa[1], inner_b + (b.shape[1] - 1) * sb[1]
+    if a.shape[0] > 1:
+        spans.append((sa[0], inner_a, inner_b))
+    for period, in_a, in_b in spans:
+        d = ((b0 - a0) // size) % period if period > 0 else 0
+        if d >= in_a and d + in_b <= period:
+            return True
+    return False
 
 
 def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -605,3 +613,88 @@ def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k
             _DTYPE_CODE[q.dtype], q.shape[0], q.shape[1], q.shape[3],
             *_rotation_args(q, positions, axes, theta, pairing))
     _lib.check(rc, "lithe_qk_norm_rotate")
+
+
+# ------------------------------------------------------------------------------------------
+# 8-bit integer linear
+# ------------------------------------------------------------------------------------------
+def quantize_rows_(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> None:
+    """lithe_quantize_rows: x (rows, k) bf16 / fp16 -> q (rows, k) int8 and scale (rows,) fp32."""
+    _require_cuda(x, "x")
+    if x.dtype not in ACTIVATION_DTYPES:
+        raise TypeError(f"x must be one of {ACTIVATION_DTYPES}, got {x.dtype}")
+    if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        raise ValueError(f"x must be (rows, k) with contiguous rows, got {tuple(x.shape)}, strides {x.stride()}")
+    if q.shape != x.shape or q.dtype != torch.int8 or q.device != x.device or (q.shape[1] > 1 and q.stride(1) != 1):
+        raise ValueError("q must be an int8 tensor of x's shape with contiguous rows, on x's device")
+    if scale.dtype != torch.float32 or scale.numel() != x.shape[0] or not scale.is_contiguous() \
+            or scale.device != x.device:
+        raise ValueError("scale must be a contiguous (rows,) float32 tensor on x's device")
+    rows, k = x.shape
+    with device_ctx(x.device):
+        rc = _lib.lib().lithe_quantize_rows(x.data_ptr(), _DTYPE_CODE[x.dtype], rows, k,
+                                            x.stride(0) if rows > 1 else 0, q.data_ptr(),
+                                            q.stride(0) if rows > 1 else padded(k), scale.data_ptr(),
+                                            stream_handle(x.device))
+    _lib.check(rc, "lithe_quantize_rows")
+
+
+def padded(k: int) -> int:
+    """Bytes between the starts of 8-bit rows of k values: rows start on 16-byte boundaries."""
+    return -(-k // 16) * 16
+
+
+def int8_linear_(q: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                 bias: Optional[torch.Tensor], out: torch.Tensor, h: Optional[torch.Tensor] = None,
+                 b_dec: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """lithe_int8_linear: out (rows, n) from q (rows, k), x_scale (rows,), weight (n, k), weight_scale (n,)."""
+    _require_cuda(q, "q")
+    dev = q.device
+    if q.dim() != 2 or weight.dim() != 2 or out.dim() != 2:
+        raise ValueError("q (rows, k), weight (n, k) and out (rows, n) must be 2-D")
+    rows, k = q.shape
+    n = weight.shape[0]
+    if weight.dtype != torch.int8 or weight.device != dev:
+        raise TypeError(f"weight must be int8 on {dev}, got {weight.dtype} on {weight.device}")
+    if weight.shape[1] != k or tuple(out.shape) != (rows, n):
+        raise ValueError(f"shapes disagree: q {tuple(q.shape)}, weight {tuple(weight.shape)}, out {tuple(out.shape)}")
+    for t, name in ((q, "q"), (weight, "weight")):
+        if t.dtype != torch.int8 or (k > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) % 16) \
+                or t.data_ptr() % 16:
+            raise ValueError(f"{name}: int8 rows must be contiguous and start on 16-byte boundaries "
+                             f"(strides {t.stride()})")
+    if out.dtype not in ACTIVATION_DTYPES or not out.is_contiguous() or out.device != dev:
+        raise ValueError("out must be a contiguous bfloat16 or float16 tensor on q's device")
+    for t, want, name in ((x_scale, rows, "x_scale"), (weight_scale, n, "weight_scale")):
+        if t.dtype != torch.float32 or t.numel() != want or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{name} must be a contiguous ({want},) float32 tensor on q's device")
+    if bias is not None and (bias.dtype != out.dtype or bias.numel() != n or not bias.is_contiguous()
+                             or bias.device != dev):
+        raise ValueError(f"bias must be a contiguous ({n},) {out.dtype} tensor on q's device")
+    rank = rows_per_sample = 0
+    if (h is None) != (b_dec is None):
+        raise ValueError("h and b_dec come together")
+    if h is not None:
+        for t, name in ((h, "h"), (b_dec, "b_dec")):
+            if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != dev:
+                raise ValueError(f"{name} must be a contiguous bfloat16 tensor on q's device")
+        if h.dim() != 2 or h.shape[0] != rows or b_dec.dim() != 3 or tuple(b_dec.shape[1:]) != (n, h.shape[1]):
+            raise ValueError(f"h must be ({rows}, rank) and b_dec (samples, {n}, rank), got {tuple(h.shape)} and "
+                             f"{tuple(b_dec.shape)}")
+        rank, samples = h.shape[1], b_dec.shape[0]
+        if rows and (samples == 0 or rows % samples):
+            raise ValueError(f"b_dec's {samples} samples do not divide {rows} rows")
+        rows_per_sample = rows // samples if samples else 0
+    if rows == 0:
+        return out
+    if err is None:
+        err = error_word(dev)
+    with device_ctx(dev):
+        rc = _lib.lib().lithe_int8_linear(
+            q.data_ptr(), q.stride(0) if rows > 1 else padded(k), x_scale.data_ptr(), weight.data_ptr(),
+            weight.stride(0) if n > 1 else padded(k), weight_scale.data_ptr(),
+            bias.data_ptr() if bias is not None else None, out.data_ptr(), _DTYPE_CODE[out.dtype], rows, n, k,
+            h.data_ptr() if h is not None else None, b_dec.data_ptr() if b_dec is not None else None,
+            rows_per_sample, rank, err.data_ptr(), stream_handle(dev))
+    _lib.check(rc, "lithe_int8_linear")
+    return out

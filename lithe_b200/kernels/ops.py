@@ -27,6 +27,8 @@ ABI as a flat list of 2 * levels * 10 floats.
   rotate_axes_(out!, x, positions, axes, theta, pairing)             lithe_rotate_axes
   qk_norm_rotate_(out_q!, out_k!, q, k, weight_q, weight_k, positions, axes, theta, eps, pairing)
                                                          lithe_qk_norm_rotate
+  quantize_rows(x) -> (q, scale)                                     lithe_quantize_rows
+  int8_linear(q, x_scale, weight, weight_scale, bias, h, b_dec, fp16) -> out     lithe_int8_linear
   decode_packed(words, n_blocks, levels, sides, lut, fp32) -> out    lithe_decode_packed
 """
 from __future__ import annotations
@@ -179,3 +181,31 @@ def qk_norm_rotate_(out_q: torch.Tensor, out_k: torch.Tensor, q: torch.Tensor, k
 @qk_norm_rotate_.register_fake
 def _qk_norm_rotate_fake(out_q, out_k, q, k, weight_q, weight_k, positions, axes, theta, eps, pairing):
     return None
+
+
+@torch.library.custom_op(f"{_NS}::quantize_rows", mutates_args=(), device_types="cuda")
+def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    rows, k = x.shape
+    q = torch.empty(rows, _launch.padded(k), dtype=torch.int8, device=x.device)[:, :k]
+    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
+    _launch.quantize_rows_(x, q, scale)
+    return q, scale
+
+
+@quantize_rows.register_fake
+def _quantize_rows_fake(x):
+    rows, k = x.shape
+    return (x.new_empty(rows, _launch.padded(k), dtype=torch.int8)[:, :k], x.new_empty(rows, dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{_NS}::int8_linear", mutates_args=(), device_types="cuda")
+def int8_linear(q: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                bias: Optional[torch.Tensor], h: Optional[torch.Tensor], b_dec: Optional[torch.Tensor],
+                fp16: bool) -> torch.Tensor:
+    out = torch.empty(q.shape[0], weight.shape[0], dtype=torch.float16 if fp16 else torch.bfloat16, device=q.device)
+    return _launch.int8_linear_(q, x_scale, weight, weight_scale, bias, out, h, b_dec)
+
+
+@int8_linear.register_fake
+def _int8_linear_fake(q, x_scale, weight, weight_scale, bias, h, b_dec, fp16):
+    return q.new_empty(q.shape[0], weight.shape[0], dtype=torch.float16 if fp16 else torch.bfloat16)
