@@ -140,6 +140,25 @@ int32_t encode_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint6
     return LITHE_OK;
 }
 
+int32_t encode_u8_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch,
+                     uint32_t box_inner, uint32_t box_rows) {
+    PFN_cuTensorMapEncodeTiled_v12000 enc;
+    int32_t rc = get_encoder(&enc);
+    if (rc != LITHE_OK) return rc;
+    const cuuint64_t dims[2] = {inner, rows};
+    const cuuint64_t strides[1] = {pitch};
+    const cuuint32_t box[2] = {box_inner, box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return fail_arg("cuTensorMapEncodeTiled failed (CUresult %d) for bytes: dims (%llu,%llu) pitch %llu",
+                        static_cast<int>(r), (unsigned long long)inner, (unsigned long long)rows,
+                        (unsigned long long)pitch);
+    return LITHE_OK;
+}
+
 void expand_lut(const float* lut, int levels, float out[2][LITHE_MAX_LEVELS][16]) {
     for (int s = 0; s < 2; ++s)
         for (int l = 0; l < LITHE_MAX_LEVELS; ++l)

@@ -36,6 +36,10 @@ int32_t encode_bf16_chunked(CUtensorMap* map, const void* base, uint64_t inner, 
 // 2-D bf16 tensor map (rows of `inner` elements), box (box_inner, box_rows), swizzle 0/32/64/128 B.
 int32_t encode_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint32_t box_inner,
                        uint32_t box_rows, int swizzle_bytes);
+// 2-D tensor map of bytes: rows of `inner` bytes, `pitch` bytes apart (a multiple of 16), box
+// (box_inner, box_rows), 128-byte swizzle.
+int32_t encode_u8_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t rows, uint64_t pitch,
+                     uint32_t box_inner, uint32_t box_rows);
 
 // Fill the kernel-side lookup table lut_dev[side][level][16] from the host-side
 // [2][levels][10] array of the C ABI.

@@ -8,6 +8,7 @@
 //   The products are summed exactly in int32 (k <= 131072), everything after in fp32.
 #include "device_common.cuh"
 #include "host_common.h"
+#include "tcgen05.cuh"
 
 namespace lithe {
 namespace i8 {
@@ -250,11 +251,400 @@ int32_t launch_rows(const Params& p, cudaStream_t st) {
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "int8_rows_kernel launch");
 }
 
+// Many rows: a persistent tcgen05 GEMM (kind::i8, int32 accumulators in TMEM).  kPair: a cluster of
+// two CTAs computes 256 x 256 tiles with cta_group::2 (M256 N256 K32); else one CTA computes
+// 128 x 128 tiles.  Either way a CTA streams 128 rows of q and 128 rows of w, 128 bytes of k each,
+// per stage (two 16 KB TMA boxes, 128-byte swizzle; rows, channels and k's past the ends come as
+// zeros), kStages deep, and keeps two accumulators so that a tile's epilogue runs under the next
+// tile's products.
+//   warp 0       TMA producer          warp 1   TMEM allocation, MMA issue (the pair's leader only)
+//   warps 2..5   epilogue: each 32 accumulator rows, 32 columns at a time
+// The epilogue reads the accumulator in the 16 x 256-bit shape, which is the register layout of a
+// warp MMA's result: scaled, with the bias added, the values are the C operand of one
+// m16n8k16 product of the rows' h and the columns' decoded B factors, so the adapters' expand
+// costs one instruction per 128 outputs and no second accumulator (an int32 accumulator cannot
+// take the expand's fp32 sums).  The factors' k runs through the same bijection in h and b_dec, so
+// that a lane reads 8 contiguous bytes of each.
+// Every mbarrier wait is bounded (4 s, LITHE_DEVERR_TIMEOUT, shared abort flag).
+constexpr int kBK = 128;                       // bytes of k per stage
+constexpr int kRows = 128;                     // rows of q and of w a CTA loads per stage
+constexpr int kBox = kRows * kBK;              // 16 KB
+constexpr int kStages = 6;
+constexpr int kEpiWarps = 4;
+constexpr int kEpiBufs = 2;
+constexpr int kEpiChunk = 32 * 32 * 2;         // staged output: 32 rows x 32 columns
+constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kGroupN = 8;                     // tile order: groups of 8 column tiles, row tiles inside a group
+
+struct Barriers {
+    uint64_t full[kStages], empty[kStages];
+    uint64_t tfull[2], tempty[2];
+    uint64_t done;
+    uint32_t tmem_base;
+    int abort;
+};
+constexpr int kSmemStages = kStages * 2 * kBox;
+constexpr int kSmemEpi = kEpiWarps * kEpiBufs * kEpiChunk;
+constexpr int kSmemBytes = kSmemStages + kSmemEpi + static_cast<int>(sizeof(Barriers)) + 1024;   // + alignment slack
+static_assert(kSmemBytes <= 232448, "shared memory of the tile kernel");
+
+struct TileParams {
+    Params p;
+    int32_t m_tiles, n_tiles, total_tiles;
+    int32_t tma_out;               // the result is stored by TMA (its rows are 16-byte aligned)
+};
+
+// Instruction descriptor of tcgen05.mma kind::i8: int32 accumulator (bits 4-5 = 2), signed A and B
+// (bits 7-9, 10-12 = 1), both K-major, N >> 3 in bits 17-22, M >> 4 in bits 24-28.
+template <bool kPair>
+constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) |
+                            (static_cast<uint32_t>((kPair ? 256 : 128) >> 3) << 17) |
+                            (static_cast<uint32_t>((kPair ? 256 : 128) >> 4) << 24);
+
+template <bool kPair>
+__device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
+    if constexpr (kPair)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(kIdesc<true>), "r"(accumulate));
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+            "l"(adesc), "l"(bdesc), "r"(kIdesc<false>), "r"(accumulate));
+}
+
+// 16 accumulator rows x 32 columns: r[4 j + i] is row lane / 4 + 8 (i / 2), column
+// 8 j + 2 (lane % 4) + i % 2.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
+__device__ __forceinline__ void tile_of(const TileParams& tp, int t, int size, int& m0, int& n0) {
+    const int per_group = kGroupN * tp.m_tiles;
+    const int g = t / per_group;
+    const int in = t - g * per_group;
+    const int width = min(kGroupN, tp.n_tiles - g * kGroupN);
+    m0 = (in / width) * size;
+    n0 = (g * kGroupN + in % width) * size;
+}
+
+template <bool kF16>
+__device__ __forceinline__ void epilogue_tile(const TileParams& tp, const CUtensorMap* tm_out, uint32_t tmem_acc,
+                                              int columns, int row0, int n0, uint8_t* bufs, uint32_t& n_st) {
+    const Params& p = tp.p;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    // the lane's rows: row0 + g + 8 i
+    float sx[4];
+    uint2 h[4];
+    int sample[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = row0 + g + 8 * i;
+        const bool in = r < p.rows;
+        sx[i] = in ? __ldg(p.x_scale + r) : 0.0f;
+        h[i] = p.h && in ? __ldg(reinterpret_cast<const uint2*>(p.h + static_cast<int64_t>(r) * kRank) + q)
+                         : make_uint2(0, 0);
+        sample[i] = p.h ? min(r, p.rows - 1) / p.rows_per_sample : 0;
+    }
+    for (int c0 = 0; c0 < columns && n0 + c0 < p.n && row0 < p.rows; c0 += 32) {
+        uint32_t acc[2][16];
+        tmem_ld_16x32(tmem_acc + c0, acc[0]);
+        tmem_ld_16x32(tmem_acc + (16u << 16) + c0, acc[1]);
+        float sw[4][2], bias[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const int n = n0 + c0 + 8 * j + 2 * q + s;
+                sw[j][s] = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
+                bias[j][s] = p.bias && n < p.n ? value_of<kF16>(__ldg(p.bias + n)) : 0.0f;
+            }
+        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        if (n_st >= static_cast<uint32_t>(kEpiBufs)) {
+            if (lane == 0) bulk_wait_group_read<kEpiBufs - 1>();
+            __syncwarp();
+        }
+        uint8_t* buf = bufs + (n_st % kEpiBufs) * kEpiChunk;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            float y[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    y[j][i] = fmaf(static_cast<float>(static_cast<int>(acc[half][4 * j + i])) * sx[2 * half + (i >> 1)],
+                                   sw[j][i & 1], bias[j][i & 1]);
+            if (p.h) {
+                // the samples of the 16 rows (one, unless a sample ends among them)
+                const int first = __shfl_sync(0xffffffffu, sample[2 * half], 0);
+                const int last = __shfl_sync(0xffffffffu, sample[2 * half + 1], 31);
+                for (int s = first; s <= last; ++s) {
+                    const bool lo = sample[2 * half] == s, hi = sample[2 * half + 1] == s;
+                    const uint32_t a[4] = {lo ? h[2 * half].x : 0u, hi ? h[2 * half + 1].x : 0u,
+                                           lo ? h[2 * half].y : 0u, hi ? h[2 * half + 1].y : 0u};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int n = min(n0 + c0 + 8 * j + g, p.n - 1);
+                        const uint2 b = __ldg(reinterpret_cast<const uint2*>(
+                                                  p.b_dec + (static_cast<int64_t>(s) * p.n + n) * kRank) + q);
+                        mma_bf16_16816(y[j], a, b.x, b.y, y[j]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 16 * half + g + 8 * i;      // staged row; 16-byte unit j at j ^ ((r >> 1) & 3)
+                    *reinterpret_cast<uint32_t*>(buf + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + 4 * q) =
+                        Act<kF16>::pack(y[j][2 * i], y[j][2 * i + 1]);
+                }
+        }
+        if (tp.tma_out) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(tm_out, buf, n0 + c0, row0);
+                bulk_commit_group();
+            }
+            ++n_st;
+        } else {
+            __syncwarp();
+            const int rows = min(32, p.rows - row0);
+            if (n0 + c0 + lane < p.n)
+                for (int r = 0; r < rows; ++r)
+                    p.out[static_cast<int64_t>(row0 + r) * p.n + n0 + c0 + lane] = *reinterpret_cast<uint16_t*>(
+                        buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (lane & 7));
+            __syncwarp();
+        }
+    }
+}
+
+template <bool kPair, bool kF16>
+__device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const CUtensorMap& tm_w,
+                                                 const CUtensorMap& tm_out, const TileParams& tp) {
+    constexpr int kSize = kPair ? 256 : 128;               // rows and columns of a tile
+    constexpr uint32_t kCols = 2 * kSize;                  // TMEM columns: two accumulators
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* epi_base = smem + kSmemStages;
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + kSmemStages + kSmemEpi);
+    volatile int* abort = &bars->abort;
+    int32_t* err = tp.p.err;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = kPair ? static_cast<int>(cluster_rank()) : 0;
+    const bool leader = rank == 0;
+    const int nk = (tp.p.k + kBK - 1) / kBK;
+    const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(&bars->full[s], 1);
+            mbar_init(&bars->empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&bars->tfull[a], 1);
+            mbar_init(&bars->tempty[a], (kPair ? 2 : 1) * kEpiWarps);
+        }
+        mbar_init(&bars->done, 1);
+        bars->abort = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_w);
+    }
+    if (warp == 1) {
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(&bars->tmem_base)),
+                         "r"(kCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                             smem_u32(&bars->tmem_base)),
+                         "r"(kCols));
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+        }
+    }
+    tc_fence_before();
+    if constexpr (kPair) cluster_sync();                   // both CTAs' barriers initialised, TMEM allocated
+    else __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = bars->tmem_base;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            for (int t = first; t < tp.total_tiles && !*abort; t += step) {
+                int m0, n0;
+                tile_of(tp, t, kSize, m0, n0);
+                for (int kb = 0; kb < nk; ++kb, ++it) {
+                    const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
+                    if (!mbar_wait(&bars->empty[s], ph ^ 1u, abort, err)) break;
+                    uint8_t* a = smem + s * 2 * kBox;
+                    if constexpr (kPair) {
+                        if (leader) mbar_arrive_expect_tx(&bars->full[s], 4 * kBox);
+                        const uint32_t fb = map_to_rank(&bars->full[s], 0);
+                        tma_load_2d_pair(a, &tm_q, fb, kb * kBK, m0 + kRows * rank);
+                        tma_load_2d_pair(a + kBox, &tm_w, fb, kb * kBK, n0 + kRows * rank);
+                    } else {
+                        mbar_arrive_expect_tx(&bars->full[s], 2 * kBox);
+                        tma_load_2d(a, &tm_q, &bars->full[s], kb * kBK, m0);
+                        tma_load_2d(a + kBox, &tm_w, &bars->full[s], kb * kBK, n0);
+                    }
+                }
+            }
+            if (*abort) drain_pause();
+        }
+    } else if (warp == 1) {
+        if (leader && lane == 0) {
+            uint32_t it = 0, tile = 0;
+            for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
+                const uint32_t acc = tile & 1u, aph = (tile >> 1) & 1u;
+                if (!mbar_wait(&bars->tempty[acc], aph ^ 1u, abort, err)) break;
+                tc_fence_after();
+                const uint32_t d = tmem + acc * kSize;
+                bool ok = true;
+                for (int kb = 0; kb < nk; ++kb, ++it) {
+                    const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
+                    if (!mbar_wait(&bars->full[s], ph, abort, err)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a = smem_u32(smem + s * 2 * kBox);
+                    const uint64_t ad = desc_k_major(a, 128, 2), bd = desc_k_major(a + kBox, 128, 2);
+#pragma unroll
+                    for (int kk = 0; kk < kBK / 32; ++kk)  // +32 bytes along k inside the 128-byte swizzle atom
+                        umma_i8<kPair>(d, ad + 2 * kk, bd + 2 * kk, (kb | kk) != 0);
+                    if constexpr (kPair) umma_commit_pair(&bars->empty[s]);
+                    else umma_commit(&bars->empty[s]);
+                }
+                if (!ok) break;
+                if constexpr (kPair) umma_commit_pair(&bars->tfull[acc]);
+                else umma_commit(&bars->tfull[acc]);
+            }
+            if constexpr (kPair) umma_commit_pair_local(&bars->done);
+            else umma_commit(&bars->done);                 // arrives once every MMA above has completed
+        }
+    } else {
+        const int quarter = warp & 3;                      // TMEM lanes 32 * quarter .. + 31
+        uint8_t* bufs = epi_base + quarter * kEpiBufs * kEpiChunk;
+        uint32_t tempty[2] = {0, 0};
+        if constexpr (kPair) {
+            tempty[0] = map_to_rank(&bars->tempty[0], 0);
+            tempty[1] = map_to_rank(&bars->tempty[1], 0);
+        }
+        uint32_t n_st = 0, tile = 0;
+        for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
+            int m0, n0;
+            tile_of(tp, t, kSize, m0, n0);
+            const uint32_t acc = tile & 1u, aph = (tile >> 1) & 1u;
+            if (!mbar_wait(&bars->tfull[acc], aph, abort, err)) break;
+            tc_fence_after();
+            epilogue_tile<kF16>(tp, &tm_out, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kSize, kSize,
+                                m0 + kRows * rank + 32 * quarter, n0, bufs, n_st);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if constexpr (kPair) mbar_arrive_remote(tempty[acc]);
+                else mbar_arrive(&bars->tempty[acc]);
+            }
+        }
+        if (lane == 0) bulk_wait_group_all();              // the last stores have left shared memory
+        __syncwarp();
+    }
+
+    __syncthreads();
+    if (leader && warp == 1 && lane == 0) {
+        const uint64_t t0 = global_timer_ns();
+        while (!mbar_try_wait(&bars->done, 0) && global_timer_ns() - t0 < 100000000ull) {
+        }
+    }
+    tc_fence_before();
+    if constexpr (kPair) cluster_sync();                   // the pair's MMAs are done before either CTA frees anything
+    else __syncthreads();
+    tc_fence_after();
+    if (warp == 1) {
+        if constexpr (kPair)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kCols));
+    }
+}
+
+template <bool kF16>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ TileParams tp) {
+    tile_kernel_body<true, kF16>(tm_q, tm_w, tm_out, tp);
+}
+
+template <bool kF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    int8_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_w,
+                     const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ TileParams tp) {
+    tile_kernel_body<false, kF16>(tm_q, tm_w, tm_out, tp);
+}
+
+template <bool kF16>
+int32_t launch_tiles(const Params& p, int device, int sms, bool pair, cudaStream_t st) {
+    CUtensorMap tm_q, tm_w, tm_out;
+    int32_t rc = encode_u8_2d(&tm_q, p.q, p.k, p.rows, p.q_stride, kBK, kRows);
+    if (rc != LITHE_OK) return rc;
+    if ((rc = encode_u8_2d(&tm_w, p.w, p.k, p.n, p.w_stride, kBK, kRows)) != LITHE_OK) return rc;
+    TileParams tp{};
+    tp.p = p;
+    tp.tma_out = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+    // the map's element type only has to have 16 bits
+    if (tp.tma_out) {
+        if ((rc = encode_bf16_2d(&tm_out, p.out, p.n, p.rows, 32, 32, 64)) != LITHE_OK) return rc;
+    } else {
+        tm_out = tm_q;
+    }
+    const int size = pair ? 256 : 128;
+    tp.m_tiles = (p.rows + size - 1) / size;
+    tp.n_tiles = (p.n + size - 1) / size;
+    const int64_t tiles = static_cast<int64_t>(tp.m_tiles) * tp.n_tiles;
+    if (tiles > 0x7fffffffLL - 0x10000) return fail_arg("too many tiles");
+    tp.total_tiles = static_cast<int32_t>(tiles);
+    static bool configured[64] = {false};
+    if (!configured[device]) {
+        cudaError_t e = cudaFuncSetAttribute(int8_pair_kernel<kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kSmemBytes);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(int8_tile_kernel<kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(int8 tile kernels)");
+        configured[device] = true;
+    }
+    if (pair) {
+        const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
+        int8_pair_kernel<kF16><<<static_cast<int>(2 * pairs), kThreads, kSmemBytes, st>>>(tm_q, tm_w, tm_out, tp);
+    } else {
+        const int grid = static_cast<int>(tiles < sms ? tiles : sms);
+        int8_tile_kernel<kF16><<<grid, kThreads, kSmemBytes, st>>>(tm_q, tm_w, tm_out, tp);
+    }
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "int8 tile kernel launch");
+}
+
 template <bool kF16>
 int32_t launch_linear(const Params& p, cudaStream_t st) {
     if (p.rows <= 8) return launch_rows<kF16, 1>(p, st);
     if (p.rows <= 16) return launch_rows<kF16, 2>(p, st);
-    return launch_rows<kF16, 4>(p, st);
+    if (p.rows <= 32) return launch_rows<kF16, 4>(p, st);
+    int device = 0, sms = 0;
+    const int32_t rc = current_device_sms(&device, &sms);
+    if (rc != LITHE_OK) return rc;
+    // Pairs once their 256 x 256 tiles fill the GPU; 128 x 128 tiles before, to use more SMs.
+    const int64_t pair_tiles = static_cast<int64_t>((p.rows + 255) / 256) * ((p.n + 255) / 256);
+    return launch_tiles<kF16>(p, device, sms, pair_tiles >= sms / 2, st);
 }
 
 template <bool kF16>
