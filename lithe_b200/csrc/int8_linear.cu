@@ -258,40 +258,79 @@ int32_t launch_rows(const Params& p, cudaStream_t st) {
 // zeros), kStages deep, and keeps two accumulators so that a tile's epilogue runs under the next
 // tile's products.
 //   warp 0       TMA producer          warp 1   TMEM allocation, MMA issue (the pair's leader only)
-//   warps 2..5   epilogue: each 32 accumulator rows, 32 columns at a time
-// The epilogue reads the accumulator in the 16 x 256-bit shape, which is the register layout of a
-// warp MMA's result: scaled, with the bias added, the values are the C operand of one
-// m16n8k16 product of the rows' h and the columns' decoded B factors, so the adapters' expand
-// costs one instruction per 128 outputs and no second accumulator (an int32 accumulator cannot
-// take the expand's fp32 sums).  The factors' k runs through the same bijection in h and b_dec, so
-// that a lane reads 8 contiguous bytes of each.
+//   warps 2..9   epilogue: each 32 accumulator rows and half of the columns, 64 at a time
+//   warp 10      (kExpandTmem) issues the expand
+// The epilogue reads the accumulator in the 16 x 256-bit shape, the register layout of a warp MMA's
+// result: a lane holds column pairs of four rows, so a column's scale and bias are read once for
+// all of them, and two neighbouring results make one staged word.
+//
+// The expand h . b_dec^T (an int32 accumulator cannot take its fp32 sums):
+//   kExpandMma    one m16n8k16 warp MMA per 128 outputs on top of the scaled sums, any rows per sample.
+//                 The factors' k runs through the same bijection in h and b_dec, so that a lane reads
+//                 8 contiguous bytes of each.
+//   kExpandTmem   (pairs, samples of whole tiles) the epilogue writes the scaled sums, now fp32, back into
+//                 TMEM in place of the int32 ones; one tcgen05.mma (kind::f16, K = 16) adds the expand
+//                 of the whole tile there, issued by a warp of its own (polled for by the products'
+//                 issuer it cost 10%), and the epilogue reads the result.  Warp MMAs share the
+//                 tensor pipe with tcgen05.mma and slow it: 57344 x 3072 -> 12288 takes 1.71 ms
+//                 this way, 2.1 ms with them and 1.6 ms without an expand (1.46 ms: the products
+//                 alone; all of it under the 1 kW cap, at 1.3 to 1.5 GHz).
+// Measured without an expand: 14336 x 3072 -> 12288 2.8 POP/s, x 768 -> 12288 130 us (an epilogue of 4
+// warps with a TMA store of 64-byte rows: 257 us).  In a tile the stages' bytes (64 KB a pair and
+// 128 k's) keep shared memory as busy as the products keep the tensor pipe.
 // Every mbarrier wait is bounded (4 s, LITHE_DEVERR_TIMEOUT, shared abort flag).
+enum Expand { kExpandNone, kExpandMma, kExpandTmem };
+
 constexpr int kBK = 128;                       // bytes of k per stage
 constexpr int kRows = 128;                     // rows of q and of w a CTA loads per stage
 constexpr int kBox = kRows * kBK;              // 16 KB
 constexpr int kStages = 6;
-constexpr int kEpiWarps = 4;
-constexpr int kEpiBufs = 2;
-constexpr int kEpiChunk = 32 * 32 * 2;         // staged output: 32 rows x 32 columns
-constexpr int kThreads = 32 * (2 + kEpiWarps);
+constexpr int kEpiWarps = 8;                   // two for each 32 accumulator rows
+constexpr int kEpiChunk = 16 * 64 * 2;         // a warp's staged output: 16 rows x 64 columns
+template <int kExpand>
+constexpr int kThreads = 32 * (2 + kEpiWarps + (kExpand == kExpandTmem ? 1 : 0));
 constexpr int kGroupN = 8;                     // tile order: groups of 8 column tiles, row tiles inside a group
+constexpr int kHBytes = kRows * kRank * 2;     // 4 KB: a CTA's rows of h
+constexpr int kExpandBytes = 2 * kHBytes;      // and 4 KB: its half of the tile's columns of b_dec
+
 
 struct Barriers {
     uint64_t full[kStages], empty[kStages];
     uint64_t tfull[2], tempty[2];
-    uint64_t done;
+    uint64_t cfull, cempty;                    // the tile's columns staged / done with
+    uint64_t lfull[2], lempty[2];              // kExpandTmem: h and b_dec of a tile
+    uint64_t ereq, efull;                      // scaled sums back in TMEM / expand added to them
+    uint64_t done, edone;                      // every product / every expand issued has completed
     uint32_t tmem_base;
     int abort;
 };
-constexpr int kSmemStages = kStages * 2 * kBox;
-constexpr int kSmemEpi = kEpiWarps * kEpiBufs * kEpiChunk;
-constexpr int kSmemBytes = kSmemStages + kSmemEpi + static_cast<int>(sizeof(Barriers)) + 1024;   // + alignment slack
-static_assert(kSmemBytes <= 232448, "shared memory of the tile kernel");
+
+// What the epilogue needs of a tile's columns, staged once per tile: scale, bias and (kExpandMma) the
+// decoded B factors of the sample of the CTA's first row; rows of other samples read theirs from
+// global memory.
+template <int kSize, int kExpand>
+struct Columns {
+    float scale[kSize];
+    uint16_t bias[kSize];
+    uint4 factors[kExpand == kExpandMma ? kSize : 1][2];
+};
+
+// Shared memory: stages, h and b_dec (two tiles), staged output, columns, barriers.
+template <int kSize, int kExpand>
+struct Layout {
+    static constexpr int kExpandAt = kStages * 2 * kBox;
+    static constexpr int kOutAt = kExpandAt + (kExpand == kExpandTmem ? 2 * kExpandBytes : 0);
+    static constexpr int kColumnsAt = kOutAt + kEpiWarps * kEpiChunk;
+    static constexpr int kBarriersAt = kColumnsAt + static_cast<int>(sizeof(Columns<kSize, kExpand>));
+    static constexpr int kBytes = kBarriersAt + static_cast<int>(sizeof(Barriers)) + 1024;   // + alignment slack
+    static_assert(kBytes <= 232448, "shared memory of the tile kernel");
+    static_assert(kColumnsAt % 16 == 0 && kBarriersAt % 16 == 0, "alignment");
+};
 
 struct TileParams {
     Params p;
     int32_t m_tiles, n_tiles, total_tiles;
-    int32_t tma_out;               // the result is stored by TMA (its rows are 16-byte aligned)
+    int32_t out16;                 // the result's rows are 16-byte aligned
 };
 
 // Instruction descriptor of tcgen05.mma kind::i8: int32 accumulator (bits 4-5 = 2), signed A and B
@@ -300,6 +339,9 @@ template <bool kPair>
 constexpr uint32_t kIdesc = (2u << 4) | (1u << 7) | (1u << 10) |
                             (static_cast<uint32_t>((kPair ? 256 : 128) >> 3) << 17) |
                             (static_cast<uint32_t>((kPair ? 256 : 128) >> 4) << 24);
+// The expand's, kind::f16: fp32 accumulator, bf16 A and B, M256 N256.
+constexpr uint32_t kIdescExpand = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(256 >> 3) << 17) |
+                                  (static_cast<uint32_t>(256 >> 4) << 24);
 
 template <bool kPair>
 __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t accumulate) {
@@ -315,16 +357,38 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
             "l"(adesc), "l"(bdesc), "r"(kIdesc<false>), "r"(accumulate));
 }
 
-// 16 accumulator rows x 32 columns: r[4 j + i] is row lane / 4 + 8 (i / 2), column
-// 8 j + 2 (lane % 4) + i % 2.
-__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void umma_expand(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-        "%15}, [%16];"
+        "{\n .reg .pred p;\n setp.eq.b32 p, 0, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+        "l"(adesc), "l"(bdesc), "r"(kIdescExpand));
+}
+
+// 16 accumulator rows x 64 columns: r[4 j + i] is row lane / 4 + 8 (i / 2), column
+// 8 j + 2 (lane % 4) + i % 2, once tcgen05.wait::ld has returned.
+__device__ __forceinline__ void tmem_ld_16x64(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(taddr));
 }
+__device__ __forceinline__ void tmem_st_16x64(uint32_t taddr, const float (&y)[8][4]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.16x256b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "f"(y[0][0]), "f"(y[0][1]), "f"(y[0][2]), "f"(y[0][3]), "f"(y[1][0]), "f"(y[1][1]), "f"(y[1][2]),
+        "f"(y[1][3]), "f"(y[2][0]), "f"(y[2][1]), "f"(y[2][2]), "f"(y[2][3]), "f"(y[3][0]), "f"(y[3][1]),
+        "f"(y[3][2]), "f"(y[3][3]), "f"(y[4][0]), "f"(y[4][1]), "f"(y[4][2]), "f"(y[4][3]), "f"(y[5][0]),
+        "f"(y[5][1]), "f"(y[5][2]), "f"(y[5][3]), "f"(y[6][0]), "f"(y[6][1]), "f"(y[6][2]), "f"(y[6][3]),
+        "f"(y[7][0]), "f"(y[7][1]), "f"(y[7][2]), "f"(y[7][3])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tile_of(const TileParams& tp, int t, int size, int& m0, int& n0) {
     const int per_group = kGroupN * tp.m_tiles;
@@ -335,107 +399,179 @@ __device__ __forceinline__ void tile_of(const TileParams& tp, int t, int size, i
     n0 = (g * kGroupN + in % width) * size;
 }
 
-template <bool kF16>
-__device__ __forceinline__ void epilogue_tile(const TileParams& tp, const CUtensorMap* tm_out, uint32_t tmem_acc,
-                                              int columns, int row0, int n0, uint8_t* bufs, uint32_t& n_st) {
-    const Params& p = tp.p;
-    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-    // the lane's rows: row0 + g + 8 i
+// One epilogue thread's part of a tile's columns, on its way from global memory: loaded while the
+// tile before is finished, so that no epilogue waits for it.
+template <int kSize, int kExpand>
+struct ColumnRegs {
+    uint4 f[2];
+    float scale;
+    uint16_t bias;
+
+    __device__ __forceinline__ void load(const Params& p, int row, int n0, int thread) {
+        if (thread >= kSize) return;
+        const int n = min(n0 + thread, p.n - 1);
+        scale = __ldg(p.w_scale + n);
+        bias = p.bias ? __ldg(p.bias + n) : static_cast<uint16_t>(0);
+        if constexpr (kExpand == kExpandMma) {
+            const int sample = min(row, p.rows - 1) / p.rows_per_sample;
+            const uint4* b = reinterpret_cast<const uint4*>(p.b_dec + (static_cast<int64_t>(sample) * p.n + n) * kRank);
+            f[0] = __ldg(b);
+            f[1] = __ldg(b + 1);
+        }
+    }
+    __device__ __forceinline__ void store(Columns<kSize, kExpand>* c, int thread) const {
+        if (thread >= kSize) return;
+        c->scale[thread] = scale;
+        c->bias[thread] = bias;
+        if constexpr (kExpand == kExpandMma) {
+            c->factors[thread][0] = f[0];
+            c->factors[thread][1] = f[1];
+        }
+    }
+};
+
+// What the epilogue needs of a lane's rows row0 + lane / 4 + 8 i.
+template <int kExpand>
+struct RowRegs {
     float sx[4];
     uint2 h[4];
     int sample[4];
+
+    __device__ __forceinline__ void load(const Params& p, int row0, int lane) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row0 + (lane >> 2) + 8 * i;
+            const bool in = r < p.rows;
+            sx[i] = in ? __ldg(p.x_scale + r) : 0.0f;
+            if constexpr (kExpand == kExpandMma) {
+                h[i] = in ? __ldg(reinterpret_cast<const uint2*>(p.h + static_cast<int64_t>(r) * kRank) + (lane & 3))
+                          : make_uint2(0, 0);
+                sample[i] = min(r, p.rows - 1) / p.rows_per_sample;
+            }
+        }
+    }
+};
+
+// The sums of 32 rows x 64 columns (c0 .. of the tile), scaled, with the bias: y[half][j][i] is row
+// 16 half + lane / 4 + 8 (i / 2), column 8 j + 2 (lane % 4) + i % 2.
+template <bool kF16, int kSize, int kExpand>
+__device__ __forceinline__ void scaled_sums(uint32_t tmem_acc, int c0, const RowRegs<kExpand>& rows,
+                                            const Columns<kSize, kExpand>* cols, float (&y)[2][8][4]) {
+    const int q = threadIdx.x & 3;
+    uint32_t acc[2][32];
+    tmem_ld_16x64(tmem_acc + c0, acc[0]);
+    tmem_ld_16x64(tmem_acc + (16u << 16) + c0, acc[1]);
+    tmem_wait_ld();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float2 s = *reinterpret_cast<const float2*>(&cols->scale[c0 + 8 * j + 2 * q]);
+        const uint32_t b = *reinterpret_cast<const uint32_t*>(&cols->bias[c0 + 8 * j + 2 * q]);
+        const float b0 = Act<kF16>::lo(b), b1 = Act<kF16>::hi(b);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                y[half][j][i] = fmaf(static_cast<float>(static_cast<int>(acc[half][4 * j + i])) * rows.sx[2 * half + (i >> 1)],
+                                     i & 1 ? s.y : s.x, i & 1 ? b1 : b0);
+    }
+}
+
+// 16 rows x 64 columns rounded into the warp's staging buffer (16 rows of 128 bytes, 16-byte unit u of
+// row r at u ^ (r & 7): no bank conflicts either way) and from there to global memory in whole
+// 128-byte lines.
+template <bool kF16>
+__device__ __forceinline__ void store_rows(const TileParams& tp, const float (&y)[8][4], int row0, int col0,
+                                           uint8_t* buf) {
+    const Params& p = tp.p;
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<uint32_t*>(buf + (g + 8 * i) * 128 + ((j ^ g) << 4) + 4 * q) =
+                Act<kF16>::pack(y[j][2 * i], y[j][2 * i + 1]);
+    __syncwarp();
+    const int col = col0 + 8 * (lane & 7);
+    uint4 v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int r = row0 + g + 8 * i;
-        const bool in = r < p.rows;
-        sx[i] = in ? __ldg(p.x_scale + r) : 0.0f;
-        h[i] = p.h && in ? __ldg(reinterpret_cast<const uint2*>(p.h + static_cast<int64_t>(r) * kRank) + q)
-                         : make_uint2(0, 0);
-        sample[i] = p.h ? min(r, p.rows - 1) / p.rows_per_sample : 0;
+        const int in = 4 * i + (lane >> 3);
+        v[i] = *reinterpret_cast<const uint4*>(buf + in * 128 + (((lane & 7) ^ (in & 7)) << 4));
     }
-    for (int c0 = 0; c0 < columns && n0 + c0 < p.n && row0 < p.rows; c0 += 32) {
-        uint32_t acc[2][16];
-        tmem_ld_16x32(tmem_acc + c0, acc[0]);
-        tmem_ld_16x32(tmem_acc + (16u << 16) + c0, acc[1]);
-        float sw[4][2], bias[4][2];
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int n = n0 + c0 + 8 * j + 2 * q + s;
-                sw[j][s] = n < p.n ? __ldg(p.w_scale + n) : 0.0f;
-                bias[j][s] = p.bias && n < p.n ? value_of<kF16>(__ldg(p.bias + n)) : 0.0f;
-            }
-        asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        if (n_st >= static_cast<uint32_t>(kEpiBufs)) {
-            if (lane == 0) bulk_wait_group_read<kEpiBufs - 1>();
-            __syncwarp();
-        }
-        uint8_t* buf = bufs + (n_st % kEpiBufs) * kEpiChunk;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            float y[4][4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    y[j][i] = fmaf(static_cast<float>(static_cast<int>(acc[half][4 * j + i])) * sx[2 * half + (i >> 1)],
-                                   sw[j][i & 1], bias[j][i & 1]);
-            if (p.h) {
-                // the samples of the 16 rows (one, unless a sample ends among them)
-                const int first = __shfl_sync(0xffffffffu, sample[2 * half], 0);
-                const int last = __shfl_sync(0xffffffffu, sample[2 * half + 1], 31);
-                for (int s = first; s <= last; ++s) {
-                    const bool lo = sample[2 * half] == s, hi = sample[2 * half + 1] == s;
-                    const uint32_t a[4] = {lo ? h[2 * half].x : 0u, hi ? h[2 * half + 1].x : 0u,
-                                           lo ? h[2 * half].y : 0u, hi ? h[2 * half + 1].y : 0u};
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int n = min(n0 + c0 + 8 * j + g, p.n - 1);
-                        const uint2 b = __ldg(reinterpret_cast<const uint2*>(
-                                                  p.b_dec + (static_cast<int64_t>(s) * p.n + n) * kRank) + q);
-                        mma_bf16_16816(y[j], a, b.x, b.y, y[j]);
-                    }
-                }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = 16 * half + g + 8 * i;      // staged row; 16-byte unit j at j ^ ((r >> 1) & 3)
-                    *reinterpret_cast<uint32_t*>(buf + r * 64 + ((j ^ ((r >> 1) & 3)) << 4) + 4 * q) =
-                        Act<kF16>::pack(y[j][2 * i], y[j][2 * i + 1]);
-                }
-        }
-        if (tp.tma_out) {
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-                tma_store_2d(tm_out, buf, n0 + c0, row0);
-                bulk_commit_group();
-            }
-            ++n_st;
+    for (int i = 0; i < 4; ++i) {
+        const int r = row0 + 4 * i + (lane >> 3);
+        if (r >= p.rows || col >= p.n) continue;
+        uint16_t* out = p.out + static_cast<int64_t>(r) * p.n + col;
+        if (tp.out16) {
+            *reinterpret_cast<uint4*>(out) = v[i];
         } else {
-            __syncwarp();
-            const int rows = min(32, p.rows - row0);
-            if (n0 + c0 + lane < p.n)
-                for (int r = 0; r < rows; ++r)
-                    p.out[static_cast<int64_t>(row0 + r) * p.n + n0 + c0 + lane] = *reinterpret_cast<uint16_t*>(
-                        buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + 2 * (lane & 7));
-            __syncwarp();
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (col + e < p.n) out[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
         }
     }
 }
 
-template <bool kPair, bool kF16>
+// kExpandMma: the expand of 32 rows x 64 columns onto y.
+template <int kSize>
+__device__ __forceinline__ void add_expand(const Params& p, int n0, int c0, int staged,
+                                           const RowRegs<kExpandMma>& rows, const Columns<kSize, kExpandMma>* cols,
+                                           float (&y)[2][8][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+    const uint2* factors = reinterpret_cast<const uint2*>(cols->factors);
+    // whether all 32 rows are the staged sample's
+    if (__all_sync(0xffffffffu, rows.sample[0] == staged && rows.sample[3] == staged)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint2 b = factors[(c0 + 8 * j + g) * 4 + q];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t a[4] = {rows.h[2 * half].x, rows.h[2 * half + 1].x, rows.h[2 * half].y,
+                                       rows.h[2 * half + 1].y};
+                mma_bf16_16816(y[half][j], a, b.x, b.y, y[half][j]);
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        // the samples of the 16 rows, one after the other
+        const int first = __shfl_sync(0xffffffffu, rows.sample[2 * half], 0);
+        const int last = __shfl_sync(0xffffffffu, rows.sample[2 * half + 1], 31);
+#pragma unroll 1
+        for (int s = first; s <= last; ++s) {
+            const bool lo = rows.sample[2 * half] == s, hi = rows.sample[2 * half + 1] == s;
+            const uint32_t a[4] = {lo ? rows.h[2 * half].x : 0u, hi ? rows.h[2 * half + 1].x : 0u,
+                                   lo ? rows.h[2 * half].y : 0u, hi ? rows.h[2 * half + 1].y : 0u};
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                uint2 b = factors[(c0 + 8 * j + g) * 4 + q];
+                if (s != staged) {
+                    const int n = min(n0 + c0 + 8 * j + g, p.n - 1);
+                    b = __ldg(reinterpret_cast<const uint2*>(p.b_dec + (static_cast<int64_t>(s) * p.n + n) * kRank) + q);
+                }
+                mma_bf16_16816(y[half][j], a, b.x, b.y, y[half][j]);
+            }
+        }
+    }
+}
+
+template <bool kPair, bool kF16, int kExpand>
 __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const CUtensorMap& tm_w,
-                                                 const CUtensorMap& tm_out, const TileParams& tp) {
+                                                 const CUtensorMap& tm_h, const CUtensorMap& tm_bd,
+                                                 const TileParams& tp) {
+    static_assert(kPair || kExpand != kExpandTmem, "the expand in TMEM is the pairs'");
     constexpr int kSize = kPair ? 256 : 128;               // rows and columns of a tile
     constexpr uint32_t kCols = 2 * kSize;                  // TMEM columns: two accumulators
+    using L = Layout<kSize, kExpand>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* epi_base = smem + kSmemStages;
-    Barriers* bars = reinterpret_cast<Barriers*>(smem + kSmemStages + kSmemEpi);
+    uint8_t* expand_base = smem + L::kExpandAt;
+    Columns<kSize, kExpand>* cols = reinterpret_cast<Columns<kSize, kExpand>*>(smem + L::kColumnsAt);
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + L::kBarriersAt);
     volatile int* abort = &bars->abort;
     int32_t* err = tp.p.err;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -452,12 +588,23 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
         for (int a = 0; a < 2; ++a) {
             mbar_init(&bars->tfull[a], 1);
             mbar_init(&bars->tempty[a], (kPair ? 2 : 1) * kEpiWarps);
+            mbar_init(&bars->lfull[a], 1);
+            mbar_init(&bars->lempty[a], 1);
         }
+        mbar_init(&bars->ereq, 2 * kEpiWarps);
+        mbar_init(&bars->efull, 1);
+        mbar_init(&bars->cfull, kEpiWarps);
+        mbar_init(&bars->cempty, kEpiWarps);
         mbar_init(&bars->done, 1);
+        mbar_init(&bars->edone, 1);
         bars->abort = 0;
         fence_mbar_init();
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_w);
+        if constexpr (kExpand == kExpandTmem) {
+            prefetch_tmap(&tm_h);
+            prefetch_tmap(&tm_bd);
+        }
     }
     if (warp == 1) {
         if constexpr (kPair) {
@@ -479,11 +626,22 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
     const uint32_t tmem = bars->tmem_base;
 
     if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer
         if (lane == 0) {
-            uint32_t it = 0;
-            for (int t = first; t < tp.total_tiles && !*abort; t += step) {
+            uint32_t it = 0, tile = 0;
+            for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
                 int m0, n0;
                 tile_of(tp, t, kSize, m0, n0);
+                if constexpr (kExpand == kExpandTmem) {
+                    const uint32_t b = tile & 1u, ph = (tile >> 1) & 1u;
+                    if (!mbar_wait(&bars->lempty[b], ph ^ 1u, abort, err)) break;
+                    if (leader) mbar_arrive_expect_tx(&bars->lfull[b], 2 * kExpandBytes);
+                    const uint32_t fb = map_to_rank(&bars->lfull[b], 0);
+                    uint8_t* l = expand_base + b * kExpandBytes;
+                    tma_load_2d_pair(l, &tm_h, fb, 0, m0 + kRows * rank);
+                    tma_load_2d_pair(l + kHBytes, &tm_bd, fb, 0,
+                                     m0 / tp.p.rows_per_sample * tp.p.n + n0 + kRows * rank);
+                }
                 for (int kb = 0; kb < nk; ++kb, ++it) {
                     const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
                     if (!mbar_wait(&bars->empty[s], ph ^ 1u, abort, err)) break;
@@ -503,6 +661,7 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
             if (*abort) drain_pause();
         }
     } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
         if (leader && lane == 0) {
             uint32_t it = 0, tile = 0;
             for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
@@ -533,32 +692,104 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
             if constexpr (kPair) umma_commit_pair_local(&bars->done);
             else umma_commit(&bars->done);                 // arrives once every MMA above has completed
         }
+    } else if (kExpand == kExpandTmem && warp == 2 + kEpiWarps) {
+        // ---------------------------------------------------------------- expand issuer
+        if (leader && lane == 0) {
+            uint32_t tile = 0;
+            for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
+                const uint32_t b = tile & 1u, ph = (tile >> 1) & 1u;
+                if (!mbar_wait(&bars->lfull[b], ph, abort, err)) break;
+                if (!mbar_wait(&bars->ereq, tile & 1u, abort, err)) break;
+                tc_fence_after();
+                const uint32_t l = smem_u32(expand_base + b * kExpandBytes);
+                umma_expand(tmem + b * kSize, desc_k_major(l, 32, 6), desc_k_major(l + kHBytes, 32, 6));
+                umma_commit_pair(&bars->efull);
+                umma_commit_pair(&bars->lempty[b]);
+            }
+            umma_commit_pair_local(&bars->edone);
+        }
     } else {
+        // ---------------------------------------------------------------- epilogue
         const int quarter = warp & 3;                      // TMEM lanes 32 * quarter .. + 31
-        uint8_t* bufs = epi_base + quarter * kEpiBufs * kEpiChunk;
-        uint32_t tempty[2] = {0, 0};
+        const int side = (warp - 2) >> 2;                  // which half of the columns
+        uint8_t* buf = smem + L::kOutAt + (warp - 2) * kEpiChunk;
+        uint32_t tempty[2] = {0, 0}, ereq = 0;
         if constexpr (kPair) {
             tempty[0] = map_to_rank(&bars->tempty[0], 0);
             tempty[1] = map_to_rank(&bars->tempty[1], 0);
+            ereq = map_to_rank(&bars->ereq, 0);
         }
-        uint32_t n_st = 0, tile = 0;
+        const int thread = threadIdx.x - 64, row_in = kRows * rank + 32 * quarter;
+        uint32_t tile = 0;
+        ColumnRegs<kSize, kExpand> next;
+        int m0 = 0, n0 = 0;
+        if (first < tp.total_tiles) {
+            tile_of(tp, first, kSize, m0, n0);
+            next.load(tp.p, m0 + kRows * rank, n0, thread);
+        }
         for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
-            int m0, n0;
-            tile_of(tp, t, kSize, m0, n0);
             const uint32_t acc = tile & 1u, aph = (tile >> 1) & 1u;
+            RowRegs<kExpand> rows;
+            rows.load(tp.p, m0 + row_in, lane);
+            const int staged =
+                kExpand == kExpandMma ? min(m0 + kRows * rank, tp.p.rows - 1) / tp.p.rows_per_sample : 0;
+            // every epilogue warp is done with the tile before's columns; then this one's are in place
+            if (!mbar_wait(&bars->cempty, (tile & 1u) ^ 1u, abort, err)) break;
+            next.store(cols, thread);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars->cfull);
+            const int row0 = m0 + row_in, col0 = n0;
+            if (t + step < tp.total_tiles) {
+                tile_of(tp, t + step, kSize, m0, n0);
+                next.load(tp.p, m0 + kRows * rank, n0, thread);
+            }
+            if (!mbar_wait(&bars->cfull, tile & 1u, abort, err)) break;
             if (!mbar_wait(&bars->tfull[acc], aph, abort, err)) break;
             tc_fence_after();
-            epilogue_tile<kF16>(tp, &tm_out, tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kSize, kSize,
-                                m0 + kRows * rank + 32 * quarter, n0, bufs, n_st);
+            const uint32_t tmem_acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kSize;
+            const int c_first = kSize / 2 * side;
+            if constexpr (kExpand == kExpandTmem) {
+                // (every warp takes part, those behind the last column too; the rows are whole tiles)
+#pragma unroll 1
+                for (int c0 = c_first; c0 < c_first + kSize / 2; c0 += 64) {
+                    float y[2][8][4];
+                    scaled_sums<kF16, kSize, kExpand>(tmem_acc, c0, rows, cols, y);
+                    tmem_st_16x64(tmem_acc + c0, y[0]);
+                    tmem_st_16x64(tmem_acc + (16u << 16) + c0, y[1]);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_remote_relaxed(ereq);
+                if (!mbar_wait(&bars->efull, tile & 1u, abort, err)) break;
+                tc_fence_after();
+            }
+#pragma unroll 1
+            for (int c0 = c_first; c0 < c_first + kSize / 2; c0 += 64) {
+                if (row0 >= tp.p.rows || col0 + c0 >= tp.p.n) break;
+                float y[2][8][4];
+                if constexpr (kExpand == kExpandTmem) {
+                    uint32_t e[2][32];
+                    tmem_ld_16x64(tmem_acc + c0, e[0]);
+                    tmem_ld_16x64(tmem_acc + (16u << 16) + c0, e[1]);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int j = 0; j < 64; ++j) y[j >> 5][(j >> 2) & 7][j & 3] = __uint_as_float(e[j >> 5][j & 31]);
+                } else {
+                    scaled_sums<kF16, kSize, kExpand>(tmem_acc, c0, rows, cols, y);
+                }
+                if constexpr (kExpand == kExpandMma) add_expand<kSize>(tp.p, col0, c0, staged, rows, cols, y);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) store_rows<kF16>(tp, y[half], row0 + 16 * half, col0 + c0, buf);
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) {
-                if constexpr (kPair) mbar_arrive_remote(tempty[acc]);
+                mbar_arrive(&bars->cempty);
+                if constexpr (kPair) mbar_arrive_remote_relaxed(tempty[acc]);
                 else mbar_arrive(&bars->tempty[acc]);
             }
         }
-        if (lane == 0) bulk_wait_group_all();              // the last stores have left shared memory
-        __syncwarp();
     }
 
     __syncthreads();
@@ -566,6 +797,9 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
         const uint64_t t0 = global_timer_ns();
         while (!mbar_try_wait(&bars->done, 0) && global_timer_ns() - t0 < 100000000ull) {
         }
+        if constexpr (kExpand == kExpandTmem)
+            while (!mbar_try_wait(&bars->edone, 0) && global_timer_ns() - t0 < 100000000ull) {
+            }
     }
     tc_fence_before();
     if constexpr (kPair) cluster_sync();                   // the pair's MMAs are done before either CTA frees anything
@@ -579,56 +813,63 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
     }
 }
 
-template <bool kF16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+template <bool kF16, int kExpand>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads<kExpand>, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_w,
-                     const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ TileParams tp) {
-    tile_kernel_body<true, kF16>(tm_q, tm_w, tm_out, tp);
+                     const __grid_constant__ CUtensorMap tm_h, const __grid_constant__ CUtensorMap tm_bd,
+                     const __grid_constant__ TileParams tp) {
+    tile_kernel_body<true, kF16, kExpand>(tm_q, tm_w, tm_h, tm_bd, tp);
 }
 
-template <bool kF16>
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool kF16, int kExpand>
+__global__ void __launch_bounds__(kThreads<kExpand>, 1)
     int8_tile_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_w,
-                     const __grid_constant__ CUtensorMap tm_out, const __grid_constant__ TileParams tp) {
-    tile_kernel_body<false, kF16>(tm_q, tm_w, tm_out, tp);
+                     const __grid_constant__ TileParams tp) {
+    tile_kernel_body<false, kF16, kExpand>(tm_q, tm_w, tm_q, tm_q, tp);
 }
 
-template <bool kF16>
-int32_t launch_tiles(const Params& p, int device, int sms, bool pair, cudaStream_t st) {
-    CUtensorMap tm_q, tm_w, tm_out;
+template <bool kPair, bool kF16, int kExpand>
+int32_t launch_tiles(const Params& p, int device, int sms, cudaStream_t st) {
+    constexpr int kSize = kPair ? 256 : 128;
+    constexpr int kBytes = Layout<kSize, kExpand>::kBytes;
+    CUtensorMap tm_q, tm_w, tm_h, tm_bd;
     int32_t rc = encode_u8_2d(&tm_q, p.q, p.k, p.rows, p.q_stride, kBK, kRows);
     if (rc != LITHE_OK) return rc;
     if ((rc = encode_u8_2d(&tm_w, p.w, p.k, p.n, p.w_stride, kBK, kRows)) != LITHE_OK) return rc;
+    if constexpr (kExpand == kExpandTmem) {
+        if ((rc = encode_bf16_2d(&tm_h, p.h, kRank, p.rows, kRank, kRows, 32)) != LITHE_OK) return rc;
+        if ((rc = encode_bf16_2d(&tm_bd, p.b_dec, kRank, static_cast<uint64_t>(p.rows / p.rows_per_sample) * p.n, kRank,
+                                 kRows, 32)) != LITHE_OK)
+            return rc;
+    }
     TileParams tp{};
     tp.p = p;
-    tp.tma_out = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-    // the map's element type only has to have 16 bits
-    if (tp.tma_out) {
-        if ((rc = encode_bf16_2d(&tm_out, p.out, p.n, p.rows, 32, 32, 64)) != LITHE_OK) return rc;
-    } else {
-        tm_out = tm_q;
-    }
-    const int size = pair ? 256 : 128;
-    tp.m_tiles = (p.rows + size - 1) / size;
-    tp.n_tiles = (p.n + size - 1) / size;
+    tp.out16 = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+    tp.m_tiles = (p.rows + kSize - 1) / kSize;
+    tp.n_tiles = (p.n + kSize - 1) / kSize;
     const int64_t tiles = static_cast<int64_t>(tp.m_tiles) * tp.n_tiles;
     if (tiles > 0x7fffffffLL - 0x10000) return fail_arg("too many tiles");
     tp.total_tiles = static_cast<int32_t>(tiles);
     static bool configured[64] = {false};
-    if (!configured[device]) {
-        cudaError_t e = cudaFuncSetAttribute(int8_pair_kernel<kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             kSmemBytes);
-        if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(int8_tile_kernel<kF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-        if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(int8 tile kernels)");
-        configured[device] = true;
-    }
-    if (pair) {
+    if constexpr (kPair) {
+        if (!configured[device]) {
+            const cudaError_t e = cudaFuncSetAttribute(int8_pair_kernel<kF16, kExpand>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+            if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(int8_pair_kernel)");
+            configured[device] = true;
+        }
         const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
-        int8_pair_kernel<kF16><<<static_cast<int>(2 * pairs), kThreads, kSmemBytes, st>>>(tm_q, tm_w, tm_out, tp);
+        int8_pair_kernel<kF16, kExpand>
+            <<<static_cast<int>(2 * pairs), kThreads<kExpand>, kBytes, st>>>(tm_q, tm_w, tm_h, tm_bd, tp);
     } else {
+        if (!configured[device]) {
+            const cudaError_t e = cudaFuncSetAttribute(int8_tile_kernel<kF16, kExpand>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+            if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(int8_tile_kernel)");
+            configured[device] = true;
+        }
         const int grid = static_cast<int>(tiles < sms ? tiles : sms);
-        int8_tile_kernel<kF16><<<grid, kThreads, kSmemBytes, st>>>(tm_q, tm_w, tm_out, tp);
+        int8_tile_kernel<kF16, kExpand><<<grid, kThreads<kExpand>, kBytes, st>>>(tm_q, tm_w, tp);
     }
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "int8 tile kernel launch");
@@ -644,7 +885,17 @@ int32_t launch_linear(const Params& p, cudaStream_t st) {
     if (rc != LITHE_OK) return rc;
     // Pairs once their 256 x 256 tiles fill the GPU; 128 x 128 tiles before, to use more SMs.
     const int64_t pair_tiles = static_cast<int64_t>((p.rows + 255) / 256) * ((p.n + 255) / 256);
-    return launch_tiles<kF16>(p, device, sms, pair_tiles >= sms / 2, st);
+    const bool pair = pair_tiles >= sms / 2;
+    if constexpr (!kF16) {
+        // b_dec's rows are TMA coordinates, 32-bit
+        const int64_t factor_rows = p.h ? static_cast<int64_t>(p.rows / p.rows_per_sample) * p.n : 0;
+        if (p.h && pair && p.rows_per_sample % 256 == 0 && factor_rows < 0x7fffffffLL - 256)
+            return launch_tiles<true, kF16, kExpandTmem>(p, device, sms, st);
+        if (p.h) return pair ? launch_tiles<true, kF16, kExpandMma>(p, device, sms, st)
+                             : launch_tiles<false, kF16, kExpandMma>(p, device, sms, st);
+    }
+    return pair ? launch_tiles<true, kF16, kExpandNone>(p, device, sms, st)
+                : launch_tiles<false, kF16, kExpandNone>(p, device, sms, st);
 }
 
 template <bool kF16>

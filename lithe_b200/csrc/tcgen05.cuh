@@ -100,6 +100,12 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
+// The same without release: for an arrival that hands on no memory the thread has written (an
+// accumulator it has read and waited for), where a release would wait for its global stores.
+__device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_addr) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // Bounded pause used on the abort path, so loads already issued land before shared memory
 // is released.
 __device__ __forceinline__ void drain_pause() {

@@ -128,7 +128,10 @@ def test_linear(rows, n, k, dtype):
 
 @pytest.mark.parametrize("samples,rps,n,k", [(1, 1, 16, 64), (14, 1, 264, 128), (5, 3, 100, 130), (2, 16, 256, 64), (3, 24, 40, 96),
                                              (3, 100, 520, 256), (2, 128, 1091, 128), (7, 37, 256, 320), (4, 256, 512, 128),
-                                             (14, 512, 768, 64), (2, 1000, 264, 100), (300, 1, 64, 64), (130, 5, 72, 64)])
+                                             (14, 512, 768, 64), (2, 1000, 264, 100), (300, 1, 64, 64), (130, 5, 72, 64),
+                                             (14, 256, 1536, 3072), (8, 1024, 1032, 320), (3, 2560, 1091, 1000),
+                                             (2, 768, 3592, 520), (1, 7168, 712, 128), (5, 1280, 3000, 136),
+                                             (5, 1000, 2000, 136), (20, 300, 1096, 1000)])
 def test_expand(samples, rps, n, k):
     bf = torch.bfloat16
     x = make((samples, rps, k), bf, 1)
