@@ -412,6 +412,21 @@ LITHE_API int32_t lithe_int8_linear(const void* q, int64_t q_stride, const float
                         int32_t rows, int32_t n, int32_t k, const void* h, const void* b_dec,
                         int32_t rows_per_sample, int32_t rank, int32_t* err_flag, void* stream);
 
+/* Bytes of device workspace lithe_int8_linear_dynamic needs: rows * (k rounded up to 16) + 4 * rows. */
+LITHE_API int64_t lithe_int8_workspace_bytes(int32_t rows, int32_t k);
+
+/*
+ * lithe_quantize_rows and lithe_int8_linear in one call: the same results, with the second launch's
+ * start overlapping the first kernel.
+ *   x            device (rows, k) of dtype, rows x_stride elements apart
+ *   workspace    device, 16-byte aligned, >= lithe_int8_workspace_bytes(rows, k); contents on entry do
+ *                not matter; calls sharing one workspace must be ordered on one stream
+ */
+LITHE_API int32_t lithe_int8_linear_dynamic(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
+                        const float* w_scale, const void* bias, void* out, int32_t dtype, int32_t rows, int32_t n,
+                        int32_t k, const void* h, const void* b_dec, int32_t rows_per_sample, int32_t rank,
+                        int32_t* err_flag, void* workspace, int64_t workspace_bytes, void* stream);
+
 /*
  * Self-test of the bounded pipeline wait (no counterpart in the reference): one warp waits on
  * an mbarrier that nothing arrives at.  After the wait's time limit (4 s) it ORs

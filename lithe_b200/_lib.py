@@ -81,6 +81,11 @@ _SIGNATURES.update({
         _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p,
         _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32,
         _c.c_void_p, _c.c_void_p]),
+    "lithe_int8_workspace_bytes": (_c.c_int64, [_c.c_int32, _c.c_int32]),
+    "lithe_int8_linear_dynamic": (_c.c_int32, [
+        _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int32,
+        _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_void_p,
+        _c.c_void_p, _c.c_int64, _c.c_void_p]),
     "lithe_rotate_axes": (_c.c_int32, [
         _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p,
         _c.c_int32, _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),

@@ -100,6 +100,7 @@ __device__ __forceinline__ uint2 quantize8(const uint4& v, float pre, float r) {
 
 template <bool kF16, int kChunks>
 __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int64_t row = blockIdx.x;
     const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_stride);
     uint2* q = reinterpret_cast<uint2*>(p.q + row * p.q_stride);
@@ -127,6 +128,7 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p
 
 template <bool kF16>
 __global__ void __launch_bounds__(kThreadsQ) quantize_any_kernel(const QuantParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int64_t row = blockIdx.x;
     const uint16_t* x = p.x + row * p.x_stride;
     int8_t* q = p.q + row * p.q_stride;
@@ -166,44 +168,109 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes of a row at k0; bytes from k on are zeros.
+// 16 bytes of a row at k0; bytes from k on are zeros.  kStream: read once, kept out of L1.
+template <bool kStream>
 __device__ __forceinline__ uint4 load16(const int8_t* row, int k0, int k) {
-    if (k0 + 16 <= k) return __ldg(reinterpret_cast<const uint4*>(row + k0));
+    if (k0 + 16 <= k) {
+        if (!kStream) return __ldg(reinterpret_cast<const uint4*>(row + k0));
+        uint4 v;
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                     : "l"(row + k0));
+        return v;
+    }
     uint32_t w[4] = {0, 0, 0, 0};
     for (int i = 0; k0 + i < k && i < 16; ++i)
         w[i >> 2] |= static_cast<uint32_t>(static_cast<uint8_t>(row[k0 + i])) << (8 * (i & 3));
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Few rows: the weights' bytes are the work.  A CTA takes 16 output channels and 8 kTiles rows;
-// its 8 warps take every 8th piece of 64 k's, so that the channels' rows are read by many warps
-// at once, and add their int32 sums at the end.  Inside a piece a lane reads 16 contiguous bytes
-// of a row and uses its four words as the k's of two MMAs: the same bijection of k for weights
-// and activations, so the sums stand.
-constexpr int kWarpsR = 8;
-constexpr int kUnroll = 4;         // pieces a warp loads before it uses the first
+// y + the expand of one output.
+__device__ __forceinline__ float expand_of(const Params& p, int r, int n, float y) {
+    const uint32_t* hr = reinterpret_cast<const uint32_t*>(p.h + static_cast<int64_t>(r) * kRank);
+    const int64_t at = static_cast<int64_t>(r / p.rows_per_sample) * p.n + n;
+    const uint32_t* br = reinterpret_cast<const uint32_t*>(p.b_dec + at * kRank);
+#pragma unroll
+    for (int j = 0; j < kRank / 2; ++j) {
+        const uint32_t hv = __ldg(hr + j), bv = __ldg(br + j);
+        y = fmaf(bf16lo_to_f32(hv), bf16lo_to_f32(bv), y);
+        y = fmaf(bf16hi_to_f32(hv), bf16hi_to_f32(bv), y);
+    }
+    return y;
+}
+
+// The linear's kernels may start while the quantisation of their activations runs (it lets them at its
+// start): they wait here before they read what it writes.  What ran before it has completed by then,
+// since it was launched in stream order.  Returns at once in a launch that depends on nothing so.
+__device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+struct Launch {
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute attrs[2];
+    Launch(int grid, int threads, size_t smem, cudaStream_t st) {
+        config.gridDim = dim3(grid);
+        config.blockDim = dim3(threads);
+        config.dynamicSmemBytes = smem;
+        config.stream = st;
+        config.attrs = attrs;
+    }
+    Launch(const Launch&) = delete;
+    void after_last() {
+        attrs[config.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attrs[config.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    void clusters_of(int n) {
+        attrs[config.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attrs[config.numAttrs].val.clusterDim.x = n;
+        attrs[config.numAttrs].val.clusterDim.y = 1;
+        attrs[config.numAttrs++].val.clusterDim.z = 1;
+    }
+};
+
+// Few rows (at most 16): the weights' bytes are the work.  A CTA takes 16 output channels and all the
+// rows (8 kTiles); its warps take turns at pieces of 128 k's and add their int32 sums at the end.
+// Inside a piece a lane reads 16 contiguous bytes of a row and uses its four words as the k's of
+// two MMAs: the same bijection of k for weights and activations, so the sums stand.  Both halves of
+// a 128-byte line are one warp's (64-byte pieces: 15% slower).  As many warps share a channel tile
+// as fill the SMs once, 32 a SM of 64 registers: one wave, all of it loading from the start.
+// Measured: 14 x 3072 -> 18432 13.4 us (4.2 TB/s), 3 x 15360 -> 3072 12.6 us, 3072 -> 3072 4.7 us (fixed costs).
+// Rings of cp.async and activations held in registers or shared memory by persistent CTAs were
+// no faster (14 to 22 us).
+constexpr int kMaxSplit = 16;                  // warps that share a channel tile
+constexpr int kRowWarps = 32;                  // per SM
+constexpr int kUnroll = 2;                     // 64-byte pieces a warp loads before it uses the first
 
 template <bool kF16, int kTiles>
-__global__ void __launch_bounds__(32 * kWarpsR) int8_rows_kernel(const Params p) {
-    __shared__ int part[kWarpsR][8 * kTiles][17];
+__global__ void __launch_bounds__(32 * kMaxSplit, 2) int8_rows_kernel(const Params p) {
+    extern __shared__ int part_raw[];
+    int(*part)[8 * kTiles][17] = reinterpret_cast<int(*)[8 * kTiles][17]>(part_raw);   // [warp][row][channel]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, kq = 16 * (lane & 3);
-    const int n0 = blockIdx.x * 16, r0 = blockIdx.y * 8 * kTiles;
+    const int split = blockDim.x >> 5, n0 = blockIdx.x * 16;
     const int8_t* w0 = p.w + static_cast<int64_t>(n0 + g) * p.w_stride;
     const int8_t* w1 = w0 + 8 * p.w_stride;
     const bool in0 = n0 + g < p.n, in1 = n0 + g + 8 < p.n;
     int acc[kTiles][4] = {};
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    for (int k0 = 64 * warp; k0 < p.k; k0 += 64 * kWarpsR * kUnroll) {
+    bool waited = false;
+    for (int k0 = 128 * warp; k0 < p.k; k0 += 128 * split) {
         uint4 a0[kUnroll], a1[kUnroll], b[kUnroll][kTiles];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
-            const int k = k0 + 64 * kWarpsR * u + kq;
-            a0[u] = in0 && k < p.k ? load16(w0, k, p.k) : zero;
-            a1[u] = in1 && k < p.k ? load16(w1, k, p.k) : zero;
+            const int k = k0 + 64 * u + kq;
+            a0[u] = in0 && k < p.k ? load16<true>(w0, k, p.k) : zero;
+            a1[u] = in1 && k < p.k ? load16<true>(w1, k, p.k) : zero;
+        }
+        if (!waited) {                         // the first weights are on their way while the quantisation ends
+            grid_dependency_wait();
+            waited = true;
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int k = k0 + 64 * u + kq;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) {
-                const int r = r0 + 8 * t + g;
-                b[u][t] = r < p.rows && k < p.k ? load16(p.q + r * p.q_stride, k, p.k) : zero;
+                const int r = 8 * t + g;
+                b[u][t] = r < p.rows && k < p.k ? load16<false>(p.q + r * p.q_stride, k, p.k) : zero;
             }
         }
 #pragma unroll
@@ -214,40 +281,35 @@ __global__ void __launch_bounds__(32 * kWarpsR) int8_rows_kernel(const Params p)
                 mma_s8(acc[t], a0[u].z, a1[u].z, a0[u].w, a1[u].w, b[u][t].z, b[u][t].w);
             }
     }
+    grid_dependency_wait();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i)        // element i: channel g + 8 (i / 2), row 2 (lane % 4) + i % 2
             part[warp][8 * t + 2 * (lane & 3) + (i & 1)][g + 8 * (i >> 1)] = acc[t][i];
     __syncthreads();
-    for (int e = threadIdx.x; e < 16 * 8 * kTiles; e += 32 * kWarpsR) {
-        const int r = r0 + (e >> 4), n = n0 + (e & 15);
+    for (int e = threadIdx.x; e < 16 * 8 * kTiles; e += blockDim.x) {
+        const int r = e >> 4, n = n0 + (e & 15);
         if (r >= p.rows || n >= p.n) continue;
         int sum = 0;
-#pragma unroll
-        for (int i = 0; i < kWarpsR; ++i) sum += part[i][e >> 4][e & 15];
-        float y = static_cast<float>(sum) * p.x_scale[r] * p.w_scale[n];
-        if (p.bias) y += value_of<kF16>(p.bias[n]);
-        if (p.h) {
-            const uint32_t* hr = reinterpret_cast<const uint32_t*>(p.h + static_cast<int64_t>(r) * kRank);
-            const int64_t at = static_cast<int64_t>(r / p.rows_per_sample) * p.n + n;
-            const uint32_t* br = reinterpret_cast<const uint32_t*>(p.b_dec + at * kRank);
-#pragma unroll
-            for (int j = 0; j < kRank / 2; ++j) {
-                const uint32_t hv = __ldg(hr + j), bv = __ldg(br + j);
-                y = fmaf(bf16lo_to_f32(hv), bf16lo_to_f32(bv), y);
-                y = fmaf(bf16hi_to_f32(hv), bf16hi_to_f32(bv), y);
-            }
-        }
+        for (int i = 0; i < split; ++i) sum += part[i][r][e & 15];
+        float y = fmaf(static_cast<float>(sum) * p.x_scale[r], p.w_scale[n], p.bias ? value_of<kF16>(p.bias[n]) : 0.0f);
+        if (p.h) y = expand_of(p, r, n, y);
         p.out[static_cast<int64_t>(r) * p.n + n] = static_cast<uint16_t>(Act<kF16>::pack(y, 0.0f) & 0xffffu);
     }
 }
 
 template <bool kF16, int kTiles>
-int32_t launch_rows(const Params& p, cudaStream_t st) {
-    const dim3 grid((p.n + 15) / 16, (p.rows + 8 * kTiles - 1) / (8 * kTiles));
-    int8_rows_kernel<kF16, kTiles><<<grid, 32 * kWarpsR, 0, st>>>(p);
-    const cudaError_t e = cudaGetLastError();
+int32_t launch_rows(const Params& p, int sms, bool after_quantize, cudaStream_t st) {
+    const int tiles = (p.n + 15) / 16, pairs = (p.k + 127) / 128;
+    int split = static_cast<int>(static_cast<int64_t>(sms) * kRowWarps / tiles);
+    split = split < 1 ? 1 : split > kMaxSplit ? kMaxSplit : split;
+    split = split < pairs ? split : pairs;
+    const int share = (pairs + split - 1) / split;
+    split = (pairs + share - 1) / share;           // no more warps than their share of the pieces needs
+    Launch l(tiles, 32 * split, split * 8 * kTiles * 17 * sizeof(int), st);
+    if (after_quantize) l.after_last();
+    const cudaError_t e = cudaLaunchKernelEx(&l.config, int8_rows_kernel<kF16, kTiles>, p);
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "int8_rows_kernel launch");
 }
 
@@ -278,6 +340,12 @@ int32_t launch_rows(const Params& p, cudaStream_t st) {
 // Measured without an expand: 14336 x 3072 -> 12288 2.8 POP/s, x 768 -> 12288 130 us (an epilogue of 4
 // warps with a TMA store of 64-byte rows: 257 us).  In a tile the stages' bytes (64 KB a pair and
 // 128 k's) keep shared memory as busy as the products keep the tensor pipe.
+// Too few 128 x 128 tiles for the SMs: a cluster of `split` CTAs takes one, each a run of its k's.  Their
+// int32 sums go through shared memory, where each CTA adds the others' for its share of the rows (an
+// exact sum, so the split does not show in the result) and finishes them.  A CTA takes in about 60
+// bytes a cycle, 0.3 us a stage of a 128 x 128 tile, and the exchange costs 4 us: 32 x 12288 -> 3072
+// takes 15.2 us on clusters of 4 and 31.0 us on single CTAs, 128 x 3072 -> 3072 (24 stages) 11.7 and 11.6,
+// 256 x 1024 -> 1024 (8 stages) 9.4 and 6.4; clusters of 8 took 4 us more to start.
 // Every mbarrier wait is bounded (4 s, LITHE_DEVERR_TIMEOUT, shared abort flag).
 enum Expand { kExpandNone, kExpandMma, kExpandTmem };
 
@@ -331,6 +399,7 @@ struct TileParams {
     Params p;
     int32_t m_tiles, n_tiles, total_tiles;
     int32_t out16;                 // the result's rows are 16-byte aligned
+    int32_t split;                 // single CTAs: CTAs of a cluster that share a tile's k
 };
 
 // Instruction descriptor of tcgen05.mma kind::i8: int32 accumulator (bits 4-5 = 2), signed A and B
@@ -491,27 +560,33 @@ __device__ __forceinline__ void store_rows(const TileParams& tp, const float (&y
             *reinterpret_cast<uint32_t*>(buf + (g + 8 * i) * 128 + ((j ^ g) << 4) + 4 * q) =
                 Act<kF16>::pack(y[j][2 * i], y[j][2 * i + 1]);
     __syncwarp();
-    const int col = col0 + 8 * (lane & 7);
-    uint4 v[4];
+    if (tp.out16) {
+        const int col = col0 + 8 * (lane & 7);
+        uint4 v[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int in = 4 * i + (lane >> 3);
-        v[i] = *reinterpret_cast<const uint4*>(buf + in * 128 + (((lane & 7) ^ (in & 7)) << 4));
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = row0 + 4 * i + (lane >> 3);
-        if (r >= p.rows || col >= p.n) continue;
-        uint16_t* out = p.out + static_cast<int64_t>(r) * p.n + col;
-        if (tp.out16) {
-            *reinterpret_cast<uint4*>(out) = v[i];
-        } else {
-            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                if (col + e < p.n) out[e] = static_cast<uint16_t>(w[e >> 1] >> (16 * (e & 1)));
+        for (int i = 0; i < 4; ++i) {
+            const int in = 4 * i + (lane >> 3);
+            v[i] = *reinterpret_cast<const uint4*>(buf + in * 128 + (((lane & 7) ^ (in & 7)) << 4));
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row0 + 4 * i + (lane >> 3);
+            if (r < p.rows && col < p.n)
+                *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(r) * p.n + col) = v[i];
+        }
+    } else {
+        // rows off the 16-byte boundaries: a column a lane, 64 bytes of a row at a time
+#pragma unroll 4
+        for (int in = 0; in < 16; ++in) {
+            uint16_t* out = p.out + static_cast<int64_t>(row0 + in) * p.n + col0;
+#pragma unroll
+            for (int c = lane; c < 64; c += 32) {
+                const uint16_t v = *reinterpret_cast<const uint16_t*>(buf + in * 128 + (((c >> 3) ^ (in & 7)) << 4) + 2 * (c & 7));
+                if (row0 + in < p.rows && col0 + c < p.n) out[c] = v;
+            }
+        }
+        __syncwarp();
     }
 }
 
@@ -559,6 +634,83 @@ __device__ __forceinline__ void add_expand(const Params& p, int n0, int c0, int 
     }
 }
 
+constexpr int kSumPitch = 132;                 // ints between the rows of a tile's sums in shared memory
+
+// A warp's 32 rows x 64 columns of a split tile's sums to shared memory (the stages' place: every load
+// and every product of the tile has completed).
+__device__ __forceinline__ void keep_sums(uint32_t tmem_acc, int* sums) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        uint32_t acc[32];
+        tmem_ld_16x64(tmem_acc + (static_cast<uint32_t>(16 * half) << 16), acc);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<uint2*>(sums + (16 * half + g + 8 * i) * kSumPitch + 8 * j + 2 * q) =
+                    make_uint2(acc[4 * j + 2 * i], acc[4 * j + 2 * i + 1]);
+    }
+}
+
+__device__ __forceinline__ uint4 ld_cluster(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "r"(addr)
+                 : "memory");
+    return v;
+}
+
+// This CTA's share of the tile's rows, the cluster's sums of them added and finished: 8 columns a
+// thread at a time.
+constexpr int kSplits = 4;                     // most CTAs of a cluster
+constexpr int kSplitStages = 24;               // fewest stages of a tile that is split
+template <bool kF16, int kSize, int kExpand>
+__device__ __forceinline__ void finish_sums(const TileParams& tp, const uint8_t* smem,
+                                            const Columns<kSize, kExpand>* cols, int part, int m0, int n0) {
+    const Params& p = tp.p;
+    const int tasks = min(kSize, p.rows - m0) * (kSize / 8);
+    const int end = tasks * (part + 1) / tp.split;
+    for (int e = tasks * part / tp.split + threadIdx.x; e < end; e += blockDim.x) {
+        const int in = e / (kSize / 8), c = 8 * (e % (kSize / 8));             // row of the tile, first column
+        const int r = m0 + in, n = n0 + c;
+        if (n >= p.n) continue;
+        const float sx = __ldg(p.x_scale + r);
+        uint4 a[kSplits][2];
+#pragma unroll
+        for (int s = 0; s < kSplits; ++s) {
+            const uint32_t at = map_to_rank(smem + (in * kSumPitch + c) * 4, s < tp.split ? s : 0);
+            a[s][0] = s < tp.split ? ld_cluster(at) : make_uint4(0, 0, 0, 0);
+            a[s][1] = s < tp.split ? ld_cluster(at + 16) : make_uint4(0, 0, 0, 0);
+        }
+        uint32_t sum[8] = {};
+#pragma unroll
+        for (int s = 0; s < kSplits; ++s) {
+            sum[0] += a[s][0].x, sum[1] += a[s][0].y, sum[2] += a[s][0].z, sum[3] += a[s][0].w;
+            sum[4] += a[s][1].x, sum[5] += a[s][1].y, sum[6] += a[s][1].z, sum[7] += a[s][1].w;
+        }
+        float y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            y[i] = fmaf(static_cast<float>(static_cast<int>(sum[i])) * sx, cols->scale[c + i], value_of<kF16>(cols->bias[c + i]));
+            if (kExpand == kExpandMma) y[i] = expand_of(p, r, min(n + i, p.n - 1), y[i]);
+        }
+        const uint4 v = make_uint4(Act<kF16>::pack(y[0], y[1]), Act<kF16>::pack(y[2], y[3]),
+                                   Act<kF16>::pack(y[4], y[5]), Act<kF16>::pack(y[6], y[7]));
+        uint16_t* out = p.out + static_cast<int64_t>(r) * p.n + n;
+        if (tp.out16) {
+            *reinterpret_cast<uint4*>(out) = v;
+        } else {
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (n + i < p.n) out[i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+        }
+    }
+}
+
 template <bool kPair, bool kF16, int kExpand>
 __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const CUtensorMap& tm_w,
                                                  const CUtensorMap& tm_h, const CUtensorMap& tm_bd,
@@ -577,8 +729,11 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = kPair ? static_cast<int>(cluster_rank()) : 0;
     const bool leader = rank == 0;
-    const int nk = (tp.p.k + kBK - 1) / kBK;
-    const int first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
+    const int group = kPair ? 2 : tp.split;                // CTAs of a tile
+    const int first = blockIdx.x / group, step = gridDim.x / group;
+    // this CTA's stages of a tile
+    const int stages = (tp.p.k + kBK - 1) / kBK, part = kPair || group == 1 ? 0 : static_cast<int>(cluster_rank());
+    const int kb0 = kPair ? 0 : stages * part / group, nk = kPair ? stages : stages * (part + 1) / group - kb0;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -628,6 +783,7 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         if (lane == 0) {
+            grid_dependency_wait();
             uint32_t it = 0, tile = 0;
             for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
                 int m0, n0;
@@ -653,8 +809,8 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
                         tma_load_2d_pair(a + kBox, &tm_w, fb, kb * kBK, n0 + kRows * rank);
                     } else {
                         mbar_arrive_expect_tx(&bars->full[s], 2 * kBox);
-                        tma_load_2d(a, &tm_q, &bars->full[s], kb * kBK, m0);
-                        tma_load_2d(a + kBox, &tm_w, &bars->full[s], kb * kBK, n0);
+                        tma_load_2d(a, &tm_q, &bars->full[s], (kb0 + kb) * kBK, m0);
+                        tma_load_2d(a + kBox, &tm_w, &bars->full[s], (kb0 + kb) * kBK, n0);
                     }
                 }
             }
@@ -663,27 +819,27 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer
         if (leader && lane == 0) {
-            uint32_t it = 0, tile = 0;
+            uint32_t s = 0, ph = 0, tile = 0;
+            const uint64_t base = desc_k_major(smem_u32(smem), 128, 2);
             for (int t = first; t < tp.total_tiles && !*abort; t += step, ++tile) {
                 const uint32_t acc = tile & 1u, aph = (tile >> 1) & 1u;
                 if (!mbar_wait(&bars->tempty[acc], aph ^ 1u, abort, err)) break;
                 tc_fence_after();
                 const uint32_t d = tmem + acc * kSize;
                 bool ok = true;
-                for (int kb = 0; kb < nk; ++kb, ++it) {
-                    const uint32_t s = it % kStages, ph = (it / kStages) & 1u;
+                for (int kb = 0; kb < nk; ++kb) {
                     if (!mbar_wait(&bars->full[s], ph, abort, err)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint32_t a = smem_u32(smem + s * 2 * kBox);
-                    const uint64_t ad = desc_k_major(a, 128, 2), bd = desc_k_major(a + kBox, 128, 2);
+                    const uint64_t ad = base + s * (2 * kBox >> 4), bd = ad + (kBox >> 4);
 #pragma unroll
                     for (int kk = 0; kk < kBK / 32; ++kk)  // +32 bytes along k inside the 128-byte swizzle atom
                         umma_i8<kPair>(d, ad + 2 * kk, bd + 2 * kk, (kb | kk) != 0);
                     if constexpr (kPair) umma_commit_pair(&bars->empty[s]);
                     else umma_commit(&bars->empty[s]);
+                    if (++s == kStages) s = 0, ph ^= 1u;
                 }
                 if (!ok) break;
                 if constexpr (kPair) umma_commit_pair(&bars->tfull[acc]);
@@ -710,6 +866,7 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
         }
     } else {
         // ---------------------------------------------------------------- epilogue
+        grid_dependency_wait();
         const int quarter = warp & 3;                      // TMEM lanes 32 * quarter .. + 31
         const int side = (warp - 2) >> 2;                  // which half of the columns
         uint8_t* buf = smem + L::kOutAt + (warp - 2) * kEpiChunk;
@@ -748,6 +905,10 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
             tc_fence_after();
             const uint32_t tmem_acc = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * kSize;
             const int c_first = kSize / 2 * side;
+            if (!kPair && group > 1) {
+                keep_sums(tmem_acc + c_first, reinterpret_cast<int*>(smem) + (32 * quarter) * kSumPitch + c_first);
+                break;                                     // (one tile a cluster)
+            }
             if constexpr (kExpand == kExpandTmem) {
                 // (every warp takes part, those behind the last column too; the rows are whole tiles)
 #pragma unroll 1
@@ -793,6 +954,13 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
     }
 
     __syncthreads();
+    if (!kPair && group > 1) {
+        cluster_sync();                                    // every CTA's sums are in place
+        int m0, n0;
+        tile_of(tp, first, kSize, m0, n0);
+        finish_sums<kF16, kSize, kExpand>(tp, smem, cols, part, m0, n0);
+        cluster_sync();                                    // no CTA leaves while its sums are read
+    }
     if (leader && warp == 1 && lane == 0) {
         const uint64_t t0 = global_timer_ns();
         while (!mbar_try_wait(&bars->done, 0) && global_timer_ns() - t0 < 100000000ull) {
@@ -829,7 +997,7 @@ __global__ void __launch_bounds__(kThreads<kExpand>, 1)
 }
 
 template <bool kPair, bool kF16, int kExpand>
-int32_t launch_tiles(const Params& p, int device, int sms, cudaStream_t st) {
+int32_t launch_tiles(const Params& p, int device, int sms, bool after_quantize, cudaStream_t st) {
     constexpr int kSize = kPair ? 256 : 128;
     constexpr int kBytes = Layout<kSize, kExpand>::kBytes;
     CUtensorMap tm_q, tm_w, tm_h, tm_bd;
@@ -850,52 +1018,59 @@ int32_t launch_tiles(const Params& p, int device, int sms, cudaStream_t st) {
     const int64_t tiles = static_cast<int64_t>(tp.m_tiles) * tp.n_tiles;
     if (tiles > 0x7fffffffLL - 0x10000) return fail_arg("too many tiles");
     tp.total_tiles = static_cast<int32_t>(tiles);
+    const auto kernel = [] {
+        if constexpr (kPair) return int8_pair_kernel<kF16, kExpand>;
+        else return int8_tile_kernel<kF16, kExpand>;
+    }();
     static bool configured[64] = {false};
-    if constexpr (kPair) {
-        if (!configured[device]) {
-            const cudaError_t e = cudaFuncSetAttribute(int8_pair_kernel<kF16, kExpand>,
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-            if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(int8_pair_kernel)");
-            configured[device] = true;
-        }
-        const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
-        int8_pair_kernel<kF16, kExpand>
-            <<<static_cast<int>(2 * pairs), kThreads<kExpand>, kBytes, st>>>(tm_q, tm_w, tm_h, tm_bd, tp);
-    } else {
-        if (!configured[device]) {
-            const cudaError_t e = cudaFuncSetAttribute(int8_tile_kernel<kF16, kExpand>,
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
-            if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(int8_tile_kernel)");
-            configured[device] = true;
-        }
-        const int grid = static_cast<int>(tiles < sms ? tiles : sms);
-        int8_tile_kernel<kF16, kExpand><<<grid, kThreads<kExpand>, kBytes, st>>>(tm_q, tm_w, tp);
+    if (!configured[device]) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes);
+        if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(int8 tile kernel)");
+        configured[device] = true;
     }
-    const cudaError_t e = cudaGetLastError();
+    tp.split = 1;
+    int grid = 0;
+    if constexpr (kPair) {
+        grid = 2 * static_cast<int>(tiles < sms / 2 ? tiles : sms / 2);
+    } else {
+        // CTAs a tile, while they find SMs, where the stages that this saves outweigh the exchange
+        const int stages = (p.k + kBK - 1) / kBK;
+        while (stages >= kSplitStages && tp.split < kSplits && tiles * tp.split * 2 <= sms) tp.split *= 2;
+        grid = static_cast<int>(tiles * tp.split < sms ? tiles * tp.split : sms);
+    }
+    Launch l(grid, kThreads<kExpand>, kBytes, st);
+    if (after_quantize) l.after_last();
+    if (tp.split > 1) l.clusters_of(tp.split);
+    cudaError_t e;
+    if constexpr (kPair) e = cudaLaunchKernelEx(&l.config, kernel, tm_q, tm_w, tm_h, tm_bd, tp);
+    else e = cudaLaunchKernelEx(&l.config, kernel, tm_q, tm_w, tp);
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "int8 tile kernel launch");
 }
 
+// b_dec's rows are TMA coordinates, 32-bit.
+inline bool factor_rows_fit(const Params& p) {
+    return static_cast<int64_t>(p.rows / p.rows_per_sample) * p.n < 0x7fffffffLL - 256;
+}
+
 template <bool kF16>
-int32_t launch_linear(const Params& p, cudaStream_t st) {
-    if (p.rows <= 8) return launch_rows<kF16, 1>(p, st);
-    if (p.rows <= 16) return launch_rows<kF16, 2>(p, st);
-    if (p.rows <= 32) return launch_rows<kF16, 4>(p, st);
+int32_t launch_linear(const Params& p, bool after_quantize, cudaStream_t st) {
     int device = 0, sms = 0;
     const int32_t rc = current_device_sms(&device, &sms);
     if (rc != LITHE_OK) return rc;
+    // (14 x 3072 -> 18432: 13.4 us, 18.4 us on the tile kernel; 32 x 3072 -> 18432: 21.7 us and 18.4 us)
+    if (p.rows <= 8) return launch_rows<kF16, 1>(p, sms, after_quantize, st);
+    if (p.rows <= 16) return launch_rows<kF16, 2>(p, sms, after_quantize, st);
     // Pairs once their 256 x 256 tiles fill the GPU; 128 x 128 tiles before, to use more SMs.
     const int64_t pair_tiles = static_cast<int64_t>((p.rows + 255) / 256) * ((p.n + 255) / 256);
     const bool pair = pair_tiles >= sms / 2;
     if constexpr (!kF16) {
-        // b_dec's rows are TMA coordinates, 32-bit
-        const int64_t factor_rows = p.h ? static_cast<int64_t>(p.rows / p.rows_per_sample) * p.n : 0;
-        if (p.h && pair && p.rows_per_sample % 256 == 0 && factor_rows < 0x7fffffffLL - 256)
-            return launch_tiles<true, kF16, kExpandTmem>(p, device, sms, st);
-        if (p.h) return pair ? launch_tiles<true, kF16, kExpandMma>(p, device, sms, st)
-                             : launch_tiles<false, kF16, kExpandMma>(p, device, sms, st);
+        if (p.h && pair && p.rows_per_sample % 256 == 0 && factor_rows_fit(p))
+            return launch_tiles<true, kF16, kExpandTmem>(p, device, sms, after_quantize, st);
+        if (p.h) return pair ? launch_tiles<true, kF16, kExpandMma>(p, device, sms, after_quantize, st)
+                             : launch_tiles<false, kF16, kExpandMma>(p, device, sms, after_quantize, st);
     }
-    return pair ? launch_tiles<true, kF16, kExpandNone>(p, device, sms, st)
-                : launch_tiles<false, kF16, kExpandNone>(p, device, sms, st);
+    return pair ? launch_tiles<true, kF16, kExpandNone>(p, device, sms, after_quantize, st)
+                : launch_tiles<false, kF16, kExpandNone>(p, device, sms, after_quantize, st);
 }
 
 template <bool kF16>
@@ -912,7 +1087,9 @@ int32_t launch_quantize(const QuantParams& p, cudaStream_t st) {
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "quantize_kernel launch");
 }
 
-int32_t check_size(int32_t rows, int32_t n, int32_t k) {
+int32_t check_size(int32_t dtype, int32_t rows, int32_t n, int32_t k) {
+    if (dtype != LITHE_DTYPE_BF16 && dtype != LITHE_DTYPE_F16)
+        return fail_arg("dtype must be LITHE_DTYPE_BF16 or _F16, got %d", dtype);
     if (rows < 0 || n <= 0 || k <= 0) return fail_arg("rows must be >= 0 and n, k > 0 (rows %d, n %d, k %d)", rows, n, k);
     if (k > kMaxK) return fail_unsupported("k %d above %d: the int32 sums could overflow", k, kMaxK);
     return LITHE_OK;
@@ -926,40 +1103,17 @@ int32_t check_bytes(const void* base, int64_t stride, int32_t k, const char* nam
     return LITHE_OK;
 }
 
-}  // namespace i8
-}  // namespace lithe
-
-extern "C" int32_t lithe_quantize_rows(const void* x, int32_t dtype, int32_t rows, int32_t k, int64_t x_stride,
-                                       void* q, int64_t q_stride, float* scale, void* stream) {
-    using namespace lithe;
-    using namespace lithe::i8;
-    clear_error();
-    if (dtype != LITHE_DTYPE_BF16 && dtype != LITHE_DTYPE_F16)
-        return fail_arg("dtype must be LITHE_DTYPE_BF16 or _F16, got %d", dtype);
-    int32_t rc = check_size(rows, 1, k);
-    if (rc != LITHE_OK) return rc;
-    if (rows == 0) return LITHE_OK;
-    if (!x || !scale) return fail_arg("x and scale must be non-NULL");
-    if (reinterpret_cast<uintptr_t>(x) % 2 || reinterpret_cast<uintptr_t>(scale) % 4)
-        return fail_arg("x and scale must be aligned to their elements");
+int32_t check_x(const void* x, int64_t x_stride) {
+    if (!x || reinterpret_cast<uintptr_t>(x) % 2) return fail_arg("x must be non-NULL and aligned to its elements");
     if (x_stride < 0) return fail_arg("x_stride must be >= 0");
-    if ((rc = check_bytes(q, q_stride, k, "q")) != LITHE_OK) return rc;
-    QuantParams p{static_cast<const uint16_t*>(x), static_cast<int8_t*>(q), scale, x_stride, q_stride, rows, k};
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == LITHE_DTYPE_F16 ? launch_quantize<true>(p, st) : launch_quantize<false>(p, st);
+    return LITHE_OK;
 }
 
-extern "C" int32_t lithe_int8_linear(const void* q, int64_t q_stride, const float* x_scale, const void* w,
-                                     int64_t w_stride, const float* w_scale, const void* bias, void* out,
-                                     int32_t dtype, int32_t rows, int32_t n, int32_t k, const void* h,
-                                     const void* b_dec, int32_t rows_per_sample, int32_t rank, int32_t* err_flag,
-                                     void* stream) {
-    using namespace lithe;
-    using namespace lithe::i8;
-    clear_error();
-    if (dtype != LITHE_DTYPE_BF16 && dtype != LITHE_DTYPE_F16)
-        return fail_arg("dtype must be LITHE_DTYPE_BF16 or _F16, got %d", dtype);
-    int32_t rc = check_size(rows, n, k);
+// The checks of a linear's operands other than its activations; fills p.
+int32_t linear_params(Params* p, const void* w, int64_t w_stride, const float* w_scale, const void* bias, void* out,
+                      int32_t dtype, int32_t rows, int32_t n, int32_t k, const void* h, const void* b_dec,
+                      int32_t rows_per_sample, int32_t rank, int32_t* err_flag) {
+    int32_t rc = check_size(dtype, rows, n, k);
     if (rc != LITHE_OK) return rc;
     if (h) {
         if (!b_dec) return fail_arg("b_dec is NULL while h is given");
@@ -971,28 +1125,106 @@ extern "C" int32_t lithe_int8_linear(const void* q, int64_t q_stride, const floa
             return fail_arg("h and b_dec must be 16-byte aligned");
     }
     if (rows == 0) return LITHE_OK;
-    if ((rc = check_bytes(q, q_stride, k, "q")) != LITHE_OK) return rc;
     if ((rc = check_bytes(w, w_stride, k, "w")) != LITHE_OK) return rc;
-    if (!x_scale || !w_scale || !out) return fail_arg("x_scale, w_scale and out must be non-NULL");
-    if (reinterpret_cast<uintptr_t>(x_scale) % 4 || reinterpret_cast<uintptr_t>(w_scale) % 4 ||
-        reinterpret_cast<uintptr_t>(out) % 2 || reinterpret_cast<uintptr_t>(bias) % 2)
-        return fail_arg("x_scale, w_scale, bias and out must be aligned to their elements");
+    if (!w_scale || !out) return fail_arg("w_scale and out must be non-NULL");
+    if (reinterpret_cast<uintptr_t>(w_scale) % 4 || reinterpret_cast<uintptr_t>(out) % 2 ||
+        reinterpret_cast<uintptr_t>(bias) % 2)
+        return fail_arg("w_scale, bias and out must be aligned to their elements");
+    p->w = static_cast<const int8_t*>(w);
+    p->w_scale = w_scale;
+    p->bias = static_cast<const uint16_t*>(bias);
+    p->out = static_cast<uint16_t*>(out);
+    p->h = static_cast<const __nv_bfloat16*>(h);
+    p->b_dec = static_cast<const __nv_bfloat16*>(b_dec);
+    p->err = err_flag;
+    p->w_stride = w_stride;
+    p->rows = rows;
+    p->n = n;
+    p->k = k;
+    p->rows_per_sample = rows_per_sample;
+    return LITHE_OK;
+}
+
+int32_t quantize(const QuantParams& p, int32_t dtype, cudaStream_t st) {
+    return dtype == LITHE_DTYPE_F16 ? launch_quantize<true>(p, st) : launch_quantize<false>(p, st);
+}
+
+// after_quantize: the stream's last launch is the quantisation of these activations.
+int32_t linear(const Params& p, int32_t dtype, bool after_quantize, cudaStream_t st) {
+    return dtype == LITHE_DTYPE_F16 ? launch_linear<true>(p, after_quantize, st)
+                                    : launch_linear<false>(p, after_quantize, st);
+}
+
+}  // namespace i8
+}  // namespace lithe
+
+extern "C" int32_t lithe_quantize_rows(const void* x, int32_t dtype, int32_t rows, int32_t k, int64_t x_stride,
+                                       void* q, int64_t q_stride, float* scale, void* stream) {
+    using namespace lithe;
+    using namespace lithe::i8;
+    clear_error();
+    int32_t rc = check_size(dtype, rows, 1, k);
+    if (rc != LITHE_OK) return rc;
+    if (rows == 0) return LITHE_OK;
+    if ((rc = check_x(x, x_stride)) != LITHE_OK) return rc;
+    if (!scale || reinterpret_cast<uintptr_t>(scale) % 4)
+        return fail_arg("scale must be non-NULL and aligned to its elements");
+    if ((rc = check_bytes(q, q_stride, k, "q")) != LITHE_OK) return rc;
+    const QuantParams p{static_cast<const uint16_t*>(x), static_cast<int8_t*>(q), scale, x_stride, q_stride, rows, k};
+    return quantize(p, dtype, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int32_t lithe_int8_linear(const void* q, int64_t q_stride, const float* x_scale, const void* w,
+                                     int64_t w_stride, const float* w_scale, const void* bias, void* out,
+                                     int32_t dtype, int32_t rows, int32_t n, int32_t k, const void* h,
+                                     const void* b_dec, int32_t rows_per_sample, int32_t rank, int32_t* err_flag,
+                                     void* stream) {
+    using namespace lithe;
+    using namespace lithe::i8;
+    clear_error();
     Params p{};
+    int32_t rc = linear_params(&p, w, w_stride, w_scale, bias, out, dtype, rows, n, k, h, b_dec, rows_per_sample, rank,
+                               err_flag);
+    if (rc != LITHE_OK || rows == 0) return rc;
+    if ((rc = check_bytes(q, q_stride, k, "q")) != LITHE_OK) return rc;
+    if (!x_scale || reinterpret_cast<uintptr_t>(x_scale) % 4)
+        return fail_arg("x_scale must be non-NULL and aligned to its elements");
     p.q = static_cast<const int8_t*>(q);
-    p.w = static_cast<const int8_t*>(w);
-    p.x_scale = x_scale;
-    p.w_scale = w_scale;
-    p.bias = static_cast<const uint16_t*>(bias);
-    p.out = static_cast<uint16_t*>(out);
-    p.h = static_cast<const __nv_bfloat16*>(h);
-    p.b_dec = static_cast<const __nv_bfloat16*>(b_dec);
-    p.err = err_flag;
     p.q_stride = q_stride;
-    p.w_stride = w_stride;
-    p.rows = rows;
-    p.n = n;
-    p.k = k;
-    p.rows_per_sample = rows_per_sample;
+    p.x_scale = x_scale;
+    return linear(p, dtype, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int64_t lithe_int8_workspace_bytes(int32_t rows, int32_t k) {
+    if (rows <= 0 || k <= 0) return 0;
+    return static_cast<int64_t>(rows) * ((static_cast<int64_t>(k) + 15) / 16 * 16 + 4);
+}
+
+extern "C" int32_t lithe_int8_linear_dynamic(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
+                                             const float* w_scale, const void* bias, void* out, int32_t dtype,
+                                             int32_t rows, int32_t n, int32_t k, const void* h, const void* b_dec,
+                                             int32_t rows_per_sample, int32_t rank, int32_t* err_flag,
+                                             void* workspace, int64_t workspace_bytes, void* stream) {
+    using namespace lithe;
+    using namespace lithe::i8;
+    clear_error();
+    Params p{};
+    int32_t rc = linear_params(&p, w, w_stride, w_scale, bias, out, dtype, rows, n, k, h, b_dec, rows_per_sample, rank,
+                               err_flag);
+    if (rc != LITHE_OK || rows == 0) return rc;
+    if ((rc = check_x(x, x_stride)) != LITHE_OK) return rc;
+    const int64_t need = lithe_int8_workspace_bytes(rows, k);
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need)
+        return fail_arg("workspace must be 16-byte aligned and hold %lld bytes, got %lld", static_cast<long long>(need),
+                        static_cast<long long>(workspace_bytes));
+    const int64_t q_stride = (static_cast<int64_t>(k) + 15) / 16 * 16;
+    int8_t* q = static_cast<int8_t*>(workspace);
+    float* scale = reinterpret_cast<float*>(q + rows * q_stride);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return dtype == LITHE_DTYPE_F16 ? launch_linear<true>(p, st) : launch_linear<false>(p, st);
+    rc = quantize(QuantParams{static_cast<const uint16_t*>(x), q, scale, x_stride, q_stride, rows, k}, dtype, st);
+    if (rc != LITHE_OK) return rc;
+    p.q = q;
+    p.q_stride = q_stride;
+    p.x_scale = scale;
+    return linear(p, dtype, true, st);
 }

@@ -6,6 +6,7 @@ kernels' device-side error word is read only by ``device_errors``.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import functools
 import threading
@@ -26,6 +27,9 @@ _err_lock = threading.Lock()
 
 def error_word(device: torch.device) -> torch.Tensor:
     """The int32 device error word the kernels of ``device`` OR their LITHE_DEVERR_* bits into."""
+    t = _err_words.get(getattr(device, "index", None))
+    if t is not None:
+        return t
     device = torch.device(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
@@ -71,7 +75,13 @@ def _sm_count(device: torch.device) -> int:
     return _SMS[idx]
 
 
+# The current stream's handle without the Python object around it (which costs more than a launch).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def stream_handle(device: torch.device) -> int:
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -109,11 +119,13 @@ def lut_from_list(lut) -> ctypes.Array:
     return arr
 
 
+_NO_CONTEXT = contextlib.nullcontext()
+
+
 def device_ctx(device: torch.device):
     """torch.cuda.device(device), or a no-op when it is already the current device."""
-    import contextlib
     if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+        return _NO_CONTEXT
     return torch.cuda.device(device)
 
 
@@ -460,11 +472,15 @@ def _axis_array(axes: tuple) -> ctypes.Array:
 
 def _heads_strides(t: torch.Tensor) -> tuple:
     """(sample, token, head) strides; a dimension of one element has none that matters."""
-    return tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3]))
+    b, s, h, _ = t.shape
+    sb, ss, sh, _ = t.stride()
+    return (sb if b != 1 else 0, ss if s != 1 else 0, sh if h != 1 else 0)
 
 
 def _heads_view(t: torch.Tensor) -> _lib.HeadsView:
-    return _lib.HeadsView(t.data_ptr(), *_heads_strides(t), t.shape[2])
+    b, s, h, _ = t.shape
+    sb, ss, sh, _ = t.stride()
+    return _lib.HeadsView(t.data_ptr(), sb if b != 1 else 0, ss if s != 1 else 0, sh if h != 1 else 0, h)
 
 
 def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
@@ -482,12 +498,18 @@ def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None
 
 
 def _byte_span(t: torch.Tensor) -> tuple:
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+    b, s, h, d = t.shape
+    sb, ss, sh, sd = t.stride()
+    first = t.data_ptr()
+    return first, first + ((b - 1) * sb + (s - 1) * ss + (h - 1) * sh + (d - 1) * sd + 1) * t.element_size()
 
 
 def _has_own_elements(t: torch.Tensor) -> bool:
     """Whether no two of ``t``'s elements share an address (an expanded tensor's do)."""
+    b, s, h, d = t.shape
+    sb, ss, sh, _ = t.stride()
+    if (h == 1 or sh >= d) and (s == 1 or ss >= (h - 1) * sh + d) and (b == 1 or sb >= (s - 1) * ss + (h - 1) * sh + d):
+        return True
     reach = 0
     for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
         if s <= reach:
@@ -533,86 +555,92 @@ def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def _check_outputs(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], names: Sequence[str]) -> None:
     """Every output is its own input (in place) or shares no element with an input or another output."""
+    spans = [_byte_span(t) for t in (*ins, *outs)]
     for i, (o, name) in enumerate(zip(outs, names)):
         if not _has_own_elements(o):
             raise ValueError(f"{name} has elements that share an address")
+        o0, o1 = spans[len(ins) + i]
         for j, x in enumerate(ins):
-            if not (i == j and _same_view(o, x)) and not _apart(o, x):
+            if spans[j][1] > o0 and o1 > spans[j][0] and not (i == j and _same_view(o, x)) and not _apart(o, x):
                 raise ValueError(f"{name} overlaps an input (it may be its own input's very view)")
         for j in range(i):
-            if not _apart(o, outs[j]):
+            k = len(ins) + j
+            if spans[k][1] > o0 and o1 > spans[k][0] and not _apart(o, outs[j]):
                 raise ValueError(f"{name} overlaps {names[j]}")
 
 
 def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta: float, pairing: int) -> tuple:
-    if positions.dtype not in _POS_CODE:
+    code = _POS_CODE.get(positions.dtype)
+    if code is None:
         raise TypeError(f"positions must be int32, int64 or float32, got {positions.dtype}")
     if positions.device != x.device:
         raise ValueError("positions must be on the inputs' device")
     b, s = x.shape[:2]
-    if tuple(positions.shape) not in ((s, len(axes)), (b, s, len(axes))):
-        raise ValueError(f"positions must be ({s}, {len(axes)}) or ({b}, {s}, {len(axes)}), got "
-                         f"{tuple(positions.shape)}")
+    shape, n = positions.shape, len(axes)
+    if shape != (s, n) and shape != (b, s, n):
+        raise ValueError(f"positions must be ({s}, {n}) or ({b}, {s}, {n}), got {tuple(shape)}")
     if not positions.is_contiguous():
         raise ValueError("positions must be contiguous")
-    return (positions.data_ptr(), _POS_CODE[positions.dtype], int(positions.dim() == 3), _axis_array(axes), len(axes),
-            theta, pairing, stream_handle(x.device))
+    return (positions.data_ptr(), code, len(shape) - 2, _axis_array(axes), n, theta, pairing, stream_handle(x.device))
 
 
 def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], theta: float,
-                 pairing: int) -> torch.Tensor:
-    """lithe_rotate_axes on torch tensors: ``out`` (batch, tokens, heads, dim) is written."""
-    _check_heads(x, "x")
-    if out is not x:
-        _check_heads(out, "out", x)
-        if out.shape != x.shape:
-            raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
+                 pairing: int, fresh: bool = False) -> torch.Tensor:
+    """lithe_rotate_axes on torch tensors: ``out`` (batch, tokens, heads, dim) is written.  ``fresh``: the
+    caller has checked x and made ``out`` for this call, so that neither needs another look."""
+    if not fresh:
+        _check_heads(x, "x")
+        if out is not x:
+            _check_heads(out, "out", x)
+            if out.shape != x.shape:
+                raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
         _check_outputs((x,), (out,), ("out",))
-    else:
-        _check_outputs((), (out,), ("x, written in place,",))
-    axes = tuple(axes)
+    b, s, _, d = x.shape
+    args = (ctypes.byref(_heads_view(x)), ctypes.byref(_heads_view(out)), _DTYPE_CODE[x.dtype], b, s, d,
+            *_rotation_args(x, positions, tuple(axes), theta, pairing))
     with device_ctx(x.device):
-        rc = _lib.lib().lithe_rotate_axes(ctypes.byref(_heads_view(x)), ctypes.byref(_heads_view(out)),
-                                          _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1], x.shape[3],
-                                          *_rotation_args(x, positions, axes, theta, pairing))
-    _lib.check(rc, "lithe_rotate_axes")
+        rc = _lib.lib().lithe_rotate_axes(*args)
+    if rc:
+        _lib.check(rc, "lithe_rotate_axes")
     return out
 
 
 def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k: torch.Tensor,
                     weight_q: Optional[torch.Tensor], weight_k: Optional[torch.Tensor], positions: torch.Tensor,
-                    axes: Sequence[int], theta: float, eps: float, pairing: int) -> None:
-    """lithe_qk_norm_rotate on torch tensors: ``out_q`` and ``out_k`` are written."""
-    _check_heads(q, "q")
-    _check_heads(k, "k", q)
-    _check_heads(out_q, "out_q", q)
-    _check_heads(out_k, "out_k", q)
-    if k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+                    axes: Sequence[int], theta: float, eps: float, pairing: int, fresh: bool = False) -> None:
+    """lithe_qk_norm_rotate on torch tensors: ``out_q`` and ``out_k`` are written.  ``fresh``: the caller
+    has checked q and k and made both outputs for this call."""
+    if not fresh:
+        _check_heads(q, "q")
+        _check_heads(k, "k", q)
+        _check_heads(out_q, "out_q", q)
+        _check_heads(out_k, "out_k", q)
+        if out_q.shape != q.shape or out_k.shape != k.shape:
+            raise ValueError(f"out_q and out_k must be {tuple(q.shape)} and {tuple(k.shape)}, got "
+                             f"{tuple(out_q.shape)} and {tuple(out_k.shape)}")
+        _check_outputs((q, k), (out_q, out_k), ("out_q", "out_k"))
+    b, s, _, d = q.shape
+    if k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch, tokens and dim")
-    if out_q.shape != q.shape or out_k.shape != k.shape:
-        raise ValueError(f"out_q and out_k must be {tuple(q.shape)} and {tuple(k.shape)}, got {tuple(out_q.shape)} "
-                         f"and {tuple(out_k.shape)}")
-    weight_dtype = q.dtype
+    dtype = weight_dtype = q.dtype
     for w, name in ((weight_q, "weight_q"), (weight_k, "weight_k")):
         if w is None:
             continue
-        if w.dtype not in (q.dtype, torch.float32):
-            raise TypeError(f"{name} must be {q.dtype} or float32, got {w.dtype}")
-        if tuple(w.shape) != (q.shape[3],) or w.device != q.device or not w.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous ({q.shape[3]},) tensor on q's device")
+        if w.dtype != dtype and w.dtype != torch.float32:
+            raise TypeError(f"{name} must be {dtype} or float32, got {w.dtype}")
+        if w.shape != (d,) or w.device != q.device or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous ({d},) tensor on q's device")
         weight_dtype = w.dtype
     if weight_q is not None and weight_k is not None and weight_q.dtype != weight_k.dtype:
         raise TypeError(f"weight_q and weight_k must have one type, got {weight_q.dtype} and {weight_k.dtype}")
-    _check_outputs((q, k), (out_q, out_k), ("out_q", "out_k"))
-    axes = tuple(axes)
-    with device_ctx(q.device):
-        rc = _lib.lib().lithe_qk_norm_rotate(
-            ctypes.byref(_heads_view(q)), ctypes.byref(_heads_view(k)), ctypes.byref(_heads_view(out_q)),
+    args = (ctypes.byref(_heads_view(q)), ctypes.byref(_heads_view(k)), ctypes.byref(_heads_view(out_q)),
             ctypes.byref(_heads_view(out_k)), weight_q.data_ptr() if weight_q is not None else None,
             weight_k.data_ptr() if weight_k is not None else None, _DTYPE_CODE[weight_dtype], eps,
-            _DTYPE_CODE[q.dtype], q.shape[0], q.shape[1], q.shape[3],
-            *_rotation_args(q, positions, axes, theta, pairing))
-    _lib.check(rc, "lithe_qk_norm_rotate")
+            _DTYPE_CODE[dtype], b, s, d, *_rotation_args(q, positions, tuple(axes), theta, pairing))
+    with device_ctx(q.device):
+        rc = _lib.lib().lithe_qk_norm_rotate(*args)
+    if rc:
+        _lib.check(rc, "lithe_qk_norm_rotate")
 
 
 # ------------------------------------------------------------------------------------------
@@ -644,57 +672,113 @@ def padded(k: int) -> int:
     return -(-k // 16) * 16
 
 
+def _int8_weight(weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optional[torch.Tensor], dtype: torch.dtype,
+                 dev: torch.device, k: int) -> tuple:
+    """The checks of a linear's int8 weight, scale and bias; (n, bytes between the weight's rows)."""
+    if weight.dtype != torch.int8 or weight.device != dev:
+        raise TypeError(f"weight must be int8 on {dev}, got {weight.dtype} on {weight.device}")
+    if weight.dim() != 2 or weight.shape[1] != k:
+        raise ValueError(f"weight must be (n, {k}), got {tuple(weight.shape)}")
+    n = weight.shape[0]
+    stride, inner = weight.stride()
+    if n == 1:
+        stride = padded(k)
+    if (k > 1 and inner != 1) or stride % 16 or weight.data_ptr() % 16:
+        raise ValueError("weight: int8 rows must be contiguous and start on 16-byte boundaries "
+                         f"(strides {weight.stride()})")
+    if weight_scale.dtype != torch.float32 or weight_scale.numel() != n or not weight_scale.is_contiguous() \
+            or weight_scale.device != dev:
+        raise ValueError(f"weight_scale must be a contiguous ({n},) float32 tensor on x's device")
+    if bias is not None and (bias.dtype != dtype or bias.numel() != n or not bias.is_contiguous()
+                             or bias.device != dev):
+        raise ValueError(f"bias must be a contiguous ({n},) {dtype} tensor on x's device")
+    return n, stride
+
+
+def _int8_expand(h: Optional[torch.Tensor], b_dec: Optional[torch.Tensor], rows: int, n: int,
+                 dev: torch.device) -> tuple:
+    """The checks of the expand's operands; their (h, b_dec, rows per sample, rank) arguments."""
+    if h is None and b_dec is None:
+        return None, None, 0, 0
+    if h is None or b_dec is None:
+        raise ValueError("h and b_dec come together")
+    for t, name in ((h, "h"), (b_dec, "b_dec")):
+        if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != dev:
+            raise ValueError(f"{name} must be a contiguous bfloat16 tensor on x's device")
+    if h.dim() != 2 or h.shape[0] != rows or b_dec.dim() != 3 or b_dec.shape[1] != n \
+            or b_dec.shape[2] != h.shape[1]:
+        raise ValueError(f"h must be ({rows}, rank) and b_dec (samples, {n}, rank), got {tuple(h.shape)} and "
+                         f"{tuple(b_dec.shape)}")
+    samples = b_dec.shape[0]
+    if rows and (samples == 0 or rows % samples):
+        raise ValueError(f"b_dec's {samples} samples do not divide {rows} rows")
+    return h.data_ptr(), b_dec.data_ptr(), rows // samples if samples else 0, h.shape[1]
+
+
 def int8_linear_(q: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
                  bias: Optional[torch.Tensor], out: torch.Tensor, h: Optional[torch.Tensor] = None,
                  b_dec: Optional[torch.Tensor] = None, err: Optional[torch.Tensor] = None) -> torch.Tensor:
     """lithe_int8_linear: out (rows, n) from q (rows, k), x_scale (rows,), weight (n, k), weight_scale (n,)."""
     _require_cuda(q, "q")
     dev = q.device
-    if q.dim() != 2 or weight.dim() != 2 or out.dim() != 2:
-        raise ValueError("q (rows, k), weight (n, k) and out (rows, n) must be 2-D")
+    if q.dim() != 2 or q.dtype != torch.int8:
+        raise ValueError(f"q must be (rows, k) int8, got {tuple(q.shape)} {q.dtype}")
     rows, k = q.shape
-    n = weight.shape[0]
-    if weight.dtype != torch.int8 or weight.device != dev:
-        raise TypeError(f"weight must be int8 on {dev}, got {weight.dtype} on {weight.device}")
-    if weight.shape[1] != k or tuple(out.shape) != (rows, n):
-        raise ValueError(f"shapes disagree: q {tuple(q.shape)}, weight {tuple(weight.shape)}, out {tuple(out.shape)}")
-    for t, name in ((q, "q"), (weight, "weight")):
-        if t.dtype != torch.int8 or (k > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) % 16) \
-                or t.data_ptr() % 16:
-            raise ValueError(f"{name}: int8 rows must be contiguous and start on 16-byte boundaries "
-                             f"(strides {t.stride()})")
-    if out.dtype not in ACTIVATION_DTYPES or not out.is_contiguous() or out.device != dev:
-        raise ValueError("out must be a contiguous bfloat16 or float16 tensor on q's device")
-    for t, want, name in ((x_scale, rows, "x_scale"), (weight_scale, n, "weight_scale")):
-        if t.dtype != torch.float32 or t.numel() != want or not t.is_contiguous() or t.device != dev:
-            raise ValueError(f"{name} must be a contiguous ({want},) float32 tensor on q's device")
-    if bias is not None and (bias.dtype != out.dtype or bias.numel() != n or not bias.is_contiguous()
-                             or bias.device != dev):
-        raise ValueError(f"bias must be a contiguous ({n},) {out.dtype} tensor on q's device")
-    rank = rows_per_sample = 0
-    if (h is None) != (b_dec is None):
-        raise ValueError("h and b_dec come together")
-    if h is not None:
-        for t, name in ((h, "h"), (b_dec, "b_dec")):
-            if t.dtype != torch.bfloat16 or not t.is_contiguous() or t.device != dev:
-                raise ValueError(f"{name} must be a contiguous bfloat16 tensor on q's device")
-        if h.dim() != 2 or h.shape[0] != rows or b_dec.dim() != 3 or tuple(b_dec.shape[1:]) != (n, h.shape[1]):
-            raise ValueError(f"h must be ({rows}, rank) and b_dec (samples, {n}, rank), got {tuple(h.shape)} and "
-                             f"{tuple(b_dec.shape)}")
-        rank, samples = h.shape[1], b_dec.shape[0]
-        if rows and (samples == 0 or rows % samples):
-            raise ValueError(f"b_dec's {samples} samples do not divide {rows} rows")
-        rows_per_sample = rows // samples if samples else 0
+    q_stride = q.stride(0) if rows > 1 else padded(k)
+    if (k > 1 and q.stride(1) != 1) or q_stride % 16 or q.data_ptr() % 16:
+        raise ValueError(f"q: int8 rows must be contiguous and start on 16-byte boundaries (strides {q.stride()})")
+    n, w_stride = _int8_weight(weight, weight_scale, bias, out.dtype, dev, k)
+    if out.dtype not in ACTIVATION_DTYPES or out.shape != (rows, n) or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out must be a contiguous ({rows}, {n}) bfloat16 or float16 tensor on q's device")
+    if x_scale.dtype != torch.float32 or x_scale.numel() != rows or not x_scale.is_contiguous() \
+            or x_scale.device != dev:
+        raise ValueError(f"x_scale must be a contiguous ({rows},) float32 tensor on q's device")
+    expand = _int8_expand(h, b_dec, rows, n, dev)
     if rows == 0:
         return out
     if err is None:
         err = error_word(dev)
     with device_ctx(dev):
         rc = _lib.lib().lithe_int8_linear(
-            q.data_ptr(), q.stride(0) if rows > 1 else padded(k), x_scale.data_ptr(), weight.data_ptr(),
-            weight.stride(0) if n > 1 else padded(k), weight_scale.data_ptr(),
+            q.data_ptr(), q_stride, x_scale.data_ptr(), weight.data_ptr(), w_stride, weight_scale.data_ptr(),
             bias.data_ptr() if bias is not None else None, out.data_ptr(), _DTYPE_CODE[out.dtype], rows, n, k,
-            h.data_ptr() if h is not None else None, b_dec.data_ptr() if b_dec is not None else None,
-            rows_per_sample, rank, err.data_ptr(), stream_handle(dev))
-    _lib.check(rc, "lithe_int8_linear")
+            *expand, err.data_ptr(), stream_handle(dev))
+    if rc:
+        _lib.check(rc, "lithe_int8_linear")
+    return out
+
+
+def int8_linear_dynamic(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                        bias: Optional[torch.Tensor], h: Optional[torch.Tensor] = None,
+                        b_dec: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """lithe_int8_linear_dynamic: (..., n) from x (..., k) bf16 / fp16, quantised within the call."""
+    _require_cuda(x, "x")
+    dev, dtype, shape = x.device, x.dtype, x.shape
+    if dtype not in ACTIVATION_DTYPES:
+        raise TypeError(f"x must be one of {ACTIVATION_DTYPES}, got {dtype}")
+    if not shape or shape[-1] < 1:
+        raise ValueError(f"x must be (..., k) with k >= 1, got {tuple(shape)}")
+    k = shape[-1]
+    if x.is_contiguous():
+        rows, x_stride = x.numel() // k, k
+    else:
+        x = x.reshape(-1, k)
+        if k > 1 and x.stride(1) != 1:
+            x = x.contiguous()
+        rows = x.shape[0]
+        x_stride = x.stride(0) if rows > 1 else k
+    n, w_stride = _int8_weight(weight, weight_scale, bias, dtype, dev, k)
+    expand = _int8_expand(h, b_dec, rows, n, dev)
+    out = x.new_empty((*shape[:-1], n))
+    if rows == 0:
+        return out
+    q_bytes = rows * padded(k)
+    space = torch.empty(q_bytes + 4 * rows, dtype=torch.uint8, device=dev)
+    with device_ctx(dev):
+        rc = _lib.lib().lithe_int8_linear_dynamic(
+            x.data_ptr(), x_stride, weight.data_ptr(), w_stride, weight_scale.data_ptr(),
+            bias.data_ptr() if bias is not None else None, out.data_ptr(), _DTYPE_CODE[dtype], rows, n, k, *expand,
+            error_word(dev).data_ptr(), space.data_ptr(), q_bytes + 4 * rows, stream_handle(dev))
+    if rc:
+        _lib.check(rc, "lithe_int8_linear_dynamic")
     return out

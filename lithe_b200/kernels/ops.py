@@ -29,6 +29,7 @@ ABI as a flat list of 2 * levels * 10 floats.
                                                          lithe_qk_norm_rotate
   quantize_rows(x) -> (q, scale)                                     lithe_quantize_rows
   int8_linear(q, x_scale, weight, weight_scale, bias, h, b_dec, fp16) -> out     lithe_int8_linear
+  int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec) -> out            lithe_int8_linear_dynamic
   decode_packed(words, n_blocks, levels, sides, lut, fp32) -> out    lithe_decode_packed
 """
 from __future__ import annotations
@@ -209,3 +210,15 @@ def int8_linear(q: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, we
 @int8_linear.register_fake
 def _int8_linear_fake(q, x_scale, weight, weight_scale, bias, h, b_dec, fp16):
     return q.new_empty(q.shape[0], weight.shape[0], dtype=torch.float16 if fp16 else torch.bfloat16)
+
+
+@torch.library.custom_op(f"{_NS}::int8_linear_dynamic", mutates_args=(), device_types="cuda")
+def int8_linear_dynamic(x: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor,
+                        bias: Optional[torch.Tensor], h: Optional[torch.Tensor],
+                        b_dec: Optional[torch.Tensor]) -> torch.Tensor:
+    return _launch.int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec)
+
+
+@int8_linear_dynamic.register_fake
+def _int8_linear_dynamic_fake(x, weight, weight_scale, bias, h, b_dec):
+    return x.new_empty(*x.shape[:-1], weight.shape[0])

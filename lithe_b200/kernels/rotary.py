@@ -17,6 +17,7 @@ allocate nothing but their results, and can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -27,11 +28,13 @@ from . import _launch
 
 
 def _inference_only(*tensors: Optional[torch.Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
 
 
-def _rotation(dim: int, axes: Sequence[int], theta: float, pairing: str) -> Tuple[Tuple[int, ...], float, int]:
+@functools.lru_cache(maxsize=256)
+def _rotation(dim: int, axes: Tuple[int, ...], theta: float, pairing: str) -> Tuple[Tuple[int, ...], float, int]:
     axes = tuple(int(a) for a in axes)
     if pairing not in _launch.PAIRINGS:
         raise ValueError(f"pairing must be one of {tuple(_launch.PAIRINGS)}, got {pairing!r}")
@@ -57,9 +60,10 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     """
     _launch._check_heads(x, "x")
     _inference_only(x)
-    axes, theta, code = _rotation(x.shape[3], axes, theta, pairing)
-    if out is None:
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    axes, theta, code = _rotation(x.shape[3], tuple(axes), theta, pairing)
+    fresh = out is None
+    if fresh:
+        out = x.new_empty(x.shape)
     positions = positions.contiguous()
     if torch.compiler.is_compiling():
         if out is x:
@@ -68,7 +72,7 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
             return x.copy_(out)
         torch.ops.lithe_b200.rotate_axes_(out, x, positions, list(axes), theta, code)
         return out
-    return _launch.rotate_axes_(x, out, positions, axes, theta, code)
+    return _launch.rotate_axes_(x, out, positions, axes, theta, code, fresh)
 
 
 def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Tensor],
@@ -90,16 +94,17 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
-    axes, theta, code = _rotation(q.shape[3], axes, theta, pairing)
+    axes, theta, code = _rotation(q.shape[3], tuple(axes), theta, pairing)
+    fresh = out_q is None and out_k is None
     if out_q is None:
-        out_q = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        out_q = q.new_empty(q.shape)
     if out_k is None:
-        out_k = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        out_k = k.new_empty(k.shape)
     positions = positions.contiguous()
     if torch.compiler.is_compiling():
         oq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is q else out_q
         ok = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is k else out_k
         torch.ops.lithe_b200.qk_norm_rotate_(oq, ok, q, k, weight_q, weight_k, positions, list(axes), theta, eps, code)
         return (q.copy_(oq) if out_q is q else oq), (k.copy_(ok) if out_k is k else ok)
-    _launch.qk_norm_rotate_(q, k, out_q, out_k, weight_q, weight_k, positions, axes, theta, eps, code)
+    _launch.qk_norm_rotate_(q, k, out_q, out_k, weight_q, weight_k, positions, axes, theta, eps, code, fresh)
     return out_q, out_k

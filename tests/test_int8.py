@@ -66,7 +66,40 @@ def test_c_quantize_refuses(over, code):
     assert _quant(**over) == code
 
 
+def _dynamic(x=0x10000, x_stride=100, w=0x30000, w_stride=128, rows=4, n=8, k=100, dtype=_lib.DTYPE_BF16, h=None,
+             b_dec=None, space=0x20000, size=4 * (112 + 4)):
+    return _lib.lib().lithe_int8_linear_dynamic(x, x_stride, w, w_stride, 0x40000, None, 0x50000, dtype, rows, n, k, h,
+                                                b_dec, 2, 16, None, space, size, None)
+
+
+@pytest.mark.parametrize("over,code", [
+    ({"x": None}, _lib.ERR_ARG),
+    ({"x": 0x10001}, _lib.ERR_ARG),
+    ({"x_stride": -100}, _lib.ERR_ARG),
+    ({"w": 0x30004}, _lib.ERR_ARG),
+    ({"dtype": _lib.DTYPE_F32}, _lib.ERR_ARG),
+    ({"space": None}, _lib.ERR_ARG),
+    ({"space": 0x20008}, _lib.ERR_ARG),
+    ({"size": 4 * (112 + 4) - 1}, _lib.ERR_ARG),
+    ({"h": 0x70000}, _lib.ERR_ARG),
+    ({"k": 200000, "w_stride": 200000}, _lib.ERR_UNSUPPORTED),
+])
+def test_c_dynamic_refuses(over, code):
+    assert _dynamic(**over) == code
+    assert _lib.lib().lithe_last_error()
+
+
+def test_workspace_bytes():
+    lib = _lib.lib()
+    assert lib.lithe_int8_workspace_bytes(4, 100) == 4 * (112 + 4)
+    assert lib.lithe_int8_workspace_bytes(0, 100) == 0
+    assert lib.lithe_int8_workspace_bytes(2 ** 31 - 1, 131072) == (2 ** 31 - 1) * (131072 + 4)
+    assert _dynamic(rows=0, x=None, space=None, size=0) == _lib.OK
+
+
 def test_python_checks():
+    with pytest.raises(ValueError, match="CUDA"):
+        int8_linear(torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.int8), torch.zeros(4))
     with pytest.raises(ValueError, match="CUDA"):
         quantize_rows(torch.zeros(2, 8, dtype=torch.bfloat16))
     with FakeTensorMode():
@@ -110,5 +143,7 @@ def test_ops_know_their_shapes():
         x = torch.empty(6, 40, dtype=torch.float16, device="cuda")
         q, scale = torch.ops.lithe_b200.quantize_rows(x)
         assert tuple(q.shape) == (6, 40) and q.stride(0) == 48 and q.dtype == torch.int8 and tuple(scale.shape) == (6,)
+        y = torch.ops.lithe_b200.int8_linear_dynamic(x.view(2, 3, 40), q[:3], scale[:3], None, None, None)
+        assert tuple(y.shape) == (2, 3, 3) and y.dtype == torch.float16
         y = torch.ops.lithe_b200.int8_linear(q, scale, q[:3], scale[:3], None, None, None, True)
         assert tuple(y.shape) == (6, 3) and y.dtype == torch.float16
