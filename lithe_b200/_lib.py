@@ -68,7 +68,8 @@ class PackSegment(ctypes.Structure):
 
 
 class HeadsView(ctypes.Structure):
-    """``lithe_heads_view``: a (batch, tokens, heads, dim) operand of the rotation kernels."""
+    """``lithe_heads_view``: a (batch, tokens, heads, dim) operand of the rotation kernels, passed by
+    address (or as the struct's bytes)."""
     _fields_ = [("base", ctypes.c_void_p), ("sample_stride", ctypes.c_int64), ("token_stride", ctypes.c_int64),
                 ("head_stride", ctypes.c_int64), ("heads", ctypes.c_int32)]
 
@@ -87,10 +88,10 @@ _SIGNATURES.update({
         _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_void_p,
         _c.c_void_p, _c.c_int64, _c.c_void_p]),
     "lithe_rotate_axes": (_c.c_int32, [
-        _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p,
+        _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p,
         _c.c_int32, _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),
     "lithe_qk_norm_rotate": (_c.c_int32, [
-        _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.POINTER(HeadsView), _c.c_void_p,
+        _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
         _c.c_void_p, _c.c_int32, _c.c_float, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_int32,
         _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),
     "lithe_sgmv_index": (_c.c_int32, [

@@ -9,13 +9,20 @@
 //   Everything in fp32 (the angle's revolution count in fp64, so that far positions keep their
 //   phase), one rounding at the store.
 //
-// Bound: HBM (each value read once and written once; about 3 to 10 operations a value).
-// Split: a warp takes one token (and a run of its heads) at a time.  The lanes that share a
-// head hold 8 of its values each, and hold the cosines and sines of their 4 pairs for all of
-// the token's heads, so the angles cost one evaluation per token and not one per head; the
-// sum of squares is a shuffle inside the lanes of a head.  kBatch heads are loaded before the
-// first is used.
+// Bound: HBM (each value is read once and written once; about 3 to 7 operations a value), with the
+// issue rate close behind: the first form, 19 instructions a value, took 380 us for 14 x 4096 tokens
+// of 24 + 24 heads of 128 where 218 us move the bytes.
+// Split: a warp takes one token (and a run of its heads) at a time.  The lanes that share a head hold
+// 8 of its values each.  A token's cosines and sines are evaluated once, each pair's by one lane,
+// handed round through shared memory, and (with the norm) multiplied by the weights once, so that a
+// pair costs four products two at a time (f32x2), the norm's factor two more.  The sum of squares is
+// a shuffle inside the lanes of a head.  kBatch heads are loaded before the first is used, the
+// token's first ones before its angles.
+// Measured on B200: 14 x 4096 tokens of 24 + 24 heads of 128, norm and rotation, 249 us (5.7 TB/s, 0.88 of
+// the measured copy rate); 32760 tokens of 24 heads, rotation, 64 us (6.3 TB/s, 0.97); one token 3.4 us.
+// A second batch of heads on its way while one is turned took registers that cost more (306 us).
 #include <cmath>
+#include <type_traits>
 
 #include "device_common.cuh"
 #include "host_common.h"
@@ -25,6 +32,7 @@ namespace ra {
 
 constexpr int kMaxPairs = LITHE_MAX_HEAD_DIM / 2;
 constexpr int kBatch = 4;          // heads a lane group loads before it uses the first
+constexpr int kMinBlocks = 4;      // CTAs that have to fit an SM (64 registers a thread)
 constexpr int kWarps = 8;          // warps of a CTA
 
 struct Heads {
@@ -49,7 +57,7 @@ struct Params {
     int32_t chunks;                // units a token is split into
     int32_t group_log2;            // lanes that share a head
     int64_t units;                 // batch * tokens * chunks
-    float eps;
+    float eps, inv_dim;
     uint8_t axis[kMaxPairs];
     double turn[kMaxPairs];        // revolutions per unit of position
 };
@@ -59,24 +67,87 @@ struct Elem;
 template <>
 struct Elem<__nv_bfloat16> {
     static __device__ __forceinline__ float get(__nv_bfloat16 v) { return __bfloat162float(v); }
-    static __device__ __forceinline__ __nv_bfloat16 put(float v) { return __float2bfloat16_rn(v); }
+    static __device__ __forceinline__ __nv_bfloat16 zero() { return __ushort_as_bfloat16(0); }
 };
 template <>
 struct Elem<__half> {
     static __device__ __forceinline__ float get(__half v) { return __half2float(v); }
-    static __device__ __forceinline__ __half put(float v) { return __float2half_rn(v); }
+    static __device__ __forceinline__ __half zero() { return __ushort_as_half(0); }
 };
 template <>
 struct Elem<float> {
     static __device__ __forceinline__ float get(float v) { return v; }
-    static __device__ __forceinline__ float put(float v) { return v; }
+    static __device__ __forceinline__ float zero() { return 0.0f; }
 };
 
-// A lane's 8 values in their stored type: value 2i and 2i + 1 are pair i's.
+// A lane's 8 values in their stored type and order: interleaved, value 2i and 2i + 1 are pair i's; halves,
+// values i and 4 + i.
 template <typename T>
 struct alignas(16) Eight {
     T v[8];
 };
+
+// Two fp32 values that one instruction computes on.
+struct F2 {
+    unsigned long long v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float a, float b) {
+        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    }
+    __device__ __forceinline__ void split(float& a, float& b) const {
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    }
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+
+// The first and second values of a lane's four pairs, two pairs to an F2; and back, rounded.
+template <typename T, bool kHalves>
+__device__ __forceinline__ void unpack(const Eight<T>& e, F2 (&a)[2], F2 (&b)[2]) {
+    float x[8];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = Elem<T>::get(e.v[i]);
+    } else {
+        constexpr bool kF16 = std::is_same<T, __half>::value;
+        const uint32_t* w = reinterpret_cast<const uint32_t*>(&e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = Act<kF16>::lo(w[i]), x[2 * i + 1] = Act<kF16>::hi(w[i]);
+    }
+    constexpr int kStep = kHalves ? 1 : 2, kSecond = kHalves ? 4 : 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        a[i] = F2(x[2 * i * kStep], x[(2 * i + 1) * kStep]);
+        b[i] = F2(x[2 * i * kStep + kSecond], x[(2 * i + 1) * kStep + kSecond]);
+    }
+}
+template <typename T, bool kHalves>
+__device__ __forceinline__ void pack(const F2 (&a)[2], const F2 (&b)[2], Eight<T>& e) {
+    constexpr int kStep = kHalves ? 1 : 2, kSecond = kHalves ? 4 : 1;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        a[i].split(x[2 * i * kStep], x[(2 * i + 1) * kStep]);
+        b[i].split(x[2 * i * kStep + kSecond], x[(2 * i + 1) * kStep + kSecond]);
+    }
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e.v[i] = x[i];
+    } else {
+        constexpr bool kF16 = std::is_same<T, __half>::value;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = Act<kF16>::pack(x[2 * i], x[2 * i + 1]);
+    }
+}
 
 // Offset inside a head of the first and second value of pair p (p < dim / 2).  Pairs from R/2 on
 // are the values that stay, taken two and two.
@@ -93,57 +164,46 @@ __device__ __forceinline__ int second_of(const Params& p, int pair) {
     return pair < h ? pair + h : pair + (p.dim >> 1);
 }
 
-// kVec: the lane's values come as whole 16-byte (interleaved) or 8- / 16-byte (halves) pieces;
-// else one by one, for strides, bases or slices that are not aligned to them.
+// kVec: the lane's values come as whole 16-byte (interleaved) or 8- / 16-byte (halves) pieces, at first
+// and (halves) second; else one by one, for strides, bases or slices that are not aligned to them.
 template <typename T, bool kHalves, bool kVec>
-__device__ __forceinline__ void load8(const Params& p, const T* head, int pair0, Eight<T>& e) {
+__device__ __forceinline__ void load8(const Params& p, const T* head, int pair0, int first, int second, Eight<T>& e) {
     if constexpr (kVec && !kHalves) {
-        const uint4* s = reinterpret_cast<const uint4*>(head + 2 * pair0);
+        const uint4* s = reinterpret_cast<const uint4*>(head + first);
         uint4* d = reinterpret_cast<uint4*>(&e);
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) d[i] = s[i];
     } else if constexpr (kVec) {
         struct alignas(4 * sizeof(T)) Four { T v[4]; };
-        const Four a = *reinterpret_cast<const Four*>(head + first_of<true>(p, pair0));
-        const Four b = *reinterpret_cast<const Four*>(head + second_of<true>(p, pair0));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            e.v[2 * i] = a.v[i];
-            e.v[2 * i + 1] = b.v[i];
-        }
+        reinterpret_cast<Four*>(&e)[0] = *reinterpret_cast<const Four*>(head + first);
+        reinterpret_cast<Four*>(&e)[1] = *reinterpret_cast<const Four*>(head + second);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool in = pair0 + i < (p.dim >> 1);
-            e.v[2 * i] = in ? head[first_of<kHalves>(p, pair0 + i)] : Elem<T>::put(0.0f);
-            e.v[2 * i + 1] = in ? head[second_of<kHalves>(p, pair0 + i)] : Elem<T>::put(0.0f);
+            e.v[kHalves ? i : 2 * i] = in ? head[first_of<kHalves>(p, pair0 + i)] : Elem<T>::zero();
+            e.v[kHalves ? 4 + i : 2 * i + 1] = in ? head[second_of<kHalves>(p, pair0 + i)] : Elem<T>::zero();
         }
     }
 }
 
 template <typename T, bool kHalves, bool kVec>
-__device__ __forceinline__ void store8(const Params& p, T* head, int pair0, const Eight<T>& e) {
+__device__ __forceinline__ void store8(const Params& p, T* head, int pair0, int first, int second, const Eight<T>& e) {
     if constexpr (kVec && !kHalves) {
-        uint4* d = reinterpret_cast<uint4*>(head + 2 * pair0);
+        uint4* d = reinterpret_cast<uint4*>(head + first);
         const uint4* s = reinterpret_cast<const uint4*>(&e);
 #pragma unroll
         for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i) d[i] = s[i];
     } else if constexpr (kVec) {
         struct alignas(4 * sizeof(T)) Four { T v[4]; };
-        Four a, b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            a.v[i] = e.v[2 * i];
-            b.v[i] = e.v[2 * i + 1];
-        }
-        *reinterpret_cast<Four*>(head + first_of<true>(p, pair0)) = a;
-        *reinterpret_cast<Four*>(head + second_of<true>(p, pair0)) = b;
+        *reinterpret_cast<Four*>(head + first) = reinterpret_cast<const Four*>(&e)[0];
+        *reinterpret_cast<Four*>(head + second) = reinterpret_cast<const Four*>(&e)[1];
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             if (pair0 + i < (p.dim >> 1)) {
-                head[first_of<kHalves>(p, pair0 + i)] = e.v[2 * i];
-                head[second_of<kHalves>(p, pair0 + i)] = e.v[2 * i + 1];
+                head[first_of<kHalves>(p, pair0 + i)] = e.v[kHalves ? i : 2 * i];
+                head[second_of<kHalves>(p, pair0 + i)] = e.v[kHalves ? 4 + i : 2 * i + 1];
             }
         }
     }
@@ -155,126 +215,217 @@ __device__ __forceinline__ double position_of(const Params& p, int64_t at) {
     return static_cast<double>(static_cast<const float*>(p.positions)[at]);
 }
 
+// The matrix of each of a lane's pairs, (a, b) -> (aa a - ab b, bb b + ba a): cosine and sine, and with
+// the norm the weights of its two values, whose products are taken once per token.
+struct Turn {
+    F2 aa[2], ab[2], bb[2], ba[2];             // (ab negated)
+};
+
 // One tensor's heads [h0, h1) of one token.  Every lane of the warp runs every iteration (the
 // norm's shuffles need them); lanes without a head or without pairs load and store nothing.
-template <typename T, bool kHalves, bool kVec, bool kNorm>
-__device__ __forceinline__ void token_heads(const Params& p, const Heads& t, int64_t sample, int64_t token, int h0,
-                                            int h1, int lane, int pair0, const float (&cs)[4], const float (&sn)[4],
-                                            const float (&w)[8]) {
-    const int group = 1 << p.group_log2;
+// kWhole: every value of a head is turned; else values that stay never meet an angle (a product with a
+// zero sine would carry a NaN or an infinity across).
+template <typename T>
+struct Batch {
+    Eight<T> e[kBatch];
+};
+
+template <typename T, bool kHalves, bool kVec>
+__device__ __forceinline__ void load_batch(const Params& p, const T* in, int64_t step, int pair0, int first, int second,
+                                           int live, Batch<T>& b) {
     const int per_iter = 32 >> p.group_log2;
-    const bool has_pairs = pair0 < (p.dim >> 1);
-    const T* in = static_cast<const T*>(t.in) + sample * t.in_sample + token * t.in_token;
-    T* out = static_cast<T*>(t.out) + sample * t.out_sample + token * t.out_token;
-    const float inv_dim = 1.0f / static_cast<float>(p.dim);
-    for (int h = h0 + (lane >> p.group_log2); __any_sync(0xffffffffu, h < h1); h += per_iter * kBatch) {
-        Eight<T> e[kBatch];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            const int hj = h + j * per_iter;
-            if (has_pairs && hj < h1)
-                load8<T, kHalves, kVec>(p, in + hj * t.in_head, pair0, e[j]);
-            else
+    for (int j = 0; j < kBatch; ++j) {
+        if (j * per_iter < live)
+            load8<T, kHalves, kVec>(p, in + j * step, pair0, first, second, b.e[j]);
+        else
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[j].v[i] = Elem<T>::put(0.0f);
+            for (int i = 0; i < 8; ++i) b.e[j].v[i] = Elem<T>::zero();
+    }
+}
+
+// live: heads from the lane's first on (0 for a lane without pairs)
+template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole>
+__device__ __forceinline__ void turn_batch(const Params& p, T* out, int64_t step, int pair0, int first, int second,
+                                           int live, const Turn& m, Batch<T>& b) {
+    const int per_iter = 32 >> p.group_log2;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+        F2 x[2], y[2];
+        unpack<T, kHalves>(b.e[j], x, y);
+        float r = 1.0f;
+        if constexpr (kNorm) {
+            F2 sum2 = mul2(x[0], x[0]);
+            sum2 = fma2(x[1], x[1], sum2);
+            sum2 = fma2(y[0], y[0], sum2);
+            sum2 = fma2(y[1], y[1], sum2);
+            float s0, s1;
+            sum2.split(s0, s1);
+            float sum = s0 + s1;
+            for (int o = (1 << p.group_log2) >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            r = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
         }
+        const F2 rr(r, r);
+        F2 u[2], v[2];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-            float x[8];
+        for (int i = 0; i < 2; ++i) {
+            u[i] = fma2(x[i], m.aa[i], mul2(y[i], m.ab[i]));
+            v[i] = fma2(y[i], m.bb[i], mul2(x[i], m.ba[i]));
+            if constexpr (kNorm) u[i] = mul2(u[i], rr), v[i] = mul2(v[i], rr);
+        }
+        if constexpr (kWhole) {
+            pack<T, kHalves>(u, v, b.e[j]);
+        } else {
+            // values that stay: not met by an angle (a product with a zero sine would carry a NaN or an
+            // infinity across), and without the norm not touched at all
+            Eight<T> turned = b.e[j];
+            float xs[4], ys[4], us[4], vs[4];
+            x[0].split(xs[0], xs[1]), x[1].split(xs[2], xs[3]), y[0].split(ys[0], ys[1]), y[1].split(ys[2], ys[3]);
+            u[0].split(us[0], us[1]), u[1].split(us[2], us[3]), v[0].split(vs[0], vs[1]), v[1].split(vs[2], vs[3]);
+            float wa[4], wb[4];
+            m.aa[0].split(wa[0], wa[1]), m.aa[1].split(wa[2], wa[3]);
+            m.bb[0].split(wb[0], wb[1]), m.bb[1].split(wb[2], wb[3]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = Elem<T>::get(e[j].v[i]);
-            if constexpr (kNorm) {
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-                for (int o = group >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                const float r = rsqrtf(fmaf(sum, inv_dim, p.eps));
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * w[i];
-            }
+            for (int i = 0; i < 4; ++i)
+                if (pair0 + i >= (p.rotated >> 1)) us[i] = xs[i] * wa[i] * r, vs[i] = ys[i] * wb[i] * r;
+            u[0] = F2(us[0], us[1]), u[1] = F2(us[2], us[3]), v[0] = F2(vs[0], vs[1]), v[1] = F2(vs[2], vs[3]);
+            pack<T, kHalves>(u, v, turned);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float a = x[2 * i], b = x[2 * i + 1];
-                const bool turned = pair0 + i < (p.rotated >> 1);     // values that stay never meet the angle
-                e[j].v[2 * i] = Elem<T>::put(turned ? a * cs[i] - b * sn[i] : a);
-                e[j].v[2 * i + 1] = Elem<T>::put(turned ? b * cs[i] + a * sn[i] : b);
+                if (!kNorm && pair0 + i >= (p.rotated >> 1)) continue;
+                constexpr int kA = kHalves ? 1 : 2, kB = kHalves ? 4 : 1;
+                b.e[j].v[kA * i] = turned.v[kA * i];
+                b.e[j].v[kA * i + kB] = turned.v[kA * i + kB];
             }
-            const int hj = h + j * per_iter;
-            if (has_pairs && hj < h1) store8<T, kHalves, kVec>(p, out + hj * t.out_head, pair0, e[j]);
         }
+        if (j * per_iter < live) store8<T, kHalves, kVec>(p, out + j * step, pair0, first, second, b.e[j]);
     }
 }
 
-template <typename T, bool kHalves>
-__device__ __forceinline__ void load_weight(const Params& p, const Heads& t, int pair0, float (&w)[8]) {
+// What every unit needs, laid out by pair once per CTA: revolutions per unit of position and axis, the
+// norms' weights of the pair's two values, and a warp's cosines and sines of its token.
+struct Tables {
+    double turn[kMaxPairs];
+    float weight[2][2][kMaxPairs];             // [tensor][first, second][pair]
+    float2 angle[kWarps][kMaxPairs];
+    int32_t axis[kMaxPairs];
+};
+
+template <typename T, bool kHalves, bool kNorm>
+__device__ __forceinline__ void fill_tables(const Params& p, Tables& tab) {
+    for (int pair = threadIdx.x; pair < kMaxPairs; pair += 32 * kWarps) {
+        const bool turned = pair < (p.rotated >> 1), in = pair < (p.dim >> 1);
+        tab.turn[pair] = turned ? p.turn[pair] : 0.0;
+        tab.axis[pair] = turned ? p.axis[pair] : 0;
+        if constexpr (kNorm) {
+            for (int t = 0; t < p.tensors; ++t)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            float v = 1.0f;
-            if (t.weight && pair0 + i < (p.dim >> 1)) {
-                const int at = s ? second_of<kHalves>(p, pair0 + i) : first_of<kHalves>(p, pair0 + i);
-                v = t.weight_f32 ? static_cast<const float*>(t.weight)[at]
-                                 : Elem<T>::get(static_cast<const T*>(t.weight)[at]);
-            }
-            w[2 * i + s] = v;
+                for (int e = 0; e < 2; ++e) {
+                    float v = 1.0f;
+                    if (p.t[t].weight && in) {
+                        const int at = e ? second_of<kHalves>(p, pair) : first_of<kHalves>(p, pair);
+                        v = p.t[t].weight_f32 ? __ldg(static_cast<const float*>(p.t[t].weight) + at)
+                                              : Elem<T>::get(__ldg(static_cast<const T*>(p.t[t].weight) + at));
+                    }
+                    tab.weight[t][e][pair] = v;
+                }
         }
     }
+    __syncthreads();
 }
 
-template <typename T, bool kHalves, bool kVec, bool kNorm>
-__global__ void __launch_bounds__(32 * kWarps) rotate_kernel(const __grid_constant__ Params p) {
+template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole>
+__global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const __grid_constant__ Params p) {
     const int lane = threadIdx.x & 31;
-    const int pair0 = 4 * (lane & ((1 << p.group_log2) - 1));
-    double turn[4];
-    int axis[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const bool in = pair0 + i < (p.rotated >> 1);
-        turn[i] = in ? p.turn[pair0 + i] : 0.0;
-        axis[i] = in ? p.axis[pair0 + i] : 0;
-    }
-    float w0[8], w1[8];
-    if constexpr (kNorm) {
-        load_weight<T, kHalves>(p, p.t[0], pair0, w0);
-        load_weight<T, kHalves>(p, p.t[1], pair0, w1);
-    }
+    const int pair0 = 4 * (lane & ((1 << p.group_log2) - 1)), sub = lane >> p.group_log2;
+    const bool has_pairs = pair0 < (p.dim >> 1);
+    const int first = has_pairs ? first_of<kHalves>(p, pair0) : 0, second = has_pairs ? second_of<kHalves>(p, pair0) : 0;
+    const int per_iter = 32 >> p.group_log2;
+    __shared__ Tables tab;
+    fill_tables<T, kHalves, kNorm>(p, tab);
+    float2* angle = tab.angle[threadIdx.x >> 5];
     const int64_t warps = static_cast<int64_t>(gridDim.x) * kWarps;
     for (int64_t u = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5); u < p.units; u += warps) {
         const int64_t row = u / p.chunks;
         const int chunk = static_cast<int>(u - row * p.chunks);
         const int64_t sample = row / p.tokens, token = row - sample * p.tokens;
-        float cs[4], sn[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // revolutions in fp64, their fraction (at most half a turn) in fp32
-            const double r = position_of(p, sample * p.pos_sample + token * p.axes + axis[i]) * turn[i];
-            sincospif(static_cast<float>(2.0 * (r - rint(r))), &sn[i], &cs[i]);
+        Batch<T> b;
+        int h = chunk * p.t[0].per_unit;
+        {
+            const Heads& t = p.t[0];
+            const int live = has_pairs ? min(h + t.per_unit, t.heads) - h - sub : 0;
+            load_batch<T, kHalves, kVec>(
+                p, static_cast<const T*>(t.in) + sample * t.in_sample + token * t.in_token + (h + sub) * t.in_head,
+                per_iter * t.in_head, pair0, first, second, live, b);
         }
-        int h0 = chunk * p.t[0].per_unit;
-        token_heads<T, kHalves, kVec, kNorm>(p, p.t[0], sample, token, h0, min(h0 + p.t[0].per_unit, p.t[0].heads),
-                                             lane, pair0, cs, sn, w0);
-        if (p.tensors > 1) {
-            h0 = chunk * p.t[1].per_unit;
-            token_heads<T, kHalves, kVec, kNorm>(p, p.t[1], sample, token, h0,
-                                                 min(h0 + p.t[1].per_unit, p.t[1].heads), lane, pair0, cs, sn, w1);
+        // revolutions in fp64, their fraction (at most half a turn) in fp32; each pair's by one lane
+        __syncwarp();
+        for (int pair = lane; pair < (4 << p.group_log2); pair += 32) {
+            float2 a = make_float2(1.0f, 0.0f);
+            if (pair < (p.rotated >> 1)) {
+                const double r =
+                    position_of(p, sample * p.pos_sample + token * p.axes + tab.axis[pair]) * tab.turn[pair];
+                sincospif(static_cast<float>(2.0 * (r - rint(r))), &a.y, &a.x);
+            }
+            angle[pair] = a;
+        }
+        __syncwarp();
+        const float4 a01 = *reinterpret_cast<const float4*>(&angle[pair0]), a23 = *reinterpret_cast<const float4*>(&angle[pair0 + 2]);
+        const float cs[4] = {a01.x, a01.z, a23.x, a23.z}, sn[4] = {a01.y, a01.w, a23.y, a23.w};
+#pragma unroll 1
+        for (int k = 0; k < p.tensors; ++k) {
+            const Heads& t = p.t[k];
+            Turn m;
+            float w[2][4] = {{1.0f, 1.0f, 1.0f, 1.0f}, {1.0f, 1.0f, 1.0f, 1.0f}};
+            if constexpr (kNorm) {
+                *reinterpret_cast<float4*>(w[0]) = *reinterpret_cast<const float4*>(&tab.weight[k][0][pair0]);
+                *reinterpret_cast<float4*>(w[1]) = *reinterpret_cast<const float4*>(&tab.weight[k][1][pair0]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int j = 2 * i;
+                m.aa[i] = F2(cs[j] * w[0][j], cs[j + 1] * w[0][j + 1]), m.ab[i] = F2(-sn[j] * w[1][j], -sn[j + 1] * w[1][j + 1]);
+                m.bb[i] = F2(cs[j] * w[1][j], cs[j + 1] * w[1][j + 1]), m.ba[i] = F2(sn[j] * w[0][j], sn[j + 1] * w[0][j + 1]);
+            }
+            h = chunk * t.per_unit;
+            const int end = min(h + t.per_unit, t.heads);
+            const T* in = static_cast<const T*>(t.in) + sample * t.in_sample + token * t.in_token + (h + sub) * t.in_head;
+            T* out = static_cast<T*>(t.out) + sample * t.out_sample + token * t.out_token + (h + sub) * t.out_head;
+            for (; h < end; h += per_iter * kBatch) {
+                const int live = has_pairs ? end - h - sub : 0;
+                if (k > 0 || h > chunk * t.per_unit)
+                    load_batch<T, kHalves, kVec>(p, in, per_iter * t.in_head, pair0, first, second, live, b);
+                turn_batch<T, kHalves, kVec, kNorm, kWhole>(p, out, per_iter * t.out_head, pair0, first, second, live, m, b);
+                in += kBatch * per_iter * t.in_head;
+                out += kBatch * per_iter * t.out_head;
+            }
         }
     }
 }
 
-template <typename T, bool kHalves, bool kVec, bool kNorm>
+template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole>
 int32_t launch(const Params& p, int sms, cudaStream_t st) {
     const int64_t blocks = (p.units + kWarps - 1) / kWarps;
-    const int64_t most = static_cast<int64_t>(sms) * 8;
-    rotate_kernel<T, kHalves, kVec, kNorm><<<static_cast<int>(blocks < most ? blocks : most), 32 * kWarps, 0, st>>>(p);
+    // (the rotation alone: four CTAs to a place, 126 us against 144 us for 14 x 4608 tokens; with the norm, whose
+    // tables a CTA lays out at its start, one: 246 us against 249 us for 14 x 4096)
+    const int64_t most = static_cast<int64_t>(sms) * kMinBlocks * (kNorm ? 1 : 4);
+    rotate_kernel<T, kHalves, kVec, kNorm, kWhole>
+        <<<static_cast<int>(blocks < most ? blocks : most), 32 * kWarps, 0, st>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "rotate_kernel launch");
 }
 
+template <typename T, bool kNorm, bool kHalves, bool kVec>
+int32_t launch_whole(const Params& p, int sms, cudaStream_t st) {
+    return p.rotated == p.dim ? launch<T, kHalves, kVec, kNorm, true>(p, sms, st)
+                              : launch<T, kHalves, kVec, kNorm, false>(p, sms, st);
+}
+
 template <typename T, bool kNorm>
 int32_t launch_layout(const Params& p, bool halves, bool vec, int sms, cudaStream_t st) {
-    if (halves) return vec ? launch<T, true, true, kNorm>(p, sms, st) : launch<T, true, false, kNorm>(p, sms, st);
-    return vec ? launch<T, false, true, kNorm>(p, sms, st) : launch<T, false, false, kNorm>(p, sms, st);
+    if (halves)
+        return vec ? launch_whole<T, kNorm, true, true>(p, sms, st) : launch<T, true, false, kNorm, false>(p, sms, st);
+    return vec ? launch_whole<T, kNorm, false, true>(p, sms, st) : launch<T, false, false, kNorm, false>(p, sms, st);
 }
 
 // Whether a tensor's heads can be read and written in whole 16-byte pieces.
@@ -369,12 +520,14 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
     p.dim = dim;
     p.rotated = rotated;
     p.eps = eps;
-    // A token's heads are split over warps while there are too few tokens to fill the SMs.
+    p.inv_dim = 1.0f / static_cast<float>(dim);
+    // A token's heads are split over warps while that leaves the SMs room: more units than resident
+    // warps pay their angles for nothing (1024 tokens of 24 heads: 5.9 us on 4 chunks, 13 us on 8).
     const int per_iter = 32 >> lg;
     const int most_chunks = (most_heads + per_iter - 1) / per_iter;
     const int64_t rows = static_cast<int64_t>(batch) * tokens;
     int chunks = 1;
-    while (chunks < most_chunks && rows * chunks < static_cast<int64_t>(sms) * 32) chunks *= 2;
+    while (chunks < most_chunks && rows * chunks * 2 <= static_cast<int64_t>(sms) * kMinBlocks * kWarps) chunks *= 2;
     chunks = chunks < most_chunks ? chunks : most_chunks;
     for (int i = 0; i < tensors; ++i) {
         const int per = (p.t[i].heads + chunks - 1) / chunks;

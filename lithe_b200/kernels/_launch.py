@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
+import struct
 import threading
 from typing import Optional, Sequence
 
@@ -477,24 +478,28 @@ def _heads_strides(t: torch.Tensor) -> tuple:
     return (sb if b != 1 else 0, ss if s != 1 else 0, sh if h != 1 else 0)
 
 
-def _heads_view(t: torch.Tensor) -> _lib.HeadsView:
+_pack_view = struct.Struct("PqqqiI").pack
+
+
+def _heads_view(t: torch.Tensor) -> bytes:
+    """A lithe_heads_view of ``t`` as the bytes of the struct (a fifth of a ctypes object's cost)."""
     b, s, h, _ = t.shape
     sb, ss, sh, _ = t.stride()
-    return _lib.HeadsView(t.data_ptr(), sb if b != 1 else 0, ss if s != 1 else 0, sh if h != 1 else 0, h)
+    return _pack_view(t.data_ptr(), sb if b != 1 else 0, ss if s != 1 else 0, sh if h != 1 else 0, h, 0)
 
 
 def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
     _require_cuda(t, name)
     if t.dtype not in _DTYPE_CODE:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
-    if t.dim() != 4:
-        raise ValueError(f"{name} must be (batch, tokens, heads, dim), got {tuple(t.shape)}")
-    if t.shape[3] > 1 and t.stride(3) != 1:
+    shape = t.shape
+    if len(shape) != 4:
+        raise ValueError(f"{name} must be (batch, tokens, heads, dim), got {tuple(shape)}")
+    if t.stride()[3] != 1 and shape[3] > 1:
         raise ValueError(f"{name}: the values of a head must be contiguous (stride 1), got stride {t.stride(3)}")
-    if like is not None:
-        if t.dtype != like.dtype or t.device != like.device:
-            raise ValueError(f"{name} must have the inputs' type and device ({like.dtype}, {like.device}), got "
-                             f"{t.dtype}, {t.device}")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must have the inputs' type and device ({like.dtype}, {like.device}), got "
+                         f"{t.dtype}, {t.device}")
 
 
 def _byte_span(t: torch.Tensor) -> tuple:
@@ -556,17 +561,20 @@ def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
 def _check_outputs(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], names: Sequence[str]) -> None:
     """Every output is its own input (in place) or shares no element with an input or another output."""
     spans = [_byte_span(t) for t in (*ins, *outs)]
-    for i, (o, name) in enumerate(zip(outs, names)):
+    n = len(ins)
+    for i, o in enumerate(outs):
         if not _has_own_elements(o):
-            raise ValueError(f"{name} has elements that share an address")
-        o0, o1 = spans[len(ins) + i]
-        for j, x in enumerate(ins):
-            if spans[j][1] > o0 and o1 > spans[j][0] and not (i == j and _same_view(o, x)) and not _apart(o, x):
-                raise ValueError(f"{name} overlaps an input (it may be its own input's very view)")
-        for j in range(i):
-            k = len(ins) + j
-            if spans[k][1] > o0 and o1 > spans[k][0] and not _apart(o, outs[j]):
-                raise ValueError(f"{name} overlaps {names[j]}")
+            raise ValueError(f"{names[i]} has elements that share an address")
+        o0, o1 = spans[n + i]
+        for j in range(n + i):
+            x0, x1 = spans[j]
+            if x1 <= o0 or o1 <= x0:
+                continue
+            if j >= n:
+                if not _apart(o, outs[j - n]):
+                    raise ValueError(f"{names[i]} overlaps {names[j - n]}")
+            elif not (i == j and _same_view(o, ins[j])) and not _apart(o, ins[j]):
+                raise ValueError(f"{names[i]} overlaps an input (it may be its own input's very view)")
 
 
 def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta: float, pairing: int) -> tuple:
@@ -585,18 +593,19 @@ def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta:
 
 
 def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], theta: float,
-                 pairing: int, fresh: bool = False) -> torch.Tensor:
-    """lithe_rotate_axes on torch tensors: ``out`` (batch, tokens, heads, dim) is written.  ``fresh``: the
-    caller has checked x and made ``out`` for this call, so that neither needs another look."""
-    if not fresh:
+                 pairing: int, checked: bool = False, fresh: bool = False) -> torch.Tensor:
+    """lithe_rotate_axes on torch tensors: ``out`` (batch, tokens, heads, dim) is written.  ``checked``: the
+    caller has checked x; ``fresh``: and made ``out`` for this call."""
+    if not checked:
         _check_heads(x, "x")
+    if not fresh:
         if out is not x:
             _check_heads(out, "out", x)
             if out.shape != x.shape:
                 raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
         _check_outputs((x,), (out,), ("out",))
     b, s, _, d = x.shape
-    args = (ctypes.byref(_heads_view(x)), ctypes.byref(_heads_view(out)), _DTYPE_CODE[x.dtype], b, s, d,
+    args = (_heads_view(x), _heads_view(out), _DTYPE_CODE[x.dtype], b, s, d,
             *_rotation_args(x, positions, tuple(axes), theta, pairing))
     with device_ctx(x.device):
         rc = _lib.lib().lithe_rotate_axes(*args)
@@ -607,12 +616,14 @@ def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, ax
 
 def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k: torch.Tensor,
                     weight_q: Optional[torch.Tensor], weight_k: Optional[torch.Tensor], positions: torch.Tensor,
-                    axes: Sequence[int], theta: float, eps: float, pairing: int, fresh: bool = False) -> None:
-    """lithe_qk_norm_rotate on torch tensors: ``out_q`` and ``out_k`` are written.  ``fresh``: the caller
-    has checked q and k and made both outputs for this call."""
-    if not fresh:
+                    axes: Sequence[int], theta: float, eps: float, pairing: int, checked: bool = False,
+                    fresh: bool = False) -> None:
+    """lithe_qk_norm_rotate on torch tensors: ``out_q`` and ``out_k`` are written.  ``checked``: the caller
+    has checked q and k; ``fresh``: and made both outputs for this call."""
+    if not checked:
         _check_heads(q, "q")
         _check_heads(k, "k", q)
+    if not fresh:
         _check_heads(out_q, "out_q", q)
         _check_heads(out_k, "out_k", q)
         if out_q.shape != q.shape or out_k.shape != k.shape:
@@ -633,8 +644,7 @@ def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k
         weight_dtype = w.dtype
     if weight_q is not None and weight_k is not None and weight_q.dtype != weight_k.dtype:
         raise TypeError(f"weight_q and weight_k must have one type, got {weight_q.dtype} and {weight_k.dtype}")
-    args = (ctypes.byref(_heads_view(q)), ctypes.byref(_heads_view(k)), ctypes.byref(_heads_view(out_q)),
-            ctypes.byref(_heads_view(out_k)), weight_q.data_ptr() if weight_q is not None else None,
+    args = (_heads_view(q), _heads_view(k), _heads_view(out_q), _heads_view(out_k), weight_q.data_ptr() if weight_q is not None else None,
             weight_k.data_ptr() if weight_k is not None else None, _DTYPE_CODE[weight_dtype], eps,
             _DTYPE_CODE[dtype], b, s, d, *_rotation_args(q, positions, tuple(axes), theta, pairing))
     with device_ctx(q.device):

@@ -60,19 +60,20 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     """
     _launch._check_heads(x, "x")
     _inference_only(x)
-    axes, theta, code = _rotation(x.shape[3], tuple(axes), theta, pairing)
+    compiling = torch.compiler.is_compiling()
+    axes, theta, code = (_rotation.__wrapped__ if compiling else _rotation)(x.shape[3], tuple(axes), theta, pairing)
     fresh = out is None
     if fresh:
         out = x.new_empty(x.shape)
     positions = positions.contiguous()
-    if torch.compiler.is_compiling():
+    if compiling:
         if out is x:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             torch.ops.lithe_b200.rotate_axes_(out, x, positions, list(axes), theta, code)
             return x.copy_(out)
         torch.ops.lithe_b200.rotate_axes_(out, x, positions, list(axes), theta, code)
         return out
-    return _launch.rotate_axes_(x, out, positions, axes, theta, code, fresh)
+    return _launch.rotate_axes_(x, out, positions, axes, theta, code, True, fresh)
 
 
 def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Tensor],
@@ -94,17 +95,18 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
-    axes, theta, code = _rotation(q.shape[3], tuple(axes), theta, pairing)
+    compiling = torch.compiler.is_compiling()
+    axes, theta, code = (_rotation.__wrapped__ if compiling else _rotation)(q.shape[3], tuple(axes), theta, pairing)
     fresh = out_q is None and out_k is None
     if out_q is None:
         out_q = q.new_empty(q.shape)
     if out_k is None:
         out_k = k.new_empty(k.shape)
     positions = positions.contiguous()
-    if torch.compiler.is_compiling():
+    if compiling:
         oq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is q else out_q
         ok = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is k else out_k
         torch.ops.lithe_b200.qk_norm_rotate_(oq, ok, q, k, weight_q, weight_k, positions, list(axes), theta, eps, code)
         return (q.copy_(oq) if out_q is q else oq), (k.copy_(ok) if out_k is k else ok)
-    _launch.qk_norm_rotate_(q, k, out_q, out_k, weight_q, weight_k, positions, axes, theta, eps, code, fresh)
+    _launch.qk_norm_rotate_(q, k, out_q, out_k, weight_q, weight_k, positions, axes, theta, eps, code, True, fresh)
     return out_q, out_k

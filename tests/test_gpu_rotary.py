@@ -140,6 +140,19 @@ def test_no_tokens_and_bad_positions():
     assert got[..., :32].isnan().all() and torch.isfinite(got[..., 32:]).all()
 
 
+def test_bad_positions_leave_the_values_that_stay():
+    q = make((1, 2, 3, 64), torch.bfloat16, 1)
+    pos = torch.tensor([[float("nan"), 1.0], [float("inf"), 1.0]], device=DEV)
+    for pairing in ("interleaved", "halves"):
+        got, _ = qk_norm_rotate(q, q, None, None, pos, (16, 8), pairing=pairing)
+        fine, _ = qk_norm_rotate(q, q, None, None, torch.ones_like(pos), (16, 8), pairing=pairing)
+        bad = torch.zeros(64, dtype=torch.bool, device=DEV)
+        bad[:16] = True
+        if pairing == "halves":
+            bad[8:16], bad[12:20] = False, True
+        assert got[..., bad].isnan().all() and torch.equal(got[..., ~bad], fine[..., ~bad])
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("pairing", ["interleaved", "halves"])
 @pytest.mark.parametrize("b,s,h,kv,d,axes", [
