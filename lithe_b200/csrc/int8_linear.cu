@@ -26,9 +26,12 @@ constexpr int kMaxK = 131072;          // 127 * 127 * kMaxK < 2^31
 // within 2^-21 |t| of halfway is a tie, which goes to the even number, and any other t rounds
 // as the quotient does.
 //
-// Bound: HBM (x read once, a byte a value written).  One CTA a row; a row of up to
-// 8 * kThreadsQ * kChunks values stays in registers between the maximum and the rounding, a
-// longer or unaligned one is read twice (the second time from L2).
+// Bound: HBM (x read once, a byte a value written).  kWarps warps take a row, each lane up to kPieces
+// 8-value pieces of it, which stay in registers between the maximum and the rounding: one warp where
+// there are many rows (57344 x 3072: 80 us, 6.6 TB/s; four a row 102 us), four where there are few and
+// their latency counts (one row 1.8 us; 3.0 us).  A longer row is read twice (the second time from L2).  The quotients of a piece are checked for
+// nearness to halfway together, with a bound (2^-13) above every 2^-21 |t|; the few pieces it stops are
+// done value by value.
 // ------------------------------------------------------------------------------------------
 constexpr int kThreadsQ = 128;
 
@@ -38,9 +41,10 @@ __device__ __forceinline__ float value_of(uint32_t bits) {
     return __uint_as_float(bits << 16);
 }
 
+constexpr float kMagic = 12582912.0f;          // 1.5 * 2^23: adding it rounds to a whole number, ties to even
+
 // Low byte: q of the value x of a row with r = 127 / max (x and r both scaled to keep r finite).
 __device__ __forceinline__ uint32_t quantize(float x, float r) {
-    constexpr float kMagic = 12582912.0f;      // 1.5 * 2^23: adding it rounds to a whole number, ties to even
     const float t = x * r;
     const float s = t + kMagic;
     const float d = fabsf(t - (s - kMagic));
@@ -48,21 +52,10 @@ __device__ __forceinline__ uint32_t quantize(float x, float r) {
     return __float_as_uint(s);
 }
 
-__device__ __forceinline__ uint32_t block_max(uint32_t v) {
-    __shared__ uint32_t part[kThreadsQ / 32];
-    v = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    uint32_t m = part[0];
-#pragma unroll
-    for (int i = 1; i < kThreadsQ / 32; ++i) m = max(m, part[i]);
-    return m;
-}
-
 // The row's scale (written by one thread) and the two factors of a value's quotient.  A row with
 // an infinity or NaN gets scale NaN (its outputs are NaN) and zeros.
 template <bool kF16>
-__device__ __forceinline__ void row_factors(uint32_t max_bits, float* scale, float& pre, float& r) {
+__device__ __forceinline__ void row_factors(uint32_t max_bits, bool write, float* scale, float& pre, float& r) {
     const float most = value_of<kF16>(max_bits);
     const bool finite = max_bits < (kF16 ? 0x7c00u : 0x7f80u);
     pre = 1.0f;
@@ -71,7 +64,7 @@ __device__ __forceinline__ void row_factors(uint32_t max_bits, float* scale, flo
         if (most < 0x1p-64f) pre = 0x1p+64f;          // keeps 127 / max finite
         r = __fdiv_rn(127.0f, most * pre);
     }
-    if (threadIdx.x == 0) *scale = finite ? __fdiv_rn(most, 127.0f) : __uint_as_float(0x7fffffffu);
+    if (write) *scale = finite ? __fdiv_rn(most, 127.0f) : __uint_as_float(0x7fffffffu);
     if (!finite) pre = 0.0f;
 }
 
@@ -88,44 +81,99 @@ template <bool kF16>
 __device__ __forceinline__ uint2 quantize8(const uint4& v, float pre, float r) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t b[8];
+    float near = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        b[2 * i] = quantize(value_of<kF16>(w[i] & 0xffffu) * pre, r);
-        b[2 * i + 1] = quantize(value_of<kF16>(w[i] >> 16) * pre, r);
+    for (int i = 0; i < 8; ++i) {
+        const float t = value_of<kF16>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu) * r;
+        const float s = t + kMagic;
+        near = fmaxf(near, fabsf(t - (s - kMagic)));
+        b[i] = __float_as_uint(s);
+    }
+    if (near > 0.5f - 0x1p-13f || pre != 1.0f) {       // (pre: rows of values below 2^-64)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            b[i] = quantize(value_of<kF16>(i & 1 ? w[i >> 1] >> 16 : w[i >> 1] & 0xffffu) * pre, r);
     }
     const uint32_t a0 = __byte_perm(b[0], b[1], 0x0040), a1 = __byte_perm(b[2], b[3], 0x0040);
     const uint32_t a2 = __byte_perm(b[4], b[5], 0x0040), a3 = __byte_perm(b[6], b[7], 0x0040);
     return make_uint2(__byte_perm(a0, a1, 0x5410), __byte_perm(a2, a3, 0x5410));
 }
 
-template <bool kF16, int kChunks>
+template <bool kF16, int kWarps, int kPieces>
 __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    const int64_t row = blockIdx.x;
+    constexpr int kLanes = 32 * kWarps, kRowsCta = kThreadsQ / kLanes;
+    __shared__ uint32_t part[kThreadsQ / 32];
+    const int warp = threadIdx.x >> 5, at0 = threadIdx.x % kLanes;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsCta + threadIdx.x / kLanes;
+    const bool live = row < p.rows;
     const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_stride);
-    uint2* q = reinterpret_cast<uint2*>(p.q + row * p.q_stride);
-    const int chunks = p.k >> 3;
-    uint4 v[kChunks];
+    const int pieces = live ? p.k >> 3 : 0;
+    uint4 v[kPieces];
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const int at = c * kThreadsQ + threadIdx.x;
-        v[c] = at < chunks ? __ldg(x + at) : make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < kPieces; ++c) {
+        const int at = c * kLanes + at0;
+        v[c] = at < pieces ? __ldg(x + at) : make_uint4(0, 0, 0, 0);
     }
     uint32_t m = 0;
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
+    for (int c = 0; c < kPieces; ++c)
         m = __vmaxu2(__vmaxu2(m, __vmaxu2(v[c].x & 0x7fff7fffu, v[c].y & 0x7fff7fffu)),
                      __vmaxu2(v[c].z & 0x7fff7fffu, v[c].w & 0x7fff7fffu));
-    m = block_max(max(m & 0xffffu, m >> 16));
-    float pre, r;
-    row_factors<kF16>(m, p.scale + row, pre, r);
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+    if constexpr (kWarps > 1) {
+        if ((threadIdx.x & 31) == 0) part[warp] = m;
+        __syncthreads();
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c) {
-        const int at = c * kThreadsQ + threadIdx.x;
-        if (at < chunks) q[at] = pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r);
+        for (int i = 0; i < kWarps; ++i) m = max(m, part[warp / kWarps * kWarps + i]);
+    }
+    if (!live) return;
+    float pre, r;
+    row_factors<kF16>(m, at0 == 0, p.scale + row, pre, r);
+    uint2* q = reinterpret_cast<uint2*>(p.q + row * p.q_stride);
+#pragma unroll
+    for (int c = 0; c < kPieces; ++c) {
+        const int at = c * kLanes + at0;
+        if (at < pieces) q[at] = pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r);
     }
 }
 
+__device__ __forceinline__ uint32_t block_max(uint32_t v) {
+    __shared__ uint32_t part[kThreadsQ / 32];
+    v = __reduce_max_sync(0xffffffffu, v);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    uint32_t m = part[0];
+#pragma unroll
+    for (int i = 1; i < kThreadsQ / 32; ++i) m = max(m, part[i]);
+    return m;
+}
+
+// Rows that start anywhere, value by value.  Short ones: a warp a row, each lane kValues of it in
+// registers (20000 x 100: 6.3 us, 21 us by the kernel below).
+template <bool kF16, int kValues>
+__global__ void __launch_bounds__(kThreadsQ) quantize_short_kernel(const QuantParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreadsQ / 32) + (threadIdx.x >> 5);
+    if (row >= p.rows) return;
+    const uint16_t* x = p.x + row * p.x_stride;
+    uint32_t v[kValues], m = 0;
+#pragma unroll
+    for (int c = 0; c < kValues; ++c) v[c] = 32 * c + lane < p.k ? __ldg(x + 32 * c + lane) : 0u;
+#pragma unroll
+    for (int c = 0; c < kValues; ++c) m = max(m, v[c] & 0x7fffu);
+    m = __reduce_max_sync(0xffffffffu, m);
+    float pre, r;
+    row_factors<kF16>(m, lane == 0, p.scale + row, pre, r);
+    int8_t* q = p.q + row * p.q_stride;
+#pragma unroll
+    for (int c = 0; c < kValues; ++c)
+        if (32 * c + lane < p.k)
+            q[32 * c + lane] = pre == 0.0f ? 0 : static_cast<int8_t>(quantize(value_of<kF16>(v[c]) * pre, r) & 0xffu);
+}
+
+// Longer ones: a CTA a row, read twice.
 template <bool kF16>
 __global__ void __launch_bounds__(kThreadsQ) quantize_any_kernel(const QuantParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -136,7 +184,7 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_any_kernel(const QuantPara
     for (int i = threadIdx.x; i < p.k; i += kThreadsQ) m = max(m, static_cast<uint32_t>(__ldg(x + i)) & 0x7fffu);
     m = block_max(m);
     float pre, r;
-    row_factors<kF16>(m, p.scale + row, pre, r);
+    row_factors<kF16>(m, threadIdx.x == 0, p.scale + row, pre, r);
     for (int i = threadIdx.x; i < p.k; i += kThreadsQ)
         q[i] = pre == 0.0f ? 0 : static_cast<int8_t>(quantize(value_of<kF16>(__ldg(x + i)) * pre, r) & 0xffu);
 }
@@ -1073,15 +1121,32 @@ int32_t launch_linear(const Params& p, bool after_quantize, cudaStream_t st) {
                 : launch_tiles<false, kF16, kExpandNone>(p, device, sms, after_quantize, st);
 }
 
+template <bool kF16, int kWarps, int kPieces>
+void launch_quantize_rows(const QuantParams& p, cudaStream_t st) {
+    constexpr int kRowsCta = kThreadsQ / (32 * kWarps);
+    quantize_kernel<kF16, kWarps, kPieces><<<static_cast<int>((static_cast<int64_t>(p.rows) + kRowsCta - 1) / kRowsCta), kThreadsQ, 0, st>>>(p);
+}
+
 template <bool kF16>
 int32_t launch_quantize(const QuantParams& p, cudaStream_t st) {
     // whole 16-byte pieces of x to whole 8-byte pieces of q
     const bool vec = p.k % 8 == 0 && p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
-    const int chunks = (p.k / 8 + kThreadsQ - 1) / kThreadsQ;
-    if (vec && chunks <= 2) quantize_kernel<kF16, 2><<<p.rows, kThreadsQ, 0, st>>>(p);
-    else if (vec && chunks <= 4) quantize_kernel<kF16, 4><<<p.rows, kThreadsQ, 0, st>>>(p);
-    else if (vec && chunks <= 8) quantize_kernel<kF16, 8><<<p.rows, kThreadsQ, 0, st>>>(p);
-    else if (vec && chunks <= 16) quantize_kernel<kF16, 16><<<p.rows, kThreadsQ, 0, st>>>(p);
+    const int pieces = p.k / 8;
+    // (3072 values: four warps a row are faster up to 1024 rows, and one from 4096 on)
+    const bool few = p.rows <= 2048;
+    const int four = static_cast<int>((static_cast<int64_t>(p.rows) + 3) / 4);
+    if (!vec && p.k <= 32 * 4) quantize_short_kernel<kF16, 4><<<four, kThreadsQ, 0, st>>>(p);
+    else if (!vec && p.k <= 32 * 16) quantize_short_kernel<kF16, 16><<<four, kThreadsQ, 0, st>>>(p);
+    else if (!vec) quantize_any_kernel<kF16><<<p.rows, kThreadsQ, 0, st>>>(p);
+    else if (few && pieces <= 128 * 4) launch_quantize_rows<kF16, 4, 4>(p, st);
+    else if (pieces <= 32 * 4) launch_quantize_rows<kF16, 1, 4>(p, st);
+    else if (pieces <= 32 * 8) launch_quantize_rows<kF16, 1, 8>(p, st);
+    else if (pieces <= 32 * 12) launch_quantize_rows<kF16, 1, 12>(p, st);
+    else if (pieces <= 64 * 8) launch_quantize_rows<kF16, 2, 8>(p, st);
+    else if (pieces <= 64 * 12) launch_quantize_rows<kF16, 2, 12>(p, st);
+    else if (pieces <= 128 * 8) launch_quantize_rows<kF16, 4, 8>(p, st);
+    else if (pieces <= 128 * 12) launch_quantize_rows<kF16, 4, 12>(p, st);
+    else if (pieces <= 128 * 16) launch_quantize_rows<kF16, 4, 16>(p, st);
     else quantize_any_kernel<kF16><<<p.rows, kThreadsQ, 0, st>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "quantize_kernel launch");
