@@ -417,10 +417,11 @@ LITHE_API int64_t lithe_int8_workspace_bytes(int32_t rows, int32_t k);
 
 /*
  * lithe_quantize_rows and lithe_int8_linear in one call: the same results, with the second launch's
- * start overlapping the first kernel.
+ * start overlapping the first kernel; or, for a single row, one launch that quantises it itself.
  *   x            device (rows, k) of dtype, rows x_stride elements apart
  *   workspace    device, 16-byte aligned, >= lithe_int8_workspace_bytes(rows, k); contents on entry do
- *                not matter; calls sharing one workspace must be ordered on one stream
+ *                not matter; calls sharing one workspace must be ordered on one stream.  Unused (may be
+ *                NULL) for one row of at most 16384 values, k a multiple of 8, x on a 16-byte boundary.
  */
 LITHE_API int32_t lithe_int8_linear_dynamic(const void* x, int64_t x_stride, const void* w, int64_t w_stride,
                         const float* w_scale, const void* bias, void* out, int32_t dtype, int32_t rows, int32_t n,

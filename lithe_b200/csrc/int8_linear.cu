@@ -29,9 +29,9 @@ constexpr int kMaxK = 131072;          // 127 * 127 * kMaxK < 2^31
 // Bound: HBM (x read once, a byte a value written).  kWarps warps take a row, each lane up to kPieces
 // 8-value pieces of it, which stay in registers between the maximum and the rounding: one warp where
 // there are many rows (57344 x 3072: 80 us, 6.6 TB/s; four a row 102 us), four where there are few and
-// their latency counts (one row 1.8 us; 3.0 us).  A longer row is read twice (the second time from L2).  The quotients of a piece are checked for
-// nearness to halfway together, with a bound (2^-13) above every 2^-21 |t|; the few pieces it stops are
-// done value by value.
+// their latency counts (one row 1.8 us; 3.0 us).  A longer row is read twice (the second time from L2).
+// The quotients of a piece are checked for nearness to halfway together, with a bound (2^-13) above every
+// 2^-21 |t|; the few pieces it stops are done value by value.
 // ------------------------------------------------------------------------------------------
 constexpr int kThreadsQ = 128;
 
@@ -193,7 +193,8 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_any_kernel(const QuantPara
 // lithe_int8_linear
 // ------------------------------------------------------------------------------------------
 struct Params {
-    const int8_t* q;               // (rows, k), row stride q_stride
+    const int8_t* q;               // (rows, k), row stride q_stride; or nullptr, and
+    const uint16_t* x;             // the activations themselves (direct_row)
     const int8_t* w;               // (n, k), row stride w_stride
     const float* x_scale;          // (rows)
     const float* w_scale;          // (n)
@@ -288,37 +289,72 @@ constexpr int kMaxSplit = 16;                  // warps that share a channel til
 constexpr int kRowWarps = 32;                  // per SM
 constexpr int kUnroll = 2;                     // 64-byte pieces a warp loads before it uses the first
 
-template <bool kF16, int kTiles>
+// kDirect: a single row, quantised here instead of in a launch of its own: every CTA needs it, and reads it
+// from L2 while its first weights come from HBM (3072 -> 3072: 5.2 us, 6.7 us in two launches; two rows of
+// 3072 -> 18432 are slower so, 15.2 us and 14.2 us).
+constexpr int kDirectMost = 16384;             // values of the row
+
+// p's row (k a multiple of 8, on a 16-byte boundary) as int8, zeros up to the next 16, in shared memory, and
+// its scale; every thread of the CTA takes part.
+template <bool kF16>
+__device__ __forceinline__ void quantize_here(const Params& p, int8_t* q, float* scale, uint32_t* part) {
+    const uint4* x = reinterpret_cast<const uint4*>(p.x);
+    uint32_t m = 0;
+    for (int at = threadIdx.x; at < p.k >> 3; at += blockDim.x) {
+        const uint4 v = __ldg(x + at);
+        m = __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)),
+                     __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+    }
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int i = 0; i < static_cast<int>(blockDim.x >> 5); ++i) m = max(m, part[i]);
+    float pre, r;
+    row_factors<kF16>(m, threadIdx.x == 0, scale, pre, r);
+    for (int at = threadIdx.x; at < (p.k + 15) / 16 * 2; at += blockDim.x)
+        *reinterpret_cast<uint2*>(q + 8 * at) =
+            at < p.k >> 3 && pre != 0.0f ? quantize8<kF16>(__ldg(x + at), pre, r) : make_uint2(0, 0);
+    __syncthreads();
+}
+
+template <bool kF16, int kTiles, bool kDirect>
 __global__ void __launch_bounds__(32 * kMaxSplit, 2) int8_rows_kernel(const Params p) {
     extern __shared__ int part_raw[];
+    __shared__ float scale;
+    __shared__ uint32_t row_max[kMaxSplit];
     int(*part)[8 * kTiles][17] = reinterpret_cast<int(*)[8 * kTiles][17]>(part_raw);   // [warp][row][channel]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, kq = 16 * (lane & 3);
     const int split = blockDim.x >> 5, n0 = blockIdx.x * 16;
+    int8_t* here = reinterpret_cast<int8_t*>(part + split);                            // kDirect: the row's q
     const int8_t* w0 = p.w + static_cast<int64_t>(n0 + g) * p.w_stride;
     const int8_t* w1 = w0 + 8 * p.w_stride;
     const bool in0 = n0 + g < p.n, in1 = n0 + g + 8 < p.n;
     int acc[kTiles][4] = {};
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    bool waited = false;
-    for (int k0 = 128 * warp; k0 < p.k; k0 += 128 * split) {
-        uint4 a0[kUnroll], a1[kUnroll], b[kUnroll][kTiles];
+    uint4 a0[kUnroll], a1[kUnroll], b[kUnroll][kTiles];
+    const auto load_weights = [&](int k0) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int k = k0 + 64 * u + kq;
             a0[u] = in0 && k < p.k ? load16<true>(w0, k, p.k) : zero;
             a1[u] = in1 && k < p.k ? load16<true>(w1, k, p.k) : zero;
         }
-        if (!waited) {                         // the first weights are on their way while the quantisation ends
-            grid_dependency_wait();
-            waited = true;
-        }
+    };
+    load_weights(128 * warp);                  // on their way while the rows are quantised
+    if constexpr (kDirect) quantize_here<kF16>(p, here, &scale, row_max);
+    else grid_dependency_wait();
+    for (int k0 = 128 * warp; k0 < p.k; k0 += 128 * split) {
+        if (k0 > 128 * warp) load_weights(k0);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int k = k0 + 64 * u + kq;
 #pragma unroll
             for (int t = 0; t < kTiles; ++t) {
                 const int r = 8 * t + g;
-                b[u][t] = r < p.rows && k < p.k ? load16<false>(p.q + r * p.q_stride, k, p.k) : zero;
+                b[u][t] = zero;
+                if (r < p.rows && k < p.k)
+                    b[u][t] = kDirect ? *reinterpret_cast<const uint4*>(here + k)
+                                      : load16<false>(p.q + r * p.q_stride, k, p.k);
             }
         }
 #pragma unroll
@@ -329,7 +365,6 @@ __global__ void __launch_bounds__(32 * kMaxSplit, 2) int8_rows_kernel(const Para
                 mma_s8(acc[t], a0[u].z, a1[u].z, a0[u].w, a1[u].w, b[u][t].z, b[u][t].w);
             }
     }
-    grid_dependency_wait();
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -341,13 +376,19 @@ __global__ void __launch_bounds__(32 * kMaxSplit, 2) int8_rows_kernel(const Para
         if (r >= p.rows || n >= p.n) continue;
         int sum = 0;
         for (int i = 0; i < split; ++i) sum += part[i][r][e & 15];
-        float y = fmaf(static_cast<float>(sum) * p.x_scale[r], p.w_scale[n], p.bias ? value_of<kF16>(p.bias[n]) : 0.0f);
+        const float sx = kDirect ? scale : p.x_scale[r];
+        float y = fmaf(static_cast<float>(sum) * sx, p.w_scale[n], p.bias ? value_of<kF16>(p.bias[n]) : 0.0f);
         if (p.h) y = expand_of(p, r, n, y);
         p.out[static_cast<int64_t>(r) * p.n + n] = static_cast<uint16_t>(Act<kF16>::pack(y, 0.0f) & 0xffffu);
     }
 }
 
-template <bool kF16, int kTiles>
+// Whether p's activations are quantised by the few-row kernel itself.
+bool direct_row(const Params& p) {
+    return p.rows == 1 && p.k <= kDirectMost && p.k % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+}
+
+template <bool kF16, int kTiles, bool kDirect>
 int32_t launch_rows(const Params& p, int sms, bool after_quantize, cudaStream_t st) {
     const int tiles = (p.n + 15) / 16, pairs = (p.k + 127) / 128;
     int split = static_cast<int>(static_cast<int64_t>(sms) * kRowWarps / tiles);
@@ -355,9 +396,11 @@ int32_t launch_rows(const Params& p, int sms, bool after_quantize, cudaStream_t 
     split = split < pairs ? split : pairs;
     const int share = (pairs + split - 1) / split;
     split = (pairs + share - 1) / share;           // no more warps than their share of the pieces needs
-    Launch l(tiles, 32 * split, split * 8 * kTiles * 17 * sizeof(int), st);
+    const int sums = split * 8 * kTiles * 17 * static_cast<int>(sizeof(int));
+    static_assert(8 * kTiles * 17 * sizeof(int) % 16 == 0, "the row behind the sums stays aligned");
+    Launch l(tiles, 32 * split, sums + (kDirect ? (p.k + 15) / 16 * 16 : 0), st);
     if (after_quantize) l.after_last();
-    const cudaError_t e = cudaLaunchKernelEx(&l.config, int8_rows_kernel<kF16, kTiles>, p);
+    const cudaError_t e = cudaLaunchKernelEx(&l.config, int8_rows_kernel<kF16, kTiles, kDirect>, p);
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "int8_rows_kernel launch");
 }
 
@@ -1106,8 +1149,9 @@ int32_t launch_linear(const Params& p, bool after_quantize, cudaStream_t st) {
     const int32_t rc = current_device_sms(&device, &sms);
     if (rc != LITHE_OK) return rc;
     // (14 x 3072 -> 18432: 13.4 us, 18.4 us on the tile kernel; 32 x 3072 -> 18432: 21.7 us and 18.4 us)
-    if (p.rows <= 8) return launch_rows<kF16, 1>(p, sms, after_quantize, st);
-    if (p.rows <= 16) return launch_rows<kF16, 2>(p, sms, after_quantize, st);
+    if (!p.q) return launch_rows<kF16, 1, true>(p, sms, false, st);
+    if (p.rows <= 8) return launch_rows<kF16, 1, false>(p, sms, after_quantize, st);
+    if (p.rows <= 16) return launch_rows<kF16, 2, false>(p, sms, after_quantize, st);
     // Pairs once their 256 x 256 tiles fill the GPU; 128 x 128 tiles before, to use more SMs.
     const int64_t pair_tiles = static_cast<int64_t>((p.rows + 255) / 256) * ((p.n + 255) / 256);
     const bool pair = pair_tiles >= sms / 2;
@@ -1278,6 +1322,9 @@ extern "C" int32_t lithe_int8_linear_dynamic(const void* x, int64_t x_stride, co
                                err_flag);
     if (rc != LITHE_OK || rows == 0) return rc;
     if ((rc = check_x(x, x_stride)) != LITHE_OK) return rc;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    p.x = static_cast<const uint16_t*>(x);
+    if (direct_row(p)) return linear(p, dtype, false, st);
     const int64_t need = lithe_int8_workspace_bytes(rows, k);
     if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 || workspace_bytes < need)
         return fail_arg("workspace must be 16-byte aligned and hold %lld bytes, got %lld", static_cast<long long>(need),
@@ -1285,7 +1332,6 @@ extern "C" int32_t lithe_int8_linear_dynamic(const void* x, int64_t x_stride, co
     const int64_t q_stride = (static_cast<int64_t>(k) + 15) / 16 * 16;
     int8_t* q = static_cast<int8_t*>(workspace);
     float* scale = reinterpret_cast<float*>(q + rows * q_stride);
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
     rc = quantize(QuantParams{static_cast<const uint16_t*>(x), q, scale, x_stride, q_stride, rows, k}, dtype, st);
     if (rc != LITHE_OK) return rc;
     p.q = q;

@@ -782,13 +782,17 @@ def int8_linear_dynamic(x: torch.Tensor, weight: torch.Tensor, weight_scale: tor
     out = x.new_empty((*shape[:-1], n))
     if rows == 0:
         return out
-    q_bytes = rows * padded(k)
-    space = torch.empty(q_bytes + 4 * rows, dtype=torch.uint8, device=dev)
+    x_ptr = x.data_ptr()
+    if rows == 1 and k <= 16384 and not (k % 8 or x_ptr % 16):
+        space, size = None, 0           # the kernel quantises such a row itself
+    else:
+        size = rows * (padded(k) + 4)
+        space = torch.empty(size, dtype=torch.uint8, device=dev)
     with device_ctx(dev):
         rc = _lib.lib().lithe_int8_linear_dynamic(
-            x.data_ptr(), x_stride, weight.data_ptr(), w_stride, weight_scale.data_ptr(),
+            x_ptr, x_stride, weight.data_ptr(), w_stride, weight_scale.data_ptr(),
             bias.data_ptr() if bias is not None else None, out.data_ptr(), _DTYPE_CODE[dtype], rows, n, k, *expand,
-            error_word(dev).data_ptr(), space.data_ptr(), q_bytes + 4 * rows, stream_handle(dev))
+            error_word(dev).data_ptr(), space.data_ptr() if space is not None else None, size, stream_handle(dev))
     if rc:
         _lib.check(rc, "lithe_int8_linear_dynamic")
     return out

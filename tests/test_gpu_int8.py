@@ -105,7 +105,7 @@ def test_extreme_rows():
         assert torch.equal(got.q[fine].double(), q) and torch.equal(got.scale[fine], s.float())
 
 
-SHAPES = [(1, 1, 1), (1, 17, 64), (3, 16, 31), (7, 100, 130), (8, 264, 3072), (9, 256, 128), (14, 300, 1000), (16, 64, 16),
+SHAPES = [(1, 1, 1), (1, 17, 64), (2, 40, 8), (4, 300, 4096), (4, 24, 4104), (3, 1091, 1000), (1, 16, 16384), (2, 3000, 136), (3, 16, 31), (7, 100, 130), (8, 264, 3072), (9, 256, 128), (14, 300, 1000), (16, 64, 16),
           (17, 512, 256), (31, 33, 65), (33, 1091, 200), (64, 256, 64), (100, 264, 1898), (127, 72, 400), (128, 256, 128),
           (129, 128, 4096), (200, 1091, 130), (255, 520, 512), (256, 256, 128), (257, 8, 1000), (300, 1000, 96),
           (513, 248, 640), (1000, 768, 1024), (1237, 1091, 1898), (2048, 3072, 320), (1, 3072, 12288), (14, 18432, 192)]
