@@ -25,6 +25,8 @@ import torch
 import torch.nn.functional as F
 from torch import nn
 
+from .kernels import qk_norm_rotate
+
 
 @dataclass
 class FluxConfig:
@@ -37,6 +39,9 @@ class FluxConfig:
     text_dim: int = 4096
     pooled_dim: int = 768
     time_dim: int = 256
+    # q and k normalised, rotated and laid into the joint sequence by ``kernels.qk_norm_rotate`` (one pass
+    # in place of the norms', the rotation's and the concatenations'); off: the plain torch form
+    fused_qk: bool = False
 
     @classmethod
     def tiny(cls) -> "FluxConfig":
@@ -99,6 +104,22 @@ def _mod(x, shift, scale):
     return x * (1 + scale[:, None]) + shift[:, None]
 
 
+def rope_axes(head_dim: int) -> tuple:
+    """The values of a head that the index, row and column axes turn (16, 56 and 56 of 128)."""
+    return (head_dim // 8, 7 * head_dim // 16, head_dim - head_dim // 8 - 7 * head_dim // 16)
+
+
+def rope_positions(n_txt: int, n_img: int, device) -> torch.Tensor:
+    """(n_txt + n_img, 3) int32 positions (index, row, column) of the joint [text; image] sequence: the
+    ids of ``rope_tables`` as whole numbers."""
+    w = max(1, math.ceil(math.sqrt(n_img)))
+    idx = torch.arange(n_img, device=device)
+    ids = torch.zeros(n_txt + n_img, 3, device=device, dtype=torch.int32)
+    ids[n_txt:, 1] = idx // w
+    ids[n_txt:, 2] = idx % w
+    return ids
+
+
 def rope_tables(n_txt: int, n_img: int, head_dim: int, device, theta: float = 10000.0):
     """(cos, sin), each (n_txt + n_img, head_dim / 2) fp32, for the joint [text; image] sequence.
 
@@ -106,7 +127,7 @@ def rope_tables(n_txt: int, n_img: int, head_dim: int, device, theta: float = 10
     (0, i // w, i % w) on a grid of width w = ceil(sqrt(n_img)).  Each axis owns a slice of the
     head's rotation pairs (16 / 56 / 56 of 128 dims), with frequencies theta^(-2j / axis_dim).
     """
-    axes = (head_dim // 8, 7 * head_dim // 16, head_dim - head_dim // 8 - 7 * head_dim // 16)
+    axes = rope_axes(head_dim)
     w = max(1, math.ceil(math.sqrt(n_img)))
     idx = torch.arange(n_img, device=device)
     ids = torch.zeros(n_txt + n_img, 3, device=device, dtype=torch.float32)
@@ -148,6 +169,23 @@ def _attend(q, k, v, heads, rope=None):
     return o.transpose(1, 2).reshape(b, s, d)
 
 
+def _attend_joint(parts, heads, positions):
+    """Attention over the joint sequence of ``parts``, each (q, k, v, norm of q, norm of k) of one stream
+    straight from its projections: ``qk_norm_rotate`` writes every stream's q and k into its place."""
+    b, d = parts[0][0].shape[0], parts[0][0].shape[2]
+    hd = d // heads
+    q, k = (parts[0][0].new_empty(b, positions.shape[0], heads, hd) for _ in range(2))
+    at = 0
+    for sq, sk, _, nq, nk in parts:
+        end = at + sq.shape[1]
+        qk_norm_rotate(sq.view(b, -1, heads, hd), sk.view(b, -1, heads, hd), nq.weight, nk.weight, positions[at:end],
+                       rope_axes(hd), out_q=q[:, at:end], out_k=k[:, at:end])
+        at = end
+    v = parts[0][2] if len(parts) == 1 else torch.cat([p[2] for p in parts], 1)
+    q, k, v = (t.transpose(1, 2) for t in (q, k, v.view(b, -1, heads, hd)))
+    return F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(b, -1, d)
+
+
 class JointAttention(nn.Module):
     def __init__(self, dim: int, heads: int, context: bool):
         super().__init__()
@@ -175,6 +213,7 @@ class DoubleBlock(nn.Module):
         d = cfg.hidden
         self.norm1, self.norm1_context = AdaNorm(d, 6), AdaNorm(d, 6)
         self.attn = JointAttention(d, cfg.heads, context=True)
+        self.fused_qk = cfg.fused_qk
         self.ff = FeedForward(d, d * cfg.mlp_ratio)
         self.ff_context = FeedForward(d, d * cfg.mlp_ratio)
 
@@ -184,9 +223,13 @@ class DoubleBlock(nn.Module):
         a = self.attn
         xi = _mod(_ln(img), sh, sc)
         xt = _mod(_ln(txt), csh, csc)
-        qi, ki, vi = a._qkv(xi, a.to_q, a.to_k, a.to_v, a.norm_q, a.norm_k)
-        qt, kt, vt = a._qkv(xt, a.add_q_proj, a.add_k_proj, a.add_v_proj, a.norm_added_q, a.norm_added_k)
-        o = _attend(torch.cat([qt, qi], 1), torch.cat([kt, ki], 1), torch.cat([vt, vi], 1), a.heads, rope)
+        if self.fused_qk:
+            o = _attend_joint([(a.add_q_proj(xt), a.add_k_proj(xt), a.add_v_proj(xt), a.norm_added_q, a.norm_added_k),
+                               (a.to_q(xi), a.to_k(xi), a.to_v(xi), a.norm_q, a.norm_k)], a.heads, rope)
+        else:
+            qi, ki, vi = a._qkv(xi, a.to_q, a.to_k, a.to_v, a.norm_q, a.norm_k)
+            qt, kt, vt = a._qkv(xt, a.add_q_proj, a.add_k_proj, a.add_v_proj, a.norm_added_q, a.norm_added_k)
+            o = _attend(torch.cat([qt, qi], 1), torch.cat([kt, ki], 1), torch.cat([vt, vi], 1), a.heads, rope)
         ot, oi = o[:, : txt.shape[1]], o[:, txt.shape[1]:]
         img = img + g[:, None] * a.to_out[0](oi.contiguous())
         txt = txt + cg[:, None] * a.to_add_out(ot.contiguous())
@@ -201,6 +244,7 @@ class SingleBlock(nn.Module):
         d = cfg.hidden
         self.norm = AdaNorm(d, 3)
         self.attn = JointAttention(d, cfg.heads, context=False)
+        self.fused_qk = cfg.fused_qk
         self.proj_mlp = nn.Linear(d, d * cfg.mlp_ratio)
         self.proj_out = nn.Linear(d + d * cfg.mlp_ratio, d)
 
@@ -208,8 +252,11 @@ class SingleBlock(nn.Module):
         sh, sc, g = self.norm(temb)
         h = _mod(_ln(x), sh, sc)
         a = self.attn
-        q, k, v = a._qkv(h, a.to_q, a.to_k, a.to_v, a.norm_q, a.norm_k)
-        o = _attend(q, k, v, a.heads, rope)
+        if self.fused_qk:
+            o = _attend_joint([(a.to_q(h), a.to_k(h), a.to_v(h), a.norm_q, a.norm_k)], a.heads, rope)
+        else:
+            q, k, v = a._qkv(h, a.to_q, a.to_k, a.to_v, a.norm_q, a.norm_k)
+            o = _attend(q, k, v, a.heads, rope)
         mlp = F.gelu(self.proj_mlp(h), approximate="tanh")
         return x + g[:, None] * self.proj_out(torch.cat([o, mlp], dim=-1))
 
@@ -239,12 +286,15 @@ class FluxShapedTransformer(nn.Module):
         return torch.cat([torch.cos(args), torch.sin(args)], dim=-1)
 
     def forward(self, latents, text, pooled, t):
-        dtype = self.x_embedder.weight.dtype
+        dtype = latents.dtype
         temb = self.time_in(self.timestep_embedding(t).to(dtype)) + self.pooled_in(pooled)
         img = self.x_embedder(latents)
         txt = self.context_embedder(text)
-        rope = rope_full(*rope_tables(txt.shape[1], img.shape[1], self.cfg.hidden // self.cfg.heads, img.device),
-                         img.dtype)
+        if self.cfg.fused_qk:
+            rope = rope_positions(txt.shape[1], img.shape[1], img.device)
+        else:
+            rope = rope_full(*rope_tables(txt.shape[1], img.shape[1], self.cfg.hidden // self.cfg.heads, img.device),
+                             img.dtype)
         for blk in self.transformer_blocks:
             img, txt = blk(img, txt, temb, rope)
         x = torch.cat([txt, img], dim=1)

@@ -11,8 +11,8 @@
 """
 from ._launch import device_errors, raise_device_errors
 from .int8 import QuantizedRows, int8_linear, quantize_rows, quantize_weight
-from .layers import (IndexLoRALinear, PackedLoRALinear, PerSampleLoRALinear, SharedInputPrep, group_shared_inputs,
-                     wrap_linears, wrap_packed)
+from .layers import (IndexLoRALinear, Int8Linear, PackedLoRALinear, PerSampleLoRALinear, SharedInputPrep,
+                     group_shared_inputs, wrap_int8, wrap_linears, wrap_packed)
 from .packed import (PackedBank, PackedLayout, SlotLoader, decode_packed, flat_indices, pack_adapter,
                      pack_indices, split_decoded, unpack_indices)
 from .rotary import qk_norm_rotate, rotate_axes
@@ -20,7 +20,7 @@ from .shared import packed_codebook_lora_delta_, shared_codebook_lora_delta, sha
 
 __all__ = [
     "IndexLoRALinear", "PackedLoRALinear", "PerSampleLoRALinear", "SharedInputPrep", "group_shared_inputs",
-    "wrap_linears", "wrap_packed",
+    "wrap_linears", "wrap_packed", "Int8Linear", "wrap_int8",
     "PackedBank", "PackedLayout", "SlotLoader", "decode_packed", "flat_indices", "pack_adapter", "pack_indices",
     "split_decoded", "unpack_indices",
     "shared_codebook_lora_delta", "shared_codebook_lora_delta_", "packed_codebook_lora_delta_",

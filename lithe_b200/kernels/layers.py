@@ -6,6 +6,8 @@
                      delta tensor, no second pass over the output).
 ``PackedLoRALinear`` the same over a shared ``PackedBank`` (9-bit packed residency): many
                      modules and thousands of slots in one device tensor.
+``Int8Linear``         a linear on 8-bit integers in an nn.Linear's place; as the base of a
+                     ``PackedLoRALinear`` the adapters' expand joins its epilogue.
 ``PerSampleLoRALinear`` decoded (dense bf16) factors per slot, the dense resident-LoRA
                      comparator (lithe/kernels/layers.py:28-95): per-sample delta with two
                      batched cuBLAS products (``kernel="sgmv"``) or a per-sample loop.
@@ -23,6 +25,7 @@ from torch import nn
 from .. import _modtree
 from .. import codebook as cb
 from . import _launch, ops
+from .int8 import int8_linear, quantize_weight
 from .packed import PackedBank
 from .shared import _check
 
@@ -45,6 +48,59 @@ def _as3d(x: torch.Tensor, out: torch.Tensor):
     if x.dim() == 3:
         return x, out
     raise ValueError(f"unsupported input rank {x.dim()}")
+
+
+class Int8Linear(nn.Module):
+    """y = W x + b on 8-bit integers (``int8_linear``): weights quantised once per output channel,
+    activations per token in every call.  Half the weight bytes of a 16-bit linear.
+
+    ``weight_q`` (out_features, in_features rounded up to 16) int8 and ``weight_scale``
+    (out_features,), which stays float32 when the model's dtype changes; ``bias`` has the
+    activations' dtype (bfloat16 or float16).
+    """
+
+    def __init__(self, in_features: int, out_features: int, weight_q: torch.Tensor, weight_scale: torch.Tensor,
+                 bias: Optional[torch.Tensor] = None):
+        super().__init__()
+        if tuple(weight_q.shape) != (out_features, _launch.padded(in_features)) or weight_q.dtype != torch.int8:
+            raise ValueError(f"weight_q must be int8 ({out_features}, {_launch.padded(in_features)}), got "
+                             f"{weight_q.dtype} {tuple(weight_q.shape)}")
+        if tuple(weight_scale.shape) != (out_features,):
+            raise ValueError(f"weight_scale must be ({out_features},), got {tuple(weight_scale.shape)}")
+        if bias is not None and tuple(bias.shape) != (out_features,):
+            raise ValueError(f"bias must be ({out_features},), got {tuple(bias.shape)}")
+        self.in_features, self.out_features = int(in_features), int(out_features)
+        self.register_buffer("weight_q", weight_q.contiguous())
+        self.register_buffer("weight_scale", weight_scale.float().contiguous())
+        self.register_buffer("bias", None if bias is None else bias.detach().contiguous())
+
+    @classmethod
+    def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
+        """The 8-bit form of a bfloat16 or float16 linear on a CUDA device."""
+        n, k = linear.weight.shape
+        q, scale = quantize_weight(linear.weight)
+        full = torch.zeros(n, _launch.padded(k), dtype=torch.int8, device=q.device)
+        full[:, :k] = q
+        return cls(k, n, full, scale, linear.bias)
+
+    def _apply(self, fn, recurse: bool = True):
+        scale = self.weight_scale
+        super()._apply(fn, recurse)
+        if self.weight_scale.dtype != torch.float32:
+            self.weight_scale = scale.to(self.weight_scale.device)
+        return self
+
+    @property
+    def weight(self) -> torch.Tensor:
+        """The int8 weight (out_features, in_features)."""
+        return self.weight_q if self.weight_q.shape[1] == self.in_features else self.weight_q[:, :self.in_features]
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+    def forward(self, x: torch.Tensor, h: Optional[torch.Tensor] = None,
+                b_dec: Optional[torch.Tensor] = None) -> torch.Tensor:
+        return int8_linear(x, self.weight, self.weight_scale, self.bias, h=h, b_dec=b_dec)
 
 
 class IndexLoRALinear(nn.Module):
@@ -175,7 +231,7 @@ class SharedInputPrep:
             if self._key.alive():
                 return None         # results for another, live input are pending: prepare alone
         members = [m for m in self.members
-                   if m.fused_gemm and m._gemm_ok(x3) and _slot_ids(m.assign, x3) is ids
+                   if m._takes_expand(x3) and _slot_ids(m.assign, x3) is ids
                    and ((w is None and m.weights is None) or (w is not None and m._weights(x3) is w))]
         if layer not in members or len(members) < 2:
             return None
@@ -236,13 +292,20 @@ def group_shared_inputs(modules: Dict[str, nn.Module]) -> List[SharedInputPrep]:
 class PackedLoRALinear(nn.Module):
     """y = W x + per-sample delta from module ``name`` of a shared packed bank.
 
+    ``base`` is the linear, an nn.Linear or an ``Int8Linear``; ``int8_base`` turns the former into the
+    latter.  On an 8-bit base the routed adapters' expand is added inside its kernel wherever
+    ``lora_prep`` takes the shapes (rank 16, bfloat16, in_features a multiple of 64, more than 8
+    tokens per sample), any number of tokens.
+
     ``rows`` = (r0, r1) serves one split target of a fused module (B rows [r0, r1), e.g. the
     k projection of a Kohya ``attn_qkv``) straight from the resident slot.
     """
 
     def __init__(self, base: nn.Linear, bank: PackedBank, name: str, rank: int, scaling: float,
-                 rows: Optional[Tuple[int, int]] = None, fused_gemm: bool = False):
+                 rows: Optional[Tuple[int, int]] = None, fused_gemm: bool = False, int8_base: bool = False):
         super().__init__()
+        if int8_base and not isinstance(base, Int8Linear):
+            base = Int8Linear.from_linear(base)
         self.base = base
         for p in self.base.parameters():
             p.requires_grad_(False)
@@ -278,6 +341,18 @@ class PackedLoRALinear(nn.Module):
         # (routing key, b_dec): the decoded B factor of the last routing on the fused-GEMM path
         self._bdec_cache: Optional[Tuple[_RouteKey, torch.Tensor]] = None
 
+    def _int8_expand_ok(self, x3: torch.Tensor) -> bool:
+        """Whether the expand joins the 8-bit base's epilogue: the shapes lora_prep takes, and enough
+        tokens per sample that its two launches cost less than the small-m form's one."""
+        return (self.rank == 16 and x3.dtype == torch.bfloat16 and self.base.in_features % 64 == 0
+                and self.base.out_features % 8 == 0 and x3.shape[1] > 8 and x3.shape[0] > 0)
+
+    def _takes_expand(self, x3: torch.Tensor) -> bool:
+        """Whether a call on x3 computes h and b_dec and adds the expand inside its base product."""
+        if isinstance(self.base, Int8Linear):
+            return self._int8_expand_ok(x3)
+        return self.fused_gemm and self._gemm_ok(x3)
+
     def _gemm_ok(self, x3: torch.Tensor) -> bool:
         w = self.base.weight
         b = self.base.bias
@@ -288,7 +363,7 @@ class PackedLoRALinear(nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x3 = x.unsqueeze(1) if x.dim() == 2 else x
-        if self.fused_gemm and x3.dim() == 3 and self._gemm_ok(x3):
+        if x3.dim() == 3 and self._takes_expand(x3):
             if torch.is_grad_enabled() and (x.requires_grad or self.base.weight.requires_grad):
                 raise RuntimeError("lithe_b200 layers are inference-only (run under torch.no_grad())")
             return self._forward_fused_gemm(x, x3.contiguous())
@@ -325,6 +400,15 @@ class PackedLoRALinear(nn.Module):
 
     def _forward_fused_gemm(self, x: torch.Tensor, x3: torch.Tensor) -> torch.Tensor:
         bsz, m, d_in = x3.shape
+        d_out = self.base.out_features
+        h, b_dec = self._expand_operands(x3)
+        if isinstance(self.base, Int8Linear):
+            return self.base(x3, h, b_dec).view(*x.shape[:-1], d_out)
+        out = torch.ops.lithe_b200.lora_gemm(x3.view(bsz * m, d_in), self.base.weight, self.base.bias, h, b_dec, m)
+        return out.view(*x.shape[:-1], d_out)
+
+    def _expand_operands(self, x3: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """(h, b_dec) of this layer for x3 and the present routing."""
         d_out = self.base.out_features
         ids = _slot_ids(self.assign, x3)
         w = self._weights(x3)
@@ -363,8 +447,7 @@ class PackedLoRALinear(nn.Module):
                 h = h_new
                 if share:
                     self._store_h(x3, ids, w, h)
-        out = torch.ops.lithe_b200.lora_gemm(x3.view(bsz * m, d_in), self.base.weight, self.base.bias, h, b_dec, m)
-        return out.view(*x.shape[:-1], d_out)
+        return h, b_dec
 
 
 class PerSampleLoRALinear(nn.Module):
@@ -440,13 +523,14 @@ def wrap_linears(model: nn.Module, paths: Iterable[str],
 
 def wrap_packed(model: nn.Module, bank: PackedBank, key_format: str = "diffusers",
                 paths: Optional[Iterable[str]] = None, scaling: Optional[float] = None,
-                fused_gemm: bool = False) -> Dict[str, PackedLoRALinear]:
+                fused_gemm: bool = False, int8_base: bool = False) -> Dict[str, PackedLoRALinear]:
     """Serve every linear the bank's layout covers from the resident packed bank.
 
     For a Kohya-format layout (304 fused modules) each diffusers linear (494) reads its own B
     rows of the fused module in place (``lithe_b200.kohya.split_targets``).  ``paths`` limits
     the wrapped set (e.g. the 342 attention / feed-forward linears); ``scaling`` defaults to
-    the layout's alpha / rank; ``fused_gemm`` selects the expand-in-GEMM path where eligible.
+    the layout's alpha / rank; ``fused_gemm`` selects the expand-in-GEMM path where eligible;
+    ``int8_base`` quantises the wrapped linears to 8 bits (``Int8Linear``), the expand inside.
     Set ``.assign`` on the returned modules to route samples.
     """
     from .. import kohya
@@ -462,12 +546,19 @@ def wrap_packed(model: nn.Module, bank: PackedBank, key_format: str = "diffusers
         name, r0, r1 = targets[path]
         rank = lay.shapes_a[lay.index(name)][0]
         full = r0 == 0 and r1 == lay.shapes_b[lay.index(name)][0]
-        return PackedLoRALinear(lin, bank, name, rank, s, rows=None if full else (r0, r1), fused_gemm=fused_gemm)
+        return PackedLoRALinear(lin, bank, name, rank, s, rows=None if full else (r0, r1), fused_gemm=fused_gemm,
+                                int8_base=int8_base)
 
     wrapped = wrap_linears(model, want, factory)
-    if fused_gemm:
+    if fused_gemm or int8_base:
         group_shared_inputs(wrapped)
     return wrapped
+
+
+def wrap_int8(model: nn.Module, paths: Iterable[str]) -> Dict[str, Int8Linear]:
+    """Put an ``Int8Linear`` in place of the ``nn.Linear`` at every dotted ``path`` of ``model`` (the
+    linears no adapter targets); returns {path: layer}."""
+    return _modtree.replace_linears(model, paths, lambda path, lin: Int8Linear.from_linear(lin))
 
 
 def pools_on(device, dtype=torch.float32):
