@@ -1060,8 +1060,25 @@ class _DenoiseSetup:
                     self.reference_check[f"{shape[0]}x{shape[1]}"] = float((d_ours.float() - d_ref).abs().max()
                                                                           / d_ref.abs().max())
 
+    def _on_int8(self):
+        """Every target linear on an 8-bit base with its adapters' expand inside the product."""
+        from lithe_b200.kernels import PackedLoRALinear, group_shared_inputs
+        table = {}
+        for n, m in self.packed.items():
+            table[n] = PackedLoRALinear(m.base, m.bank, m.name, m.rank, m.scaling, rows=m.rows, int8_base=True)
+            table[n].assign = m.assign
+        group_shared_inputs(table)
+        return table
+
     def install(self, kind):
         from lithe_b200.kernels.layers import FUSED_GEMM_MAX_K
+        fused_qk = kind.endswith("_qk")
+        kind = kind[:-3] if fused_qk else kind
+        self.model.cfg.fused_qk = fused_qk
+        for blk in (*self.model.transformer_blocks, *self.model.single_transformer_blocks):
+            blk.fused_qk = fused_qk
+        if kind == "lithe_int8" and kind not in self.tables:
+            self.tables[kind] = self._on_int8()
         for m in self.packed.values():
             m.fused_gemm = kind.startswith("lithe_fused")
             # lithe_fused: the default policy (in_features <= FUSED_GEMM_MAX_K); _all: every eligible linear
@@ -1145,6 +1162,8 @@ DENOISE = {  # workload -> (image tokens, text tokens, batch, steps, adapter key
 
 
 DENOISE_VARIANTS = ("base", "plain_gemm", "lithe", "lithe_fused", "lithe_fused_all", "dense")
+# on request: q and k normalised and rotated in one pass (_qk), the target linears on 8-bit bases
+DENOISE_MORE = ("base_qk", "lithe_fused_qk", "lithe_int8", "lithe_int8_qk")
 
 
 def run_denoise(args):
@@ -1153,7 +1172,8 @@ def run_denoise(args):
     every eligible linear, dense resident LoRA), ABBA order.  Targets: the 342 diffusers
     linears, or the 494 linears a Kohya-304 adapter covers (its fused q/k/v modules served in
     place).  ``--variants`` times a subset; its ``reference_triton`` variant adds the
-    reference's own GPU path (its IndexLoRALinear from baseline/_ref) on the 342 layout."""
+    reference's own GPU path (its IndexLoRALinear from baseline/_ref) on the 342 layout, and those of
+    DENOISE_MORE the 8-bit bases and the fused norm and rotation."""
     from lithe_b200.shard import shard_bounds
     img_tok, txt_tok, batch, steps, key_format = DENOISE[args.workload]
     world, rank, local = dist_env()
@@ -1164,7 +1184,7 @@ def run_denoise(args):
                               "flux_sweep_b14 workload"}), flush=True)
         return
     kinds = tuple(args.variants.split(",")) if args.variants else DENOISE_VARIANTS
-    unknown = [k for k in kinds if k not in DENOISE_VARIANTS + ("reference_triton",)]
+    unknown = [k for k in kinds if k not in DENOISE_VARIANTS + DENOISE_MORE + ("reference_triton",)]
     if unknown or "base" not in kinds:
         raise SystemExit(f"--variants: unknown {unknown}" if unknown else "--variants must include base")
     reference = None
@@ -1735,7 +1755,8 @@ def main():
                          "every rank its own B=14 batch (the default line also reports weak scaling as a secondary key)")
     ap.add_argument("--variants", default="", help="denoise_*: comma list of variants to time (default: "
                     + ",".join(DENOISE_VARIANTS) + "); reference_triton adds the reference's own GPU path "
-                    "(its IndexLoRALinear from baseline/_ref)")
+                    "(its IndexLoRALinear from baseline/_ref); "
+                    + ", ".join(DENOISE_MORE) + ": 8-bit bases, fused norm and rotation of q and k")
     ap.add_argument("--no-denoise", action="store_true",
                     help="leave out the 28-step 1024^2 denoise record of the default line")
     ap.add_argument("--shapes", default="", help="comma list of d_inxd_out to run (default: all four), "
