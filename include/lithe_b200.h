@@ -353,20 +353,22 @@ typedef struct lithe_heads_view {
  * Rotary positions with several axes (time, row, column): out = x with every head's pairs turned.
  * It has no counterpart in the reference, whose pipelines take the rotation from diffusers.
  *   pair p of the axis-a slice (axis_dims[a] / 2 pairs, slices in order) turns by
- *   positions[token][a] * theta^(-2 i / axis_dims[a]), i = p's index inside the slice:
+ *   positions[token][a] * frequencies[p]:
  *   (u, v) -> (u cos - v sin, v cos + u sin), in fp32 with the revolution count in fp64, rounded
  *   once.  The values from R = sum(axis_dims) on are copied.
  *   dtype      LITHE_DTYPE_BF16, _F16 or _F32 of x and out; out may be x itself (the same view),
  *              any other overlap of the two is undefined
  *   positions  device (tokens, n_axes), or (batch, tokens, n_axes) when per_sample != 0, contiguous,
  *              of pos_type; integers beyond 2^53 are rounded
- *   axis_dims  HOST (n_axes) even, >= 0, sum at most dim; n_axes 1..LITHE_MAX_AXES
+ *   axis_dims  HOST (n_axes) even, >= 0, sum R at most dim; n_axes 1..LITHE_MAX_AXES
+ *   frequencies  HOST (R / 2), radians per unit of position, finite; theta^(-2 i / axis_dims[a]) for the
+ *              i-th pair of a slice is the usual choice
  * dim even, at most LITHE_MAX_HEAD_DIM (LITHE_ERR_UNSUPPORTED above).  batch or tokens 0: no-op.
  */
 LITHE_API int32_t lithe_rotate_axes(const lithe_heads_view* x, const lithe_heads_view* out, int32_t dtype,
                         int32_t batch, int32_t tokens, int32_t dim, const void* positions, int32_t pos_type,
-                        int32_t per_sample, const int32_t* axis_dims, int32_t n_axes, double theta,
-                        int32_t pairing, void* stream);
+                        int32_t per_sample, const int32_t* axis_dims, int32_t n_axes,
+                        const double* frequencies, int32_t pairing, void* stream);
 
 /*
  * RMS norm of every head of q and k, then the rotation of lithe_rotate_axes, in one pass:
@@ -380,7 +382,8 @@ LITHE_API int32_t lithe_qk_norm_rotate(const lithe_heads_view* q, const lithe_he
                         const lithe_heads_view* out_q, const lithe_heads_view* out_k, const void* weight_q,
                         const void* weight_k, int32_t weight_dtype, float eps, int32_t dtype, int32_t batch,
                         int32_t tokens, int32_t dim, const void* positions, int32_t pos_type, int32_t per_sample,
-                        const int32_t* axis_dims, int32_t n_axes, double theta, int32_t pairing, void* stream);
+                        const int32_t* axis_dims, int32_t n_axes, const double* frequencies, int32_t pairing,
+                        void* stream);
 
 /*
  * Rows to 8-bit integers, one scale a row (activations per token, weights per output channel):

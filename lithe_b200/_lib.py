@@ -89,11 +89,11 @@ _SIGNATURES.update({
         _c.c_void_p, _c.c_int64, _c.c_void_p]),
     "lithe_rotate_axes": (_c.c_int32, [
         _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p,
-        _c.c_int32, _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),
+        _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_int32, _c.c_void_p, _c.c_int32, _c.c_void_p]),
     "lithe_qk_norm_rotate": (_c.c_int32, [
         _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p,
         _c.c_void_p, _c.c_int32, _c.c_float, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_int32,
-        _c.c_int32, _c.POINTER(_c.c_int32), _c.c_int32, _c.c_double, _c.c_int32, _c.c_void_p]),
+        _c.c_int32, _c.c_void_p, _c.c_int32, _c.c_void_p, _c.c_int32, _c.c_void_p]),
     "lithe_sgmv_index": (_c.c_int32, [
         _c.c_void_p, _c.c_void_p, _c.c_int32, _c.POINTER(IndexView), _c.POINTER(IndexView), _c.c_int64,
         _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32,

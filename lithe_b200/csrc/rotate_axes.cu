@@ -1,8 +1,8 @@
 // Rotary positions with several axes, and the per-head RMS norm of q and k with that rotation
 // in the same pass.
 //
-//   angle(token, pair p) = position(token, axis of p) * theta^(-2 i / d_axis),  i = p's index
-//   inside its axis's slice of d_axis / 2 pairs; the axes' slices follow one another.
+//   angle(token, pair p) = position(token, axis of p) * frequency(p); every axis has a slice of
+//   d_axis / 2 pairs, the slices follow one another.
 //   (a, b) -> (a cos - b sin, b cos + a sin) for pair p's two values: neighbours 2p, 2p + 1
 //   ("interleaved") or p, p + R/2 ("halves"), R = sum of d_axis; values from R on stay.
 //   With the norm: a, b are first x * rsqrt(mean(x^2) + eps) * weight over the head's dim.
@@ -447,7 +447,7 @@ int32_t check_heads(const lithe_heads_view& v, const char* name, int32_t batch, 
 int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void* const* weight, int tensors,
             bool norm, float eps, int32_t weight_dtype, int32_t dtype, int32_t batch, int32_t tokens, int32_t dim,
             const void* positions, int32_t pos_type, int32_t per_sample, const int32_t* axis_dims, int32_t n_axes,
-            double theta, int32_t pairing, void* stream) {
+            const double* frequencies, int32_t pairing, void* stream) {
     clear_error();
     if (dtype != LITHE_DTYPE_BF16 && dtype != LITHE_DTYPE_F16 && dtype != LITHE_DTYPE_F32)
         return fail_arg("dtype must be LITHE_DTYPE_BF16, _F16 or _F32, got %d", dtype);
@@ -455,8 +455,7 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
     if (dim <= 0 || dim % 2) return fail_arg("the head dim must be positive and even, got %d", dim);
     if (dim > LITHE_MAX_HEAD_DIM) return fail_unsupported("head dim %d above %d", dim, LITHE_MAX_HEAD_DIM);
     if (n_axes < 1 || n_axes > LITHE_MAX_AXES) return fail_arg("1 to %d axes, got %d", LITHE_MAX_AXES, n_axes);
-    if (!axis_dims) return fail_arg("axis_dims must be non-NULL");
-    if (!(theta > 0.0) || !std::isfinite(theta)) return fail_arg("theta must be positive and finite");
+    if (!axis_dims || !frequencies) return fail_arg("axis_dims and frequencies must be non-NULL");
     if (pairing != LITHE_PAIR_INTERLEAVED && pairing != LITHE_PAIR_HALVES)
         return fail_arg("pairing must be LITHE_PAIR_INTERLEAVED or LITHE_PAIR_HALVES, got %d", pairing);
     if (pos_type != LITHE_POS_I32 && pos_type != LITHE_POS_I64 && pos_type != LITHE_POS_F32)
@@ -474,7 +473,9 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
                             dim, a, d);
         for (int i = 0; i < d / 2; ++i) {
             p.axis[rotated / 2 + i] = static_cast<uint8_t>(a);
-            p.turn[rotated / 2 + i] = std::pow(theta, -2.0 * i / d) / two_pi;
+            const double f = frequencies[rotated / 2 + i];
+            if (!std::isfinite(f)) return fail_arg("frequency %d is not finite", rotated / 2 + i);
+            p.turn[rotated / 2 + i] = f / two_pi;
         }
         rotated += d;
     }
@@ -553,10 +554,10 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
 extern "C" int32_t lithe_rotate_axes(const lithe_heads_view* x, const lithe_heads_view* out, int32_t dtype,
                                      int32_t batch, int32_t tokens, int32_t dim, const void* positions,
                                      int32_t pos_type, int32_t per_sample, const int32_t* axis_dims, int32_t n_axes,
-                                     double theta, int32_t pairing, void* stream) {
+                                     const double* frequencies, int32_t pairing, void* stream) {
     if (!x || !out) return lithe::fail_arg("x and out must be non-NULL");
     return lithe::ra::run(x, out, nullptr, 1, false, 0.0f, LITHE_DTYPE_F32, dtype, batch, tokens, dim, positions,
-                          pos_type, per_sample, axis_dims, n_axes, theta, pairing, stream);
+                          pos_type, per_sample, axis_dims, n_axes, frequencies, pairing, stream);
 }
 
 extern "C" int32_t lithe_qk_norm_rotate(const lithe_heads_view* q, const lithe_heads_view* k,
@@ -564,11 +565,11 @@ extern "C" int32_t lithe_qk_norm_rotate(const lithe_heads_view* q, const lithe_h
                                         const void* weight_q, const void* weight_k, int32_t weight_dtype, float eps,
                                         int32_t dtype, int32_t batch, int32_t tokens, int32_t dim,
                                         const void* positions, int32_t pos_type, int32_t per_sample,
-                                        const int32_t* axis_dims, int32_t n_axes, double theta, int32_t pairing,
-                                        void* stream) {
+                                        const int32_t* axis_dims, int32_t n_axes, const double* frequencies,
+                                        int32_t pairing, void* stream) {
     if (!q || !k || !out_q || !out_k) return lithe::fail_arg("q, k, out_q and out_k must be non-NULL");
     const lithe_heads_view in[2] = {*q, *k}, out[2] = {*out_q, *out_k};
     const void* weight[2] = {weight_q, weight_k};
     return lithe::ra::run(in, out, weight, 2, true, eps, weight_dtype, dtype, batch, tokens, dim, positions, pos_type,
-                          per_sample, axis_dims, n_axes, theta, pairing, stream);
+                          per_sample, axis_dims, n_axes, frequencies, pairing, stream);
 }

@@ -467,8 +467,10 @@ PAIRINGS = {"interleaved": _lib.PAIR_INTERLEAVED, "halves": _lib.PAIR_HALVES}
 
 
 @functools.lru_cache(maxsize=256)
-def _axis_array(axes: tuple) -> ctypes.Array:
-    return (ctypes.c_int32 * max(1, len(axes)))(*axes)
+def _axis_arrays(axes: tuple, theta: float) -> tuple:
+    """The axes' dims and the pairs' frequencies theta^(-2 i / dim), as the C entries take them."""
+    freqs = [theta ** (-2.0 * i / d) for d in axes for i in range(d // 2)]
+    return (ctypes.c_int32 * max(1, len(axes)))(*axes), (ctypes.c_double * max(1, len(freqs)))(*freqs)
 
 
 def _heads_strides(t: torch.Tensor) -> tuple:
@@ -589,7 +591,8 @@ def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta:
         raise ValueError(f"positions must be ({s}, {n}) or ({b}, {s}, {n}), got {tuple(shape)}")
     if not positions.is_contiguous():
         raise ValueError("positions must be contiguous")
-    return (positions.data_ptr(), code, len(shape) - 2, _axis_array(axes), n, theta, pairing, stream_handle(x.device))
+    dims, freqs = _axis_arrays(axes, theta)
+    return positions.data_ptr(), code, len(shape) - 2, dims, n, freqs, pairing, stream_handle(x.device)
 
 
 def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], theta: float,

@@ -16,11 +16,12 @@ def _view(**over):
 
 
 def _rotate(x=None, out=None, dtype=_lib.DTYPE_BF16, batch=1, tokens=4, dim=64, positions=0x30000, pos_type=_lib.POS_F32,
-            axes=(16, 24, 24), n_axes=None, theta=1e4, pairing=0):
+            axes=(16, 24, 24), n_axes=None, freqs=(1.0,) * 128, pairing=0):
     x, out = x or _view(), out or _view(base=0x20000)
     arr = (ctypes.c_int32 * max(1, len(axes)))(*axes)
     return _lib.lib().lithe_rotate_axes(ctypes.byref(x), ctypes.byref(out), dtype, batch, tokens, dim, positions,
-                                        pos_type, 0, arr, len(axes) if n_axes is None else n_axes, theta, pairing, None)
+                                        pos_type, 0, arr, len(axes) if n_axes is None else n_axes,
+                                        None if freqs is None else (ctypes.c_double * len(freqs))(*freqs), pairing, None)
 
 
 @pytest.mark.parametrize("over,code", [
@@ -35,8 +36,9 @@ def _rotate(x=None, out=None, dtype=_lib.DTYPE_BF16, batch=1, tokens=4, dim=64, 
     ({"axes": (2147483646, 4)}, _lib.ERR_ARG),
     ({"n_axes": 0}, _lib.ERR_ARG),
     ({"axes": (2,) * 9}, _lib.ERR_ARG),
-    ({"theta": 0.0}, _lib.ERR_ARG),
-    ({"theta": float("nan")}, _lib.ERR_ARG),
+    ({"freqs": None}, _lib.ERR_ARG),
+    ({"freqs": (1.0,) * 31 + (float("nan"),)}, _lib.ERR_ARG),
+    ({"freqs": (float("inf"),) + (1.0,) * 127}, _lib.ERR_ARG),
     ({"pairing": 2}, _lib.ERR_ARG),
     ({"pos_type": 3}, _lib.ERR_ARG),
     ({"positions": None}, _lib.ERR_ARG),
@@ -62,7 +64,7 @@ def test_c_norm_entry_refuses():
     def call(eps=1e-6, wtype=_lib.DTYPE_BF16, k=v):
         return _lib.lib().lithe_qk_norm_rotate(ctypes.byref(v), None if k is None else ctypes.byref(k), ctypes.byref(v),
                                                ctypes.byref(v), None, None, wtype, eps, _lib.DTYPE_BF16, 1, 0, 64,
-                                               0x30000, 0, 0, arr, 1, 1e4, 0, None)
+                                               0x30000, 0, 0, arr, 1, (ctypes.c_double * 8)(), 0, None)
     assert call() == _lib.OK
     assert call(eps=-1.0) == _lib.ERR_ARG
     assert call(wtype=_lib.DTYPE_F16) == _lib.ERR_ARG
