@@ -48,7 +48,7 @@ def build(verbose: bool = False, force: bool = False) -> Path:
         return LIB_PATH
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = [nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-shared",
+    cmd = [nvcc_path(), *ARCH_FLAGS, "--threads", "0", "-O3", "-lineinfo", "-std=c++17", "-shared",
            "-Xcompiler", "-fPIC,-fvisibility=hidden", "-cudart", "static",
            f"-I{INCLUDE}", f"-I{CSRC}", "--expt-relaxed-constexpr",
            "-DLITHE_BUILDING_LIBRARY"]

@@ -18,8 +18,9 @@
 // pair costs four products two at a time (f32x2), the norm's factor two more.  The sum of squares is
 // a shuffle inside the lanes of a head.  kBatch heads are loaded before the first is used, the
 // token's first ones before its angles.
-// Measured on B200: 14 x 4096 tokens of 24 + 24 heads of 128, norm and rotation, 249 us (5.7 TB/s, 0.88 of
-// the measured copy rate); 32760 tokens of 24 heads, rotation, 64 us (6.3 TB/s, 0.97); one token 3.4 us.
+// Measured on B200: 14 x 4096 tokens of 24 + 24 heads of 128, norm and rotation, 242 us (5.8 TB/s, 0.90 of
+// the measured copy rate; 250 us back to back, at the 1 kW cap); 32760 tokens of 24 heads, rotation, 64 us
+// (6.3 TB/s, 0.98); one token 3.2 us.
 // A second batch of heads on its way while one is turned took registers that cost more (306 us).
 #include <cmath>
 #include <type_traits>
@@ -55,7 +56,7 @@ struct Params {
     int32_t tensors;
     int32_t tokens, dim, rotated;  // rotated = R
     int32_t chunks;                // units a token is split into
-    int32_t group_log2;            // lanes that share a head
+    int32_t group;                 // lanes that share a head
     int64_t units;                 // batch * tokens * chunks
     float eps, inv_dim;
     uint8_t axis[kMaxPairs];
@@ -221,19 +222,18 @@ struct Turn {
     F2 aa[2], ab[2], bb[2], ba[2];             // (ab negated)
 };
 
-// One tensor's heads [h0, h1) of one token.  Every lane of the warp runs every iteration (the
-// norm's shuffles need them); lanes without a head or without pairs load and store nothing.
-// kWhole: every value of a head is turned; else values that stay never meet an angle (a product with a
-// zero sine would carry a NaN or an infinity across).
+// A lane's part of the heads that a warp has loaded: kBatch heads, 32 / kGroup apart, from the lane's own on.
+// live: how many heads there are from it on (none for a lane without pairs); the others load zeros and store
+// nothing, but take part in the norm's shuffles.
 template <typename T>
 struct Batch {
     Eight<T> e[kBatch];
 };
 
-template <typename T, bool kHalves, bool kVec>
+template <typename T, bool kHalves, bool kVec, int kGroup>
 __device__ __forceinline__ void load_batch(const Params& p, const T* in, int64_t step, int pair0, int first, int second,
                                            int live, Batch<T>& b) {
-    const int per_iter = 32 >> p.group_log2;
+    const int per_iter = 32 / kGroup;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
         if (j * per_iter < live)
@@ -244,11 +244,11 @@ __device__ __forceinline__ void load_batch(const Params& p, const T* in, int64_t
     }
 }
 
-// live: heads from the lane's first on (0 for a lane without pairs)
-template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole>
+// kWhole: every value of a head is turned; else the values that stay never meet an angle.
+template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole, int kGroup>
 __device__ __forceinline__ void turn_batch(const Params& p, T* out, int64_t step, int pair0, int first, int second,
                                            int live, const Turn& m, Batch<T>& b) {
-    const int per_iter = 32 >> p.group_log2;
+    const int per_iter = 32 / kGroup;
 #pragma unroll
     for (int j = 0; j < kBatch; ++j) {
         F2 x[2], y[2];
@@ -262,8 +262,11 @@ __device__ __forceinline__ void turn_batch(const Params& p, T* out, int64_t step
             float s0, s1;
             sum2.split(s0, s1);
             float sum = s0 + s1;
-            for (int o = (1 << p.group_log2) >> 1; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-            r = rsqrtf(fmaf(sum, p.inv_dim, p.eps));
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1)
+                if (o < kGroup) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            const float mean = fmaf(sum, p.inv_dim, p.eps);
+            r = rsqrtf(mean);
         }
         const F2 rr(r, r);
         F2 u[2], v[2];
@@ -334,13 +337,13 @@ __device__ __forceinline__ void fill_tables(const Params& p, Tables& tab) {
     __syncthreads();
 }
 
-template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole>
+template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole, int kGroup>
 __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const __grid_constant__ Params p) {
     const int lane = threadIdx.x & 31;
-    const int pair0 = 4 * (lane & ((1 << p.group_log2) - 1)), sub = lane >> p.group_log2;
+    const int pair0 = 4 * (lane & (kGroup - 1)), sub = lane / kGroup;
     const bool has_pairs = pair0 < (p.dim >> 1);
     const int first = has_pairs ? first_of<kHalves>(p, pair0) : 0, second = has_pairs ? second_of<kHalves>(p, pair0) : 0;
-    const int per_iter = 32 >> p.group_log2;
+    const int per_iter = 32 / kGroup;
     __shared__ Tables tab;
     fill_tables<T, kHalves, kNorm>(p, tab);
     float2* angle = tab.angle[threadIdx.x >> 5];
@@ -354,13 +357,13 @@ __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const _
         {
             const Heads& t = p.t[0];
             const int live = has_pairs ? min(h + t.per_unit, t.heads) - h - sub : 0;
-            load_batch<T, kHalves, kVec>(
+            load_batch<T, kHalves, kVec, kGroup>(
                 p, static_cast<const T*>(t.in) + sample * t.in_sample + token * t.in_token + (h + sub) * t.in_head,
                 per_iter * t.in_head, pair0, first, second, live, b);
         }
         // revolutions in fp64, their fraction (at most half a turn) in fp32; each pair's by one lane
         __syncwarp();
-        for (int pair = lane; pair < (4 << p.group_log2); pair += 32) {
+        for (int pair = lane; pair < (4 * kGroup); pair += 32) {
             float2 a = make_float2(1.0f, 0.0f);
             if (pair < (p.rotated >> 1)) {
                 const double r =
@@ -394,8 +397,8 @@ __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const _
             for (; h < end; h += per_iter * kBatch) {
                 const int live = has_pairs ? end - h - sub : 0;
                 if (k > 0 || h > chunk * t.per_unit)
-                    load_batch<T, kHalves, kVec>(p, in, per_iter * t.in_head, pair0, first, second, live, b);
-                turn_batch<T, kHalves, kVec, kNorm, kWhole>(p, out, per_iter * t.out_head, pair0, first, second, live, m, b);
+                    load_batch<T, kHalves, kVec, kGroup>(p, in, per_iter * t.in_head, pair0, first, second, live, b);
+                turn_batch<T, kHalves, kVec, kNorm, kWhole, kGroup>(p, out, per_iter * t.out_head, pair0, first, second, live, m, b);
                 in += kBatch * per_iter * t.in_head;
                 out += kBatch * per_iter * t.out_head;
             }
@@ -403,29 +406,37 @@ __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const _
     }
 }
 
-template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole>
+template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole, int kGroup>
 int32_t launch(const Params& p, int sms, cudaStream_t st) {
     const int64_t blocks = (p.units + kWarps - 1) / kWarps;
     // (the rotation alone: four CTAs to a place, 126 us against 144 us for 14 x 4608 tokens; with the norm, whose
     // tables a CTA lays out at its start, one: 246 us against 249 us for 14 x 4096)
     const int64_t most = static_cast<int64_t>(sms) * kMinBlocks * (kNorm ? 1 : 4);
-    rotate_kernel<T, kHalves, kVec, kNorm, kWhole>
+    rotate_kernel<T, kHalves, kVec, kNorm, kWhole, kGroup>
         <<<static_cast<int>(blocks < most ? blocks : most), 32 * kWarps, 0, st>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "rotate_kernel launch");
 }
 
-template <typename T, bool kNorm, bool kHalves, bool kVec>
-int32_t launch_whole(const Params& p, int sms, cudaStream_t st) {
-    return p.rotated == p.dim ? launch<T, kHalves, kVec, kNorm, true>(p, sms, st)
-                              : launch<T, kHalves, kVec, kNorm, false>(p, sms, st);
+// The lanes of a head are a compile-time number: 8, 16 or 32 (with the norm 252 us for 14 x 4096 tokens against
+// 276 us with a run-time one, both at the power cap).
+template <typename T, bool kHalves, bool kNorm, bool kWhole>
+int32_t launch_group(const Params& p, int sms, cudaStream_t st) {
+    if (p.group == 8) return launch<T, kHalves, true, kNorm, kWhole, 8>(p, sms, st);
+    if (p.group == 16) return launch<T, kHalves, true, kNorm, kWhole, 16>(p, sms, st);
+    return launch<T, kHalves, true, kNorm, kWhole, 32>(p, sms, st);
+}
+
+template <typename T, bool kNorm, bool kHalves>
+int32_t launch_vec(const Params& p, bool vec, int sms, cudaStream_t st) {
+    if (!vec) return launch<T, kHalves, false, kNorm, false, 32>(p, sms, st);
+    return p.rotated == p.dim ? launch_group<T, kHalves, kNorm, true>(p, sms, st)
+                              : launch_group<T, kHalves, kNorm, false>(p, sms, st);
 }
 
 template <typename T, bool kNorm>
 int32_t launch_layout(const Params& p, bool halves, bool vec, int sms, cudaStream_t st) {
-    if (halves)
-        return vec ? launch_whole<T, kNorm, true, true>(p, sms, st) : launch<T, true, false, kNorm, false>(p, sms, st);
-    return vec ? launch_whole<T, kNorm, false, true>(p, sms, st) : launch<T, false, false, kNorm, false>(p, sms, st);
+    return halves ? launch_vec<T, kNorm, true>(p, vec, sms, st) : launch_vec<T, kNorm, false>(p, vec, sms, st);
 }
 
 // Whether a tensor's heads can be read and written in whole 16-byte pieces.
@@ -480,10 +491,6 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
         rotated += d;
     }
     const int size = dtype == LITHE_DTYPE_F32 ? 4 : 2;
-    // Lanes that share a head: 4 pairs each, a power of two for the norm's shuffles.
-    int lg = 0;
-    while ((4 << lg) < dim / 2) ++lg;
-    p.group_log2 = lg;
     p.tensors = tensors;
     // Pieces of 16 bytes need every stride, base and (pairs half a head apart) slice aligned to
     // them; the other form loads value by value.
@@ -524,7 +531,9 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
     p.inv_dim = 1.0f / static_cast<float>(dim);
     // A token's heads are split over warps while that leaves the SMs room: more units than resident
     // warps pay their angles for nothing (1024 tokens of 24 heads: 5.9 us on 4 chunks, 13 us on 8).
-    const int per_iter = 32 >> lg;
+    // Lanes that share a head: 4 pairs each, a power of two for the norm's shuffles.
+    p.group = !vec || dim > 128 ? 32 : dim > 64 ? 16 : 8;
+    const int per_iter = 32 / p.group;
     const int most_chunks = (most_heads + per_iter - 1) / per_iter;
     const int64_t rows = static_cast<int64_t>(batch) * tokens;
     int chunks = 1;
