@@ -15,6 +15,7 @@ namespace i8 {
 
 constexpr int kRank = 16;              // rank of the fused expand
 constexpr int kMaxK = 131072;          // 127 * 127 * kMaxK < 2^31
+constexpr int kMostRows = 0x7fffffff - 1024;   // rows and channels of whole tiles stay inside 32 bits
 
 // ------------------------------------------------------------------------------------------
 // lithe_quantize_rows
@@ -1201,6 +1202,7 @@ int32_t check_size(int32_t dtype, int32_t rows, int32_t n, int32_t k) {
         return fail_arg("dtype must be LITHE_DTYPE_BF16 or _F16, got %d", dtype);
     if (rows < 0 || n <= 0 || k <= 0) return fail_arg("rows must be >= 0 and n, k > 0 (rows %d, n %d, k %d)", rows, n, k);
     if (k > kMaxK) return fail_unsupported("k %d above %d: the int32 sums could overflow", k, kMaxK);
+    if (rows > kMostRows || n > kMostRows) return fail_unsupported("rows %d or n %d above %d", rows, n, kMostRows);
     return LITHE_OK;
 }
 

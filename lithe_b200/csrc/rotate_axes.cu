@@ -32,6 +32,7 @@ namespace lithe {
 namespace ra {
 
 constexpr int kMaxPairs = LITHE_MAX_HEAD_DIM / 2;
+constexpr int kMostHeads = 1 << 30;            // the heads' arithmetic stays inside 32 bits
 constexpr int kBatch = 4;          // heads a lane group loads before it uses the first
 constexpr int kMinBlocks = 4;      // CTAs that have to fit an SM (64 registers a thread)
 constexpr int kWarps = 8;          // warps of a CTA
@@ -307,7 +308,7 @@ __device__ __forceinline__ void turn_batch(const Params& p, T* out, int64_t step
 
 // What every unit needs, laid out by pair once per CTA: revolutions per unit of position and axis, the
 // norms' weights of the pair's two values, and a warp's cosines and sines of its token.
-struct Tables {
+struct alignas(16) Tables {
     double turn[kMaxPairs];
     float weight[2][2][kMaxPairs];             // [tensor][first, second][pair]
     float2 angle[kWarps][kMaxPairs];
@@ -448,6 +449,7 @@ bool aligned(const Heads& t, int size) {
 
 int32_t check_heads(const lithe_heads_view& v, const char* name, int32_t batch, int32_t tokens, int64_t* elements) {
     if (v.heads <= 0) return fail_arg("%s: heads must be positive, got %d", name, v.heads);
+    if (v.heads > kMostHeads) return fail_unsupported("%s: %d heads above %d", name, v.heads, kMostHeads);
     if (!v.base) return fail_arg("%s must be non-NULL", name);
     if (v.sample_stride < 0 || v.token_stride < 0 || v.head_stride < 0)
         return fail_arg("%s: strides must not be negative", name);

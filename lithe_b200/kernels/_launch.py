@@ -473,6 +473,14 @@ def _axis_arrays(axes: tuple, theta: float) -> tuple:
     return (ctypes.c_int32 * max(1, len(axes)))(*axes), (ctypes.c_double * max(1, len(freqs)))(*freqs)
 
 
+_MOST = 2 ** 31 - 1025       # a dimension the C entries take (ctypes would cut a larger one to 32 bits)
+
+
+def _check_sizes(t: torch.Tensor, name: str) -> None:
+    if t.numel() > _MOST and max(t.shape) > _MOST:
+        raise NotImplementedError(f"{name}: a dimension of {tuple(t.shape)} is above {_MOST}")
+
+
 def _heads_strides(t: torch.Tensor) -> tuple:
     """(sample, token, head) strides; a dimension of one element has none that matters."""
     b, s, h, _ = t.shape
@@ -497,6 +505,7 @@ def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None
     shape = t.shape
     if len(shape) != 4:
         raise ValueError(f"{name} must be (batch, tokens, heads, dim), got {tuple(shape)}")
+    _check_sizes(t, name)
     if t.stride()[3] != 1 and shape[3] > 1:
         raise ValueError(f"{name}: the values of a head must be contiguous (stride 1), got stride {t.stride(3)}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
@@ -671,6 +680,7 @@ def quantize_rows_(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor) -> Non
     if scale.dtype != torch.float32 or scale.numel() != x.shape[0] or not scale.is_contiguous() \
             or scale.device != x.device:
         raise ValueError("scale must be a contiguous (rows,) float32 tensor on x's device")
+    _check_sizes(x, "x")
     rows, k = x.shape
     with device_ctx(x.device):
         rc = _lib.lib().lithe_quantize_rows(x.data_ptr(), _DTYPE_CODE[x.dtype], rows, k,
@@ -692,6 +702,7 @@ def _int8_weight(weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optiona
         raise TypeError(f"weight must be int8 on {dev}, got {weight.dtype} on {weight.device}")
     if weight.dim() != 2 or weight.shape[1] != k:
         raise ValueError(f"weight must be (n, {k}), got {tuple(weight.shape)}")
+    _check_sizes(weight, "weight")
     n = weight.shape[0]
     stride, inner = weight.stride()
     if n == 1:
@@ -736,6 +747,7 @@ def int8_linear_(q: torch.Tensor, x_scale: torch.Tensor, weight: torch.Tensor, w
     dev = q.device
     if q.dim() != 2 or q.dtype != torch.int8:
         raise ValueError(f"q must be (rows, k) int8, got {tuple(q.shape)} {q.dtype}")
+    _check_sizes(q, "q")
     rows, k = q.shape
     q_stride = q.stride(0) if rows > 1 else padded(k)
     if (k > 1 and q.stride(1) != 1) or q_stride % 16 or q.data_ptr() % 16:
@@ -780,6 +792,8 @@ def int8_linear_dynamic(x: torch.Tensor, weight: torch.Tensor, weight_scale: tor
             x = x.contiguous()
         rows = x.shape[0]
         x_stride = x.stride(0) if rows > 1 else k
+    if rows > _MOST:
+        raise NotImplementedError(f"x: {rows} rows are above {_MOST}")
     n, w_stride = _int8_weight(weight, weight_scale, bias, dtype, dev, k)
     expand = _int8_expand(h, b_dec, rows, n, dev)
     out = x.new_empty((*shape[:-1], n))

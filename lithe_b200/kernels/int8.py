@@ -44,6 +44,8 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
         raise ValueError(f"x must be (..., k) with k >= 1, got {tuple(x.shape)}")
     _inference_only(x)
     k = x.shape[-1]
+    if x.numel() // k > _launch._MOST:
+        raise NotImplementedError(f"x: {x.numel() // k} rows are above {_launch._MOST}")
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     if k > 1 and x2.stride(1) != 1:
         x2 = x2.contiguous()

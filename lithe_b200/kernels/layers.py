@@ -153,6 +153,12 @@ class IndexLoRALinear(nn.Module):
 FUSED_GEMM_MAX_K = 4096
 
 
+def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether torch counts the tensors' versions (it does not under inference_mode): without them a key
+    could not tell a changed tensor, so nothing is shared or kept."""
+    return not any(t is not None and t.is_inference() for t in tensors)
+
+
 class _InputKey:
     """Identifies one call's input, routing and weights by tensor identity and version, through
     weak references: a key does not keep the activation it names alive."""
@@ -220,6 +226,8 @@ class SharedInputPrep:
     def prep(self, layer: "PackedLoRALinear", x3: torch.Tensor, ids: torch.Tensor,
              w: Optional[torch.Tensor]) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
         """(h, b_dec) of ``layer`` for this call, or None when the group does not apply."""
+        if not _tracked(x3, ids, w):
+            return None
         if self._key is not None:
             if self._key.matches(x3, ids, w, None):
                 got = self._ready.pop(id(layer), None)
@@ -425,7 +433,8 @@ class PackedLoRALinear(nn.Module):
         if got is not None:
             h, b_dec = got
         else:
-            share = self.rows is not None and not compiling
+            share = self.rows is not None and not compiling and _tracked(x3, ids, w)
+            keep = not compiling and _tracked(ids)
             h = self._shared_h(x3, ids, w) if share else None
             fresh = h is None
             words = self.bank.words
@@ -433,12 +442,12 @@ class PackedLoRALinear(nn.Module):
             # contents are unchanged (a denoise loop's steps); traced graphs decode every call
             b_dec = None
             bank_key = self.bank.contents_key()
-            if not compiling and self._bdec_cache is not None and self._bdec_cache[0].matches(ids, bank_key):
+            if keep and self._bdec_cache is not None and self._bdec_cache[0].matches(ids, bank_key):
                 b_dec = self._bdec_cache[1]
             if b_dec is None:
                 h_new, b_dec = torch.ops.lithe_b200.lora_prep(x3, words, words, self._va, self._vb, self.bank.n_slots,
                                                               ids, w, d_out, self._lut, self.scaling, fresh)
-                if not compiling:
+                if keep:
                     self._bdec_cache = (_RouteKey(ids, bank_key), b_dec)
             elif fresh:
                 h_new = torch.ops.lithe_b200.lora_prep_h(x3, words, words, self._va, self._vb, self.bank.n_slots, ids,

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 from typing import Optional, Sequence, Tuple
 
 import torch
@@ -33,9 +34,16 @@ def _inference_only(*tensors: Optional[torch.Tensor]) -> None:
             raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
 
 
+def _written(*tensors: torch.Tensor) -> None:
+    """Move the version counters of tensors written behind torch's back, as an in-place op does."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
+
+
 @functools.lru_cache(maxsize=256)
 def _rotation(dim: int, axes: Tuple[int, ...], theta: float, pairing: str) -> Tuple[Tuple[int, ...], float, int]:
-    axes = tuple(int(a) for a in axes)
+    axes = tuple(operator.index(a) for a in axes)
     if pairing not in _launch.PAIRINGS:
         raise ValueError(f"pairing must be one of {tuple(_launch.PAIRINGS)}, got {pairing!r}")
     if not 1 <= len(axes) <= _lib.MAX_AXES:
@@ -59,7 +67,7 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     projection).  The result is a new tensor, or ``out`` (x itself to rotate in place).
     """
     _launch._check_heads(x, "x")
-    _inference_only(x)
+    _inference_only(x, out)
     compiling = torch.compiler.is_compiling()
     axes, theta, code = (_rotation.__wrapped__ if compiling else _rotation)(x.shape[3], tuple(axes), theta, pairing)
     fresh = out is None
@@ -73,7 +81,10 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
             return x.copy_(out)
         torch.ops.lithe_b200.rotate_axes_(out, x, positions, list(axes), theta, code)
         return out
-    return _launch.rotate_axes_(x, out, positions, axes, theta, code, True, fresh)
+    _launch.rotate_axes_(x, out, positions, axes, theta, code, True, fresh)
+    if not fresh:
+        _written(out)
+    return out
 
 
 def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Tensor],
@@ -91,7 +102,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     """
     _launch._check_heads(q, "q")
     _launch._check_heads(k, "k", q)
-    _inference_only(q, k, weight_q, weight_k)
+    _inference_only(q, k, weight_q, weight_k, out_q, out_k)
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
@@ -109,4 +120,6 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
         torch.ops.lithe_b200.qk_norm_rotate_(oq, ok, q, k, weight_q, weight_k, positions, list(axes), theta, eps, code)
         return (q.copy_(oq) if out_q is q else oq), (k.copy_(ok) if out_k is k else ok)
     _launch.qk_norm_rotate_(q, k, out_q, out_k, weight_q, weight_k, positions, axes, theta, eps, code, True, fresh)
+    if not fresh:
+        _written(out_q, out_k)
     return out_q, out_k

@@ -225,6 +225,31 @@ def test_compiled_model_on_8_bit_bases():
         assert torch.equal(torch.compile(model, fullgraph=True, backend="aot_eager")(*args), eager)
 
 
+@pytest.mark.parametrize("int8", [True, False])
+def test_inference_mode(int8):
+    """Under inference_mode torch counts no versions: nothing is shared, and the results are the same."""
+    model, args = tiny(8, int8)
+    if not int8:
+        args = (make((2, 256, 16), BF, 1), make((2, 256, 64), BF, 2), *args[2:])
+    targets = lora_targets(model)
+    bank = bank_of([(n, m.in_features, m.out_features) for n, m in targets], seed=9)
+    wrapped = wrap_packed(model, bank, scaling=20.0, int8_base=int8, fused_gemm=not int8)
+    with torch.no_grad():
+        for m in wrapped.values():
+            m.assign = torch.tensor([1, 3], dtype=torch.int32, device=DEV)
+        want = model(*args)
+    with torch.inference_mode():
+        ids = torch.tensor([1, 3], dtype=torch.int32, device=DEV)
+        for m in wrapped.values():
+            m.assign = ids
+        assert torch.equal(model(*args), want)
+        ids.copy_(torch.tensor([4, 4], dtype=torch.int32, device=DEV))
+        moved = model(*args)
+        x = make((1, 3, 2, 64), BF, 1)
+        qk_norm_rotate(x, x.clone(), None, None, torch.zeros(3, 1, device=DEV), (64,), out_q=x)
+    assert not torch.equal(moved, want)
+
+
 def test_captured_layer():
     bank = bank_of([("m", 256, 512)])
     layer = PackedLoRALinear(linear(256, 512), bank, "m", 16, 2.0, int8_base=True)

@@ -188,6 +188,17 @@ def test_joint_buffer_leaves_the_other_tokens():
     assert torch.equal(joint[:, :30], before[:, :30]) and torch.equal(joint[:, 51:], before[:, 51:])
 
 
+def test_a_written_tensor_says_so():
+    """torch's version counter of an output that the caller gave moves, as for any in-place write (the
+    layers' shared preparations tell inputs apart by it)."""
+    x = make((1, 3, 2, 64), torch.bfloat16, 1)
+    pos = torch.zeros(3, 1, device=DEV)
+    for write in (lambda: rotate_axes(x, pos, (64,), out=x), lambda: qk_norm_rotate(x, x.clone(), None, None, pos, (64,), out_q=x)):
+        before = x._version
+        write()
+        assert x._version > before
+
+
 def test_heads_do_not_meet():
     """A head of zeros stays zero, a head with a NaN or an infinity spoils only itself."""
     q = make((1, 3, 6, 64), torch.bfloat16, 1)

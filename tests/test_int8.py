@@ -19,6 +19,8 @@ def _linear(q=0x10000, q_stride=128, xs=0x20000, w=0x30000, w_stride=128, ws=0x4
     ({"n": 0}, _lib.ERR_ARG),
     ({"k": 0}, _lib.ERR_ARG),
     ({"k": 131073, "q_stride": 131088, "w_stride": 131088}, _lib.ERR_UNSUPPORTED),
+    ({"rows": 2 ** 31 - 1}, _lib.ERR_UNSUPPORTED),
+    ({"n": 2 ** 31 - 1}, _lib.ERR_UNSUPPORTED),
     ({"q": 0x10008}, _lib.ERR_ARG),
     ({"q": None}, _lib.ERR_ARG),
     ({"q_stride": 100}, _lib.ERR_ARG),
@@ -135,6 +137,18 @@ def test_launch_checks(monkeypatch):
                      ("b_dec", None)]:
         with pytest.raises((ValueError, TypeError)):
             _launch.int8_linear_(**{**ok, key: bad})
+
+
+def test_sizes_beyond_32_bits_are_refused(monkeypatch):
+    monkeypatch.setattr(_launch, "_require_cuda", lambda t, what: None)
+    x = torch.zeros(1, 1, dtype=torch.bfloat16).expand(2 ** 32 + 5, 1)
+    w, ws = torch.zeros(4, 16, dtype=torch.int8)[:, :1], torch.zeros(4)
+    with pytest.raises(NotImplementedError):
+        int8_linear(x, w, ws)
+    with pytest.raises(NotImplementedError):
+        quantize_rows(x)
+    with pytest.raises(NotImplementedError):
+        int8_linear(x[:1], w[:1].expand(2 ** 31, 1), ws[:1].expand(2 ** 31))
 
 
 def test_ops_know_their_shapes():

@@ -45,6 +45,7 @@ def _rotate(x=None, out=None, dtype=_lib.DTYPE_BF16, batch=1, tokens=4, dim=64, 
     ({"x": _view(base=None)}, _lib.ERR_ARG),
     ({"x": _view(base=0x10001)}, _lib.ERR_ARG),
     ({"x": _view(heads=0)}, _lib.ERR_ARG),
+    ({"x": _view(heads=2 ** 30 + 1)}, _lib.ERR_UNSUPPORTED),
     ({"x": _view(token_stride=-256)}, _lib.ERR_ARG),
     ({"out": _view(heads=3)}, _lib.ERR_ARG),
 ])
@@ -96,6 +97,12 @@ def test_python_checks():
             rotate_axes(x.transpose(2, 3), pos, (2,))
         with pytest.raises(RuntimeError, match="inference-only"):
             rotate_axes(x.float().requires_grad_(), pos, (32, 32))
+        with pytest.raises(TypeError):
+            rotate_axes(x, pos, (32.5, 2))
+        with pytest.raises(RuntimeError, match="inference-only"):
+            rotate_axes(x, pos, (32, 32), out=torch.empty(2, 4, 3, 64, dtype=x.dtype, device="cuda", requires_grad=True))
+        with pytest.raises(NotImplementedError):
+            rotate_axes(x[:1].expand(2 ** 31, 4, 3, 64), pos, (32, 32))
         with pytest.raises(ValueError, match="eps"):
             qk_norm_rotate(x, x, None, None, pos, (32, 32), eps=-1.0)
         with pytest.raises(ValueError, match="type and device"):
