@@ -78,6 +78,11 @@ LITHE_API int32_t lithe_abi_version(void);
 /* Message for the last non-zero return on the calling thread ("" if none). */
 LITHE_API const char* lithe_last_error(void);
 
+/* The id of the CUDA-graph capture in progress on the stream, 0 when there is none, -1 when the stream
+ * cannot be queried.  Work recorded in a capture runs only at its replays: a result made in one capture
+ * must not be handed to a call outside of it, nor the other way round. */
+LITHE_API int64_t lithe_capture_id(void* stream);
+
 /*
  * Fused index-resident per-sample LoRA forward for one linear (replaces the two Triton
  * launches of shared_codebook_lora_delta, lithe/kernels/shared.py:197-263, plus the

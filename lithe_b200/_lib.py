@@ -46,6 +46,7 @@ _c = ctypes
 _SIGNATURES = {
     "lithe_abi_version": (_c.c_int32, []),
     "lithe_last_error": (_c.c_char_p, []),
+    "lithe_capture_id": (_c.c_int64, [_c.c_void_p]),
 }
 
 

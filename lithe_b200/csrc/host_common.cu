@@ -174,4 +174,16 @@ int32_t lithe_abi_version(void) { return LITHE_ABI_VERSION; }
 
 const char* lithe_last_error(void) { return lithe::g_error; }
 
+int64_t lithe_capture_id(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id);
+    if (e != cudaSuccess) {
+        lithe::fail_cuda(e, "cudaStreamGetCaptureInfo");
+        cudaGetLastError();          // the caller is told; its next launch check must not be
+        return -1;
+    }
+    return status == cudaStreamCaptureStatusActive ? static_cast<int64_t>(id) : 0;
+}
+
 }  // extern "C"

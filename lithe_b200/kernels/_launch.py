@@ -11,7 +11,7 @@ import ctypes
 import functools
 import struct
 import threading
-from typing import Optional, Sequence
+from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -84,6 +84,14 @@ def stream_handle(device: torch.device) -> int:
     if _raw_stream is not None and device.index is not None:
         return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def ordered_after(device: torch.device) -> Optional[Tuple[int, int]]:
+    """What a later call must share with this one to find its results made: the current stream and the
+    CUDA-graph capture in progress there (0 for none).  None when the stream cannot be queried."""
+    stream = stream_handle(device)
+    capture = _lib.lib().lithe_capture_id(stream)
+    return None if capture < 0 else (stream, capture)
 
 
 _lut_cache: dict = {}

@@ -161,34 +161,44 @@ def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
 
 class _InputKey:
     """Identifies one call's input, routing and weights by tensor identity and version, through
-    weak references: a key does not keep the activation it names alive."""
+    weak references: a key does not keep the activation it names alive.  It names the stream and the
+    graph capture too: on another stream the results may not be there yet, and a captured call whose
+    replays see new values in the same tensors needs its own, made in that capture."""
 
     def __init__(self, x3, ids, w, scaling):
         self._refs = (weakref.ref(x3), weakref.ref(ids), None if w is None else weakref.ref(w))
         self._vals = (x3._version, ids._version, None if w is None else w._version, scaling)
+        self._where = _launch.ordered_after(x3.device)
 
     def alive(self) -> bool:
         """The input tensor still exists (an activation is freed once its forward is done)."""
         return self._refs[0]() is not None
 
+    def here(self, device) -> bool:
+        """The key was made on the current stream, inside the same capture or outside of any."""
+        return self._where == _launch.ordered_after(device)
+
     def matches(self, x3, ids, w, scaling) -> bool:
         rx, ri, rw = self._refs
         if rx() is not x3 or ri() is not ids or (rw is None) != (w is None) or (rw is not None and rw() is not w):
             return False
-        return self._vals == (x3._version, ids._version, None if w is None else w._version, scaling)
+        return (self._vals == (x3._version, ids._version, None if w is None else w._version, scaling)
+                and self._where is not None and self._where == _launch.ordered_after(x3.device))
 
 
 class _RouteKey:
     """Identifies the routing a decoded B factor was made for: the slot-id tensor (identity and
-    version, through a weak reference) and the caller's tuple of what else it depends on (the
-    index bank's contents key, the group's members)."""
+    version, through a weak reference), the caller's tuple of what else it depends on (the
+    index bank's contents key, the group's members), and the stream and capture (see _InputKey)."""
 
     def __init__(self, ids, extra):
         self._ref = weakref.ref(ids)
         self._vals = (ids._version, extra)
+        self._where = _launch.ordered_after(ids.device)
 
     def matches(self, ids, extra) -> bool:
-        return self._ref() is ids and self._vals == (ids._version, extra)
+        return (self._ref() is ids and self._vals == (ids._version, extra)
+                and self._where is not None and self._where == _launch.ordered_after(ids.device))
 
 
 class SharedInputPrep:
@@ -199,7 +209,8 @@ class SharedInputPrep:
     each member's own lithe_lora_prep.  A member called on another input while results for a
     live input are pending, called again on an input it already took, on the cuBLAS path, or
     under torch.compile (the hand-over keys on tensor identity, which a traced graph does not
-    have), computes its own.  Pending results for an input that has been freed are dropped.
+    have), computes its own.  Pending results for an input that has been freed, or that were
+    made on another stream or in another graph capture, are dropped.
     Members must share one ``assign`` tensor (int32, on the device) for the hand-over to
     apply.  The members' decoded B factors are kept for the last routing (see
     PackedLoRALinear's B-factor cache)."""
@@ -236,7 +247,7 @@ class SharedInputPrep:
                 # None: this member already took its result for this input and is called on it
                 # again; it prepares its own
                 return got
-            if self._key.alive():
+            if self._key.alive() and self._key.here(x3.device):
                 return None         # results for another, live input are pending: prepare alone
         members = [m for m in self.members
                    if m._takes_expand(x3) and _slot_ids(m.assign, x3) is ids

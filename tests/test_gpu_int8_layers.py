@@ -265,3 +265,61 @@ def test_captured_layer():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, layer(x))
+
+
+@pytest.mark.parametrize("int8", [True, False])
+def test_captured_block_computes_its_own(int8):
+    """q, k and v of one block, called on an input before and while a graph is captured: replays follow the
+    input's and the routing's new values, also once the layers have gone on to another routing."""
+    names = ["b.attn.to_q", "b.attn.to_k", "b.attn.to_v"]
+    bank = bank_of([(n, 256, 256) for n in names])
+    block = nn.Module()
+    block.b = nn.Module()
+    block.b.attn = nn.Module()
+    for i, n in enumerate(names):
+        setattr(block.b.attn, n.split(".")[-1], linear(256, 256, seed=20 * i))
+    layers = list(wrap_packed(block, bank, scaling=2.0, int8_base=int8, fused_gemm=not int8).values())
+    ids = torch.tensor([1, 4], dtype=torch.int32, device=DEV)
+    for m in layers:
+        m.assign = ids
+    assert layers[0].prep_group is not None
+    x = make((2, 128, 256), BF, 1)
+    with torch.no_grad():
+        layers[0](x)                                 # leaves the other two's results pending
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            outs = [m(x) for m in layers]
+            pending = len(layers[0].prep_group._ready)
+        assert pending == 0                          # one preparation, shared among the three
+        x.copy_(make((2, 128, 256), BF, 2))
+        ids.copy_(torch.tensor([3, 0], dtype=torch.int32, device=DEV))
+        other = torch.tensor([5, 5], dtype=torch.int32, device=DEV)
+        for m in layers:
+            m.assign = other
+            m(make((2, 128, 256), BF, 3))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [o.clone() for o in outs]
+        for m, g in zip(layers, got):
+            m.assign = ids
+            assert torch.equal(m(x), g)
+
+
+def test_results_shared_on_one_stream_alone():
+    """A kept B factor is used on the stream that made it; another stream's call makes its own."""
+    bank = bank_of([("m", 256, 512)])
+    layer = PackedLoRALinear(linear(256, 512), bank, "m", 16, 2.0, int8_base=True)
+    layer.assign = torch.tensor([1, 4], dtype=torch.int32, device=DEV)
+    x = make((2, 40, 256), BF, 1)
+    with torch.no_grad():
+        want = layer(x)
+        kept = layer._bdec_cache[1]
+        assert torch.equal(layer(x), want) and layer._bdec_cache[1] is kept
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = layer(x)
+            assert layer._bdec_cache[1] is not kept
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
