@@ -30,7 +30,9 @@ constexpr int kMostRows = 0x7fffffff - 1024;   // rows and channels of whole til
 // Bound: HBM (x read once, a byte a value written).  kWarps warps take a row, each lane up to kPieces
 // 8-value pieces of it, which stay in registers between the maximum and the rounding: one warp where
 // there are many rows (57344 x 3072: 80 us, 6.6 TB/s; four a row 102 us), four where there are few and
-// their latency counts (one row 1.8 us; 3.0 us).  A longer row is read twice (the second time from L2).
+// their latency counts (one row 1.8 us; 3.0 us).  A longer row is read twice, the second time from L2
+// (20000 x 18432: 216 us, 5.1 TB/s).  Rows that do not start on 16-byte boundaries are put together out of
+// aligned pieces (20000 x 1001: 18 us, value by value 29 us; 1237 x 1898: 3.8 and 6.1 us).
 // The quotients of a piece are checked for nearness to halfway together, with a bound (2^-13) above every
 // 2^-21 |t|; the few pieces it stops are done value by value.
 // ------------------------------------------------------------------------------------------
@@ -100,7 +102,71 @@ __device__ __forceinline__ uint2 quantize8(const uint4& v, float pre, float r) {
     return make_uint2(__byte_perm(a0, a1, 0x5410), __byte_perm(a2, a3, 0x5410));
 }
 
-template <bool kF16, int kWarps, int kPieces>
+// A lane's kPieces pieces of a row of k values, the first one's number at0 and the rest kLanes apart: piece
+// `at` is the values 8 at to 8 at + 7, zeros from k on.  kWhole: rows are whole pieces on 16-byte
+// boundaries.  Else a piece is shifted together out of the two 16-byte granules it lies in, all of them
+// loaded before the first is used; those that reach beyond the row are read value by value then.
+template <bool kWhole, int kLanes, int kPieces>
+__device__ __forceinline__ void load_pieces(const uint16_t* row, int at0, int k, uint4 (&v)[kPieces]) {
+    if constexpr (kWhole) {
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+            const int at = c * kLanes + at0;
+            v[c] = 8 * at < k ? __ldg(reinterpret_cast<const uint4*>(row) + at) : make_uint4(0, 0, 0, 0);
+        }
+    } else {
+        const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 7;
+        uint4 g[kPieces][2];
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int first = 8 * (c * kLanes + at0 + e) - shift;          // the granule's first value
+                g[c][e] = first >= 0 && first + 8 <= k ? __ldg(reinterpret_cast<const uint4*>(row + first))
+                                                       : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int first = 8 * (c * kLanes + at0 + e) - shift;
+                if (first < k && (first < 0 || first + 8 > k)) {
+                    uint32_t x[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = first + i >= 0 && first + i < k ? __ldg(row + first + i) : 0u;
+                    g[c][e] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+                }
+                w[4 * e] = g[c][e].x, w[4 * e + 1] = g[c][e].y, w[4 * e + 2] = g[c][e].z, w[4 * e + 3] = g[c][e].w;
+            }
+#pragma unroll
+            for (int i = 0; i < 6; ++i) w[i] = shift & 4 ? w[i + 2] : w[i];
+#pragma unroll
+            for (int i = 0; i < 5; ++i) w[i] = shift & 2 ? w[i + 1] : w[i];
+            const int half = 16 * (shift & 1);
+            v[c] = make_uint4(__funnelshift_r(w[0], w[1], half), __funnelshift_r(w[1], w[2], half),
+                              __funnelshift_r(w[2], w[3], half), __funnelshift_r(w[3], w[4], half));
+        }
+    }
+}
+
+// Its bytes to q's row (which starts on a 16-byte boundary); those from k on are left as they are.
+template <bool kWhole>
+__device__ __forceinline__ void store_piece(int8_t* row, int at, int k, const uint2& b) {
+    if (kWhole || 8 * at + 8 <= k) {
+        reinterpret_cast<uint2*>(row)[at] = b;
+    } else {
+        for (int i = 0; 8 * at + i < k; ++i)
+            row[8 * at + i] = static_cast<int8_t>(((i < 4 ? b.x : b.y) >> (8 * (i & 3))) & 0xffu);
+    }
+}
+
+__device__ __forceinline__ uint32_t max_of(uint32_t m, const uint4& v) {
+    return __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)),
+                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+}
+
+template <bool kF16, bool kWhole, int kWarps, int kPieces>
 __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int kLanes = 32 * kWarps, kRowsCta = kThreadsQ / kLanes;
@@ -108,19 +174,13 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p
     const int warp = threadIdx.x >> 5, at0 = threadIdx.x % kLanes;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsCta + threadIdx.x / kLanes;
     const bool live = row < p.rows;
-    const uint4* x = reinterpret_cast<const uint4*>(p.x + row * p.x_stride);
-    const int pieces = live ? p.k >> 3 : 0;
+    const uint16_t* x = p.x + row * p.x_stride;
+    const int pieces = live ? (p.k + 7) >> 3 : 0;
     uint4 v[kPieces];
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c) {
-        const int at = c * kLanes + at0;
-        v[c] = at < pieces ? __ldg(x + at) : make_uint4(0, 0, 0, 0);
-    }
+    load_pieces<kWhole, kLanes>(x, at0, live ? p.k : 0, v);
     uint32_t m = 0;
 #pragma unroll
-    for (int c = 0; c < kPieces; ++c)
-        m = __vmaxu2(__vmaxu2(m, __vmaxu2(v[c].x & 0x7fff7fffu, v[c].y & 0x7fff7fffu)),
-                     __vmaxu2(v[c].z & 0x7fff7fffu, v[c].w & 0x7fff7fffu));
+    for (int c = 0; c < kPieces; ++c) m = max_of(m, v[c]);
     m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
     if constexpr (kWarps > 1) {
         if ((threadIdx.x & 31) == 0) part[warp] = m;
@@ -131,63 +191,72 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p
     if (!live) return;
     float pre, r;
     row_factors<kF16>(m, at0 == 0, p.scale + row, pre, r);
-    uint2* q = reinterpret_cast<uint2*>(p.q + row * p.q_stride);
+    int8_t* q = p.q + row * p.q_stride;
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
         const int at = c * kLanes + at0;
-        if (at < pieces) q[at] = pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r);
+        if (at < pieces)
+            store_piece<kWhole>(q, at, p.k, pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r));
     }
 }
 
-__device__ __forceinline__ uint32_t block_max(uint32_t v) {
-    __shared__ uint32_t part[kThreadsQ / 32];
-    v = __reduce_max_sync(0xffffffffu, v);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    uint32_t m = part[0];
-#pragma unroll
-    for (int i = 1; i < kThreadsQ / 32; ++i) m = max(m, part[i]);
-    return m;
-}
-
-// Rows that start anywhere, value by value.  Short ones: a warp a row, each lane kValues of it in
-// registers (20000 x 100: 6.3 us, 21 us by the kernel below).
-template <bool kF16, int kValues>
+// Short rows that start anywhere: a warp a row, value by value, each lane kShort of them (20000 x 100: 6.0 us
+// by 4 a lane, 7.4 us by 12, 10.2 us by pieces; x 301: 10.7 and 13.1 us; x 500: 14.5 by 16 and 11.7 us).
+constexpr int kShortMost = 12;
+template <bool kF16, int kShort>
 __global__ void __launch_bounds__(kThreadsQ) quantize_short_kernel(const QuantParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * (kThreadsQ / 32) + (threadIdx.x >> 5);
     if (row >= p.rows) return;
     const uint16_t* x = p.x + row * p.x_stride;
-    uint32_t v[kValues], m = 0;
+    uint32_t v[kShort], m = 0;
 #pragma unroll
-    for (int c = 0; c < kValues; ++c) v[c] = 32 * c + lane < p.k ? __ldg(x + 32 * c + lane) : 0u;
+    for (int c = 0; c < kShort; ++c) v[c] = 32 * c + lane < p.k ? __ldg(x + 32 * c + lane) : 0u;
 #pragma unroll
-    for (int c = 0; c < kValues; ++c) m = max(m, v[c] & 0x7fffu);
+    for (int c = 0; c < kShort; ++c) m = max(m, v[c] & 0x7fffu);
     m = __reduce_max_sync(0xffffffffu, m);
     float pre, r;
     row_factors<kF16>(m, lane == 0, p.scale + row, pre, r);
     int8_t* q = p.q + row * p.q_stride;
 #pragma unroll
-    for (int c = 0; c < kValues; ++c)
+    for (int c = 0; c < kShort; ++c)
         if (32 * c + lane < p.k)
             q[32 * c + lane] = pre == 0.0f ? 0 : static_cast<int8_t>(quantize(value_of<kF16>(v[c]) * pre, r) & 0xffu);
 }
 
-// Longer ones: a CTA a row, read twice.
-template <bool kF16>
-__global__ void __launch_bounds__(kThreadsQ) quantize_any_kernel(const QuantParams p) {
+// Rows that registers do not hold: a CTA a row, read twice.
+template <bool kF16, bool kWhole>
+__global__ void __launch_bounds__(kThreadsQ) quantize_long_kernel(const QuantParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    __shared__ uint32_t part[kThreadsQ / 32];
     const int64_t row = blockIdx.x;
     const uint16_t* x = p.x + row * p.x_stride;
     int8_t* q = p.q + row * p.q_stride;
+    constexpr int kPieces = 4;
+    const int pieces = (p.k + 7) >> 3;
     uint32_t m = 0;
-    for (int i = threadIdx.x; i < p.k; i += kThreadsQ) m = max(m, static_cast<uint32_t>(__ldg(x + i)) & 0x7fffu);
-    m = block_max(m);
+    uint4 v[kPieces];
+    for (int at = threadIdx.x; at < pieces; at += kPieces * kThreadsQ) {
+        load_pieces<kWhole, kThreadsQ>(x, at, p.k, v);
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) m = max_of(m, v[c]);
+    }
+    m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreadsQ / 32; ++i) m = max(m, part[i]);
     float pre, r;
     row_factors<kF16>(m, threadIdx.x == 0, p.scale + row, pre, r);
-    for (int i = threadIdx.x; i < p.k; i += kThreadsQ)
-        q[i] = pre == 0.0f ? 0 : static_cast<int8_t>(quantize(value_of<kF16>(__ldg(x + i)) * pre, r) & 0xffu);
+    for (int at = threadIdx.x; at < pieces; at += kPieces * kThreadsQ) {
+        load_pieces<kWhole, kThreadsQ>(x, at, p.k, v);
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c)
+            if (at + c * kThreadsQ < pieces)
+                store_piece<kWhole>(q, at + c * kThreadsQ, p.k,
+                                    pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r));
+    }
 }
 
 // ------------------------------------------------------------------------------------------
@@ -1166,33 +1235,33 @@ int32_t launch_linear(const Params& p, bool after_quantize, cudaStream_t st) {
                 : launch_tiles<false, kF16, kExpandNone>(p, device, sms, after_quantize, st);
 }
 
-template <bool kF16, int kWarps, int kPieces>
+template <bool kF16, bool kWhole, int kWarps, int kPieces>
 void launch_quantize_rows(const QuantParams& p, cudaStream_t st) {
     constexpr int kRowsCta = kThreadsQ / (32 * kWarps);
-    quantize_kernel<kF16, kWarps, kPieces><<<static_cast<int>((static_cast<int64_t>(p.rows) + kRowsCta - 1) / kRowsCta), kThreadsQ, 0, st>>>(p);
+    const int64_t ctas = (static_cast<int64_t>(p.rows) + kRowsCta - 1) / kRowsCta;
+    quantize_kernel<kF16, kWhole, kWarps, kPieces><<<static_cast<int>(ctas), kThreadsQ, 0, st>>>(p);
 }
 
-template <bool kF16>
+template <bool kF16, bool kWhole>
 int32_t launch_quantize(const QuantParams& p, cudaStream_t st) {
-    // whole 16-byte pieces of x to whole 8-byte pieces of q
-    const bool vec = p.k % 8 == 0 && p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
-    const int pieces = p.k / 8;
+    const int pieces = (p.k + 7) / 8;
+    const int short_ctas = static_cast<int>((static_cast<int64_t>(p.rows) + kThreadsQ / 32 - 1) / (kThreadsQ / 32));
     // (3072 values: four warps a row are faster up to 1024 rows, and one from 4096 on)
-    const bool few = p.rows <= 2048;
-    const int four = static_cast<int>((static_cast<int64_t>(p.rows) + 3) / 4);
-    if (!vec && p.k <= 32 * 4) quantize_short_kernel<kF16, 4><<<four, kThreadsQ, 0, st>>>(p);
-    else if (!vec && p.k <= 32 * 16) quantize_short_kernel<kF16, 16><<<four, kThreadsQ, 0, st>>>(p);
-    else if (!vec) quantize_any_kernel<kF16><<<p.rows, kThreadsQ, 0, st>>>(p);
-    else if (few && pieces <= 128 * 4) launch_quantize_rows<kF16, 4, 4>(p, st);
-    else if (pieces <= 32 * 4) launch_quantize_rows<kF16, 1, 4>(p, st);
-    else if (pieces <= 32 * 8) launch_quantize_rows<kF16, 1, 8>(p, st);
-    else if (pieces <= 32 * 12) launch_quantize_rows<kF16, 1, 12>(p, st);
-    else if (pieces <= 64 * 8) launch_quantize_rows<kF16, 2, 8>(p, st);
-    else if (pieces <= 64 * 12) launch_quantize_rows<kF16, 2, 12>(p, st);
-    else if (pieces <= 128 * 8) launch_quantize_rows<kF16, 4, 8>(p, st);
-    else if (pieces <= 128 * 12) launch_quantize_rows<kF16, 4, 12>(p, st);
-    else if (pieces <= 128 * 16) launch_quantize_rows<kF16, 4, 16>(p, st);
-    else quantize_any_kernel<kF16><<<p.rows, kThreadsQ, 0, st>>>(p);
+    const bool few = p.rows <= 2048 && pieces > 32 * 2;
+    if (!kWhole && p.k <= 32 * 4) quantize_short_kernel<kF16, 4><<<short_ctas, kThreadsQ, 0, st>>>(p);
+    else if (!kWhole && p.k <= 32 * kShortMost) quantize_short_kernel<kF16, kShortMost><<<short_ctas, kThreadsQ, 0, st>>>(p);
+    else if (few && pieces <= 128 * 2) launch_quantize_rows<kF16, kWhole, 4, 2>(p, st);
+    else if (few && pieces <= 128 * 4) launch_quantize_rows<kF16, kWhole, 4, 4>(p, st);
+    else if (pieces <= 32 * 2) launch_quantize_rows<kF16, kWhole, 1, 2>(p, st);
+    else if (pieces <= 32 * 4) launch_quantize_rows<kF16, kWhole, 1, 4>(p, st);
+    else if (pieces <= 32 * 8) launch_quantize_rows<kF16, kWhole, 1, 8>(p, st);
+    else if (kWhole && pieces <= 32 * 12) launch_quantize_rows<kF16, kWhole, 1, 12>(p, st);
+    else if (pieces <= 64 * 8) launch_quantize_rows<kF16, kWhole, 2, 8>(p, st);
+    else if (kWhole && pieces <= 64 * 12) launch_quantize_rows<kF16, kWhole, 2, 12>(p, st);
+    else if (pieces <= 128 * 8) launch_quantize_rows<kF16, kWhole, 4, 8>(p, st);
+    else if (kWhole && pieces <= 128 * 12) launch_quantize_rows<kF16, kWhole, 4, 12>(p, st);
+    else if (kWhole && pieces <= 128 * 16) launch_quantize_rows<kF16, kWhole, 4, 16>(p, st);
+    else quantize_long_kernel<kF16, kWhole><<<p.rows, kThreadsQ, 0, st>>>(p);
     const cudaError_t e = cudaGetLastError();
     return e == cudaSuccess ? LITHE_OK : fail_cuda(e, "quantize_kernel launch");
 }
@@ -1257,7 +1326,10 @@ int32_t linear_params(Params* p, const void* w, int64_t w_stride, const float* w
 }
 
 int32_t quantize(const QuantParams& p, int32_t dtype, cudaStream_t st) {
-    return dtype == LITHE_DTYPE_F16 ? launch_quantize<true>(p, st) : launch_quantize<false>(p, st);
+    // whole 16-byte pieces of x to whole 8-byte pieces of q
+    const bool whole = p.k % 8 == 0 && p.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(p.x) % 16 == 0;
+    if (dtype == LITHE_DTYPE_F16) return whole ? launch_quantize<true, true>(p, st) : launch_quantize<true, false>(p, st);
+    return whole ? launch_quantize<false, true>(p, st) : launch_quantize<false, false>(p, st);
 }
 
 // after_quantize: the stream's last launch is the quantisation of these activations.

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 from lithe_b200 import device_errors
-from lithe_b200.kernels import int8_linear, quantize_rows, quantize_weight
+from lithe_b200.kernels import _launch, int8_linear, quantize_rows, quantize_weight
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -257,3 +257,26 @@ def test_compiled_call():
     x = make((5, 96), torch.bfloat16, 1)
     fn = torch.compile(lambda t: int8_linear(t, w, ws), fullgraph=True, backend="aot_eager")
     assert torch.equal(fn(x), int8_linear(x, w, ws))
+
+
+@pytest.mark.parametrize("k", [1, 7, 15, 127, 129, 384, 385, 392, 500, 1001, 2049, 4100, 8191, 8200, 16385, 20481])
+def test_rows_from_any_element_on(k):
+    """Rows from each of the 8 places in a 16-byte piece on, an odd stride apart, between NaNs that are not
+    theirs; the bytes behind a row of q are left as they are."""
+    rows = 5
+    wide = torch.full((rows, (k + 20) | 1), NAN, dtype=torch.bfloat16, device=DEV)
+    values = make((rows, k), torch.bfloat16, k)
+    values[rows - 1, k - 1] = 9.0                   # the maximum as the last value
+    want, scale = exact_rows(values)
+    for at in range(9):
+        wide.fill_(NAN)
+        wide[:, at:at + k] = values
+        q = torch.full((rows, (k + 15) // 16 * 16 + 16), 77, dtype=torch.int8, device=DEV)
+        s = torch.empty(rows, device=DEV)
+        _launch.quantize_rows_(wide[:, at:at + k], q[:, :k], s)
+        assert torch.equal(q[:, :k].double(), want) and torch.equal(s, scale.float()), at
+        assert bool((q[:, k:] == 77).all()), at
+    many = values.repeat(500, 1)                    # 2500 rows: another split
+    if k % 2:
+        got = quantize_rows(many)
+        assert torch.equal(got.q.double(), want.repeat(500, 1))
