@@ -129,11 +129,13 @@ def lut_from_list(lut) -> ctypes.Array:
 
 
 _NO_CONTEXT = contextlib.nullcontext()
+# The current device without torch.cuda's look at whether CUDA is up (a tensor of the device is at hand).
+_raw_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def device_ctx(device: torch.device):
     """torch.cuda.device(device), or a no-op when it is already the current device."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == _raw_device():
         return _NO_CONTEXT
     return torch.cuda.device(device)
 
@@ -499,11 +501,30 @@ def _heads_strides(t: torch.Tensor) -> tuple:
 _pack_view = struct.Struct("PqqqiI").pack
 
 
-def _heads_view(t: torch.Tensor) -> bytes:
-    """A lithe_heads_view of ``t`` as the bytes of the struct (a fifth of a ctypes object's cost)."""
-    b, s, h, _ = t.shape
+def _heads_layout(t: torch.Tensor) -> tuple:
+    """(lithe_heads_view of ``t``, the address of its first byte, the one behind its last, whether its heads,
+    tokens and samples follow one another without meeting)."""
+    b, s, h, d = t.shape
     sb, ss, sh, _ = t.stride()
-    return _pack_view(t.data_ptr(), sb if b != 1 else 0, ss if s != 1 else 0, sh if h != 1 else 0, h, 0)
+    apart = True
+    inner = d
+    if h == 1:
+        sh = 0
+    else:
+        apart = sh >= inner
+        inner += (h - 1) * sh
+    if s == 1:
+        ss = 0
+    else:
+        apart = apart and ss >= inner
+        inner += (s - 1) * ss
+    if b == 1:
+        sb = 0
+    else:
+        apart = apart and sb >= inner
+        inner += (b - 1) * sb
+    first = t.data_ptr()
+    return _pack_view(first, sb, ss, sh, h, 0), first, first + inner * t.element_size(), apart
 
 
 def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
@@ -521,19 +542,8 @@ def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None
                          f"{t.dtype}, {t.device}")
 
 
-def _byte_span(t: torch.Tensor) -> tuple:
-    b, s, h, d = t.shape
-    sb, ss, sh, sd = t.stride()
-    first = t.data_ptr()
-    return first, first + ((b - 1) * sb + (s - 1) * ss + (h - 1) * sh + (d - 1) * sd + 1) * t.element_size()
-
-
 def _has_own_elements(t: torch.Tensor) -> bool:
     """Whether no two of ``t``'s elements share an address (an expanded tensor's do)."""
-    b, s, h, d = t.shape
-    sb, ss, sh, _ = t.stride()
-    if (h == 1 or sh >= d) and (s == 1 or ss >= (h - 1) * sh + d) and (b == 1 or sb >= (s - 1) * ss + (h - 1) * sh + d):
-        return True
     reach = 0
     for s, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
         if s <= reach:
@@ -547,8 +557,8 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
     not meet, or they are slices of one buffer that leave each other's part of every token alone."""
     if a.numel() == 0 or b.numel() == 0:
         return True
-    a0, a1 = _byte_span(a)
-    b0, b1 = _byte_span(b)
+    _, a0, a1, _ = _heads_layout(a)
+    _, b0, b1, _ = _heads_layout(b)
     if a1 <= b0 or b1 <= a0:
         return True
     sa, sb = _heads_strides(a), _heads_strides(b)
@@ -577,17 +587,20 @@ def _same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a.data_ptr() == b.data_ptr() and a.shape == b.shape and _heads_strides(a) == _heads_strides(b)
 
 
-def _check_outputs(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], names: Sequence[str]) -> None:
-    """Every output is its own input (in place) or shares no element with an input or another output."""
-    spans = [_byte_span(t) for t in (*ins, *outs)]
+def _check_outputs(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], names: Sequence[str],
+                   layouts: Optional[Sequence[tuple]] = None) -> None:
+    """Every output is its own input (in place) or shares no element with an input or another output.
+    ``layouts``: _heads_layout of the inputs and the outputs, where they are at hand."""
     n = len(ins)
+    if layouts is None:
+        layouts = [_heads_layout(t) for t in (*ins, *outs)]
     for i, o in enumerate(outs):
-        if not _has_own_elements(o):
+        _, o0, o1, apart = layouts[n + i]
+        if not apart and not _has_own_elements(o):
             raise ValueError(f"{names[i]} has elements that share an address")
-        o0, o1 = spans[n + i]
         for j in range(n + i):
-            x0, x1 = spans[j]
-            if x1 <= o0 or o1 <= x0:
+            x = layouts[j]
+            if x[2] <= o0 or o1 <= x[1]:
                 continue
             if j >= n:
                 if not _apart(o, outs[j - n]):
@@ -623,9 +636,11 @@ def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, ax
             _check_heads(out, "out", x)
             if out.shape != x.shape:
                 raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
-        _check_outputs((x,), (out,), ("out",))
+    of_x, of_out = _heads_layout(x), _heads_layout(out)
+    if not fresh:
+        _check_outputs((x,), (out,), ("out",), (of_x, of_out))
     b, s, _, d = x.shape
-    args = (_heads_view(x), _heads_view(out), _DTYPE_CODE[x.dtype], b, s, d,
+    args = (of_x[0], of_out[0], _DTYPE_CODE[x.dtype], b, s, d,
             *_rotation_args(x, positions, tuple(axes), theta, pairing))
     with device_ctx(x.device):
         rc = _lib.lib().lithe_rotate_axes(*args)
@@ -649,7 +664,9 @@ def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k
         if out_q.shape != q.shape or out_k.shape != k.shape:
             raise ValueError(f"out_q and out_k must be {tuple(q.shape)} and {tuple(k.shape)}, got "
                              f"{tuple(out_q.shape)} and {tuple(out_k.shape)}")
-        _check_outputs((q, k), (out_q, out_k), ("out_q", "out_k"))
+    layouts = [_heads_layout(t) for t in (q, k, out_q, out_k)]
+    if not fresh:
+        _check_outputs((q, k), (out_q, out_k), ("out_q", "out_k"), layouts)
     b, s, _, d = q.shape
     if k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch, tokens and dim")
@@ -664,7 +681,7 @@ def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k
         weight_dtype = w.dtype
     if weight_q is not None and weight_k is not None and weight_q.dtype != weight_k.dtype:
         raise TypeError(f"weight_q and weight_k must have one type, got {weight_q.dtype} and {weight_k.dtype}")
-    args = (_heads_view(q), _heads_view(k), _heads_view(out_q), _heads_view(out_k), weight_q.data_ptr() if weight_q is not None else None,
+    args = (*(t[0] for t in layouts), weight_q.data_ptr() if weight_q is not None else None,
             weight_k.data_ptr() if weight_k is not None else None, _DTYPE_CODE[weight_dtype], eps,
             _DTYPE_CODE[dtype], b, s, d, *_rotation_args(q, positions, tuple(axes), theta, pairing))
     with device_ctx(q.device):

@@ -35,10 +35,9 @@ def _inference_only(*tensors: Optional[torch.Tensor]) -> None:
 
 
 def _written(*tensors: torch.Tensor) -> None:
-    """Move the version counters of tensors written behind torch's back, as an in-place op does."""
-    for t in tensors:
-        if not t.is_inference():
-            torch.autograd.graph.increment_version(t)
+    """Move the version counters of tensors written behind torch's back, as an in-place op does (tensors
+    of inference_mode have none and are passed over)."""
+    torch.autograd.graph.increment_version(tensors)
 
 
 @functools.lru_cache(maxsize=256)
