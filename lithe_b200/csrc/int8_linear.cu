@@ -1222,9 +1222,14 @@ int32_t launch_linear(const Params& p, bool after_quantize, cudaStream_t st) {
     if (!p.q) return launch_rows<kF16, 1, true>(p, sms, false, st);
     if (p.rows <= 8) return launch_rows<kF16, 1, false>(p, sms, after_quantize, st);
     if (p.rows <= 16) return launch_rows<kF16, 2, false>(p, sms, after_quantize, st);
-    // Pairs once their 256 x 256 tiles fill the GPU; 128 x 128 tiles before, to use more SMs.
+    // A stage takes both kernels equally long, so pairs where their 256 x 256 tiles take fewer passes over the
+    // GPU (us, pairs and 128 x 128 tiles: 1024 x 12288 -> 3072, one pass and two, 44 and 68; 1024 x 3072 -> 3072
+    // 16.9 and 22.5; 600 x 1000 -> 4000 11.1 and 13.2), and the smaller tiles, whose epilogue is shorter and
+    // which use more SMs, where they take as many (512 x 3072 -> 3072 15.4 and 14.3; 1237 x 1898 -> 1091 18.4
+    // and 15.9).
     const int64_t pair_tiles = static_cast<int64_t>((p.rows + 255) / 256) * ((p.n + 255) / 256);
-    const bool pair = pair_tiles >= sms / 2;
+    const int64_t tiles = static_cast<int64_t>((p.rows + 127) / 128) * ((p.n + 127) / 128);
+    const bool pair = (pair_tiles + sms / 2 - 1) / (sms / 2) < (tiles + sms - 1) / sms;
     if constexpr (!kF16) {
         if (p.h && pair && p.rows_per_sample % 256 == 0 && factor_rows_fit(p))
             return launch_tiles<true, kF16, kExpandTmem>(p, device, sms, after_quantize, st);
