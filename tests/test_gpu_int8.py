@@ -280,3 +280,22 @@ def test_rows_from_any_element_on(k):
     if k % 2:
         got = quantize_rows(many)
         assert torch.equal(got.q.double(), want.repeat(500, 1))
+
+
+@pytest.mark.parametrize("samples,rps,n,k", [(8, 256, 1290, 200), (10, 100, 3000, 136), (1, 1000, 3001, 4096), (3, 768, 1160, 64)])
+def test_one_pass_of_pairs(samples, rps, n, k):
+    """Pair tiles that fill less than the GPU, chosen since the smaller tiles would take two passes."""
+    for dtype in (torch.bfloat16, torch.float16):
+        x = make((samples, rps, k), dtype, 1)
+        w, ws = quantize_weight(make((n, k), dtype, 2, 0.02))
+        bias = make((n,), dtype, 3)
+        check(int8_linear(x, w, ws, bias), *exact_linear(x, w, ws, bias))
+        space = torch.full((samples * rps * n + 512,), 7.0, dtype=dtype, device=DEV)
+        out = space[:samples * rps * n].view(samples * rps, n)
+        rows = quantize_rows(x)
+        _launch.int8_linear_(rows.q, rows.scale, w, ws, bias, out)
+        assert torch.equal(out.view(samples, rps, n), int8_linear(x, w, ws, bias))
+        assert bool((space[samples * rps * n:] == 7.0).all())
+        if dtype == torch.bfloat16:
+            h, b_dec = make((samples * rps, 16), dtype, 4), make((samples, n, 16), dtype, 5, 0.1)
+            check(int8_linear(x, w, ws, bias, h=h, b_dec=b_dec), *exact_linear(x, w, ws, bias, h, b_dec))
