@@ -33,7 +33,10 @@ namespace ra {
 
 constexpr int kMaxPairs = LITHE_MAX_HEAD_DIM / 2;
 constexpr int kMostHeads = 1 << 30;            // the heads' arithmetic stays inside 32 bits
-constexpr int kBatch = 4;          // heads a lane group loads before it uses the first
+// heads a lane group loads before it uses the first: 64 bytes a lane (four heads of fp32 spill: 2767 x 4 tokens
+// of 4 heads of 64, norm and rotation, 11.4 us, 8.4 us with two)
+template <typename T, bool kVec>
+constexpr int kBatch = sizeof(T) == 4 || !kVec ? 2 : 4;
 constexpr int kMinBlocks = 4;      // CTAs that have to fit an SM (64 registers a thread)
 constexpr int kWarps = 8;          // warps of a CTA
 
@@ -167,9 +170,17 @@ __device__ __forceinline__ int second_of(const Params& p, int pair) {
 }
 
 // kVec: the lane's values come as whole 16-byte (interleaved) or 8- / 16-byte (halves) pieces, at first
-// and (halves) second; else one by one, for strides, bases or slices that are not aligned to them.
-template <typename T, bool kHalves, bool kVec>
-__device__ __forceinline__ void load8(const Params& p, const T* head, int pair0, int first, int second, Eight<T>& e) {
+// and (halves) second, and its pairs are neighbours; else one by one, for strides, bases or slices that are
+// not aligned to them, and its pairs are as many apart as lanes share the head, so that the lanes' values
+// are neighbours (5 x 5295 tokens of 32 heads of 32 in fp32, halves of 9: 62 us; 281 us with neighbouring
+// pairs and 32 lanes to every head).
+template <bool kVec, int kGroup>
+__device__ __forceinline__ int pair_of(int lane, int i) {
+    return kVec ? 4 * lane + i : lane + kGroup * i;
+}
+
+template <typename T, bool kHalves, bool kVec, int kGroup>
+__device__ __forceinline__ void load8(const Params& p, const T* head, int lane, int first, int second, Eight<T>& e) {
     if constexpr (kVec && !kHalves) {
         const uint4* s = reinterpret_cast<const uint4*>(head + first);
         uint4* d = reinterpret_cast<uint4*>(&e);
@@ -182,15 +193,16 @@ __device__ __forceinline__ void load8(const Params& p, const T* head, int pair0,
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const bool in = pair0 + i < (p.dim >> 1);
-            e.v[kHalves ? i : 2 * i] = in ? head[first_of<kHalves>(p, pair0 + i)] : Elem<T>::zero();
-            e.v[kHalves ? 4 + i : 2 * i + 1] = in ? head[second_of<kHalves>(p, pair0 + i)] : Elem<T>::zero();
+            const int pair = pair_of<kVec, kGroup>(lane, i);
+            const bool in = pair < (p.dim >> 1);
+            e.v[kHalves ? i : 2 * i] = in ? head[first_of<kHalves>(p, pair)] : Elem<T>::zero();
+            e.v[kHalves ? 4 + i : 2 * i + 1] = in ? head[second_of<kHalves>(p, pair)] : Elem<T>::zero();
         }
     }
 }
 
-template <typename T, bool kHalves, bool kVec>
-__device__ __forceinline__ void store8(const Params& p, T* head, int pair0, int first, int second, const Eight<T>& e) {
+template <typename T, bool kHalves, bool kVec, int kGroup>
+__device__ __forceinline__ void store8(const Params& p, T* head, int lane, int first, int second, const Eight<T>& e) {
     if constexpr (kVec && !kHalves) {
         uint4* d = reinterpret_cast<uint4*>(head + first);
         const uint4* s = reinterpret_cast<const uint4*>(&e);
@@ -203,9 +215,10 @@ __device__ __forceinline__ void store8(const Params& p, T* head, int pair0, int 
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (pair0 + i < (p.dim >> 1)) {
-                head[first_of<kHalves>(p, pair0 + i)] = e.v[kHalves ? i : 2 * i];
-                head[second_of<kHalves>(p, pair0 + i)] = e.v[kHalves ? 4 + i : 2 * i + 1];
+            const int pair = pair_of<kVec, kGroup>(lane, i);
+            if (pair < (p.dim >> 1)) {
+                head[first_of<kHalves>(p, pair)] = e.v[kHalves ? i : 2 * i];
+                head[second_of<kHalves>(p, pair)] = e.v[kHalves ? 4 + i : 2 * i + 1];
             }
         }
     }
@@ -221,24 +234,31 @@ __device__ __forceinline__ double position_of(const Params& p, int64_t at) {
 // the norm the weights of its two values, whose products are taken once per token.
 struct Turn {
     F2 aa[2], ab[2], bb[2], ba[2];             // (ab negated)
+    uint32_t stay;                             // bit i: no axis turns the lane's pair i
 };
+
+// With whole pieces of halves a lane's pairs all stay or all turn (R / 2 is a multiple of 4).
+template <bool kHalves, bool kVec>
+__device__ __forceinline__ bool stays(uint32_t stay, int i) {
+    return kHalves && kVec ? (stay & 1) != 0 : (stay >> i & 1) != 0;
+}
 
 // A lane's part of the heads that a warp has loaded: kBatch heads, 32 / kGroup apart, from the lane's own on.
 // live: how many heads there are from it on (none for a lane without pairs); the others load zeros and store
 // nothing, but take part in the norm's shuffles.
-template <typename T>
+template <typename T, bool kVec>
 struct Batch {
-    Eight<T> e[kBatch];
+    Eight<T> e[kBatch<T, kVec>];
 };
 
 template <typename T, bool kHalves, bool kVec, int kGroup>
-__device__ __forceinline__ void load_batch(const Params& p, const T* in, int64_t step, int pair0, int first, int second,
-                                           int live, Batch<T>& b) {
+__device__ __forceinline__ void load_batch(const Params& p, const T* in, int64_t step, int lane, int first, int second,
+                                           int live, Batch<T, kVec>& b) {
     const int per_iter = 32 / kGroup;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
+    for (int j = 0; j < kBatch<T, kVec>; ++j) {
         if (j * per_iter < live)
-            load8<T, kHalves, kVec>(p, in + j * step, pair0, first, second, b.e[j]);
+            load8<T, kHalves, kVec, kGroup>(p, in + j * step, lane, first, second, b.e[j]);
         else
 #pragma unroll
             for (int i = 0; i < 8; ++i) b.e[j].v[i] = Elem<T>::zero();
@@ -247,11 +267,11 @@ __device__ __forceinline__ void load_batch(const Params& p, const T* in, int64_t
 
 // kWhole: every value of a head is turned; else the values that stay never meet an angle.
 template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole, int kGroup>
-__device__ __forceinline__ void turn_batch(const Params& p, T* out, int64_t step, int pair0, int first, int second,
-                                           int live, const Turn& m, Batch<T>& b) {
+__device__ __forceinline__ void turn_batch(const Params& p, T* out, int64_t step, int lane, int first, int second,
+                                           int live, const Turn& m, Batch<T, kVec>& b) {
     const int per_iter = 32 / kGroup;
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j) {
+    for (int j = 0; j < kBatch<T, kVec>; ++j) {
         F2 x[2], y[2];
         unpack<T, kHalves>(b.e[j], x, y);
         float r = 1.0f;
@@ -270,39 +290,39 @@ __device__ __forceinline__ void turn_batch(const Params& p, T* out, int64_t step
             r = rsqrtf(mean);
         }
         const F2 rr(r, r);
-        F2 u[2], v[2];
+        F2 u[2], v[2], xc[2] = {x[0], x[1]}, yc[2] = {y[0], y[1]};
+        if constexpr (!kWhole) {
+            // pairs that stay: their values do not meet (a product with a zero sine would carry a NaN or an
+            // infinity across)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            u[i] = fma2(x[i], m.aa[i], mul2(y[i], m.ab[i]));
-            v[i] = fma2(y[i], m.bb[i], mul2(x[i], m.ba[i]));
-            if constexpr (kNorm) u[i] = mul2(u[i], rr), v[i] = mul2(v[i], rr);
-        }
-        if constexpr (kWhole) {
-            pack<T, kHalves>(u, v, b.e[j]);
-        } else {
-            // values that stay: not met by an angle (a product with a zero sine would carry a NaN or an
-            // infinity across), and without the norm not touched at all
-            Eight<T> turned = b.e[j];
-            float xs[4], ys[4], us[4], vs[4];
-            x[0].split(xs[0], xs[1]), x[1].split(xs[2], xs[3]), y[0].split(ys[0], ys[1]), y[1].split(ys[2], ys[3]);
-            u[0].split(us[0], us[1]), u[1].split(us[2], us[3]), v[0].split(vs[0], vs[1]), v[1].split(vs[2], vs[3]);
-            float wa[4], wb[4];
-            m.aa[0].split(wa[0], wa[1]), m.aa[1].split(wa[2], wa[3]);
-            m.bb[0].split(wb[0], wb[1]), m.bb[1].split(wb[2], wb[3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (pair0 + i >= (p.rotated >> 1)) us[i] = xs[i] * wa[i] * r, vs[i] = ys[i] * wb[i] * r;
-            u[0] = F2(us[0], us[1]), u[1] = F2(us[2], us[3]), v[0] = F2(vs[0], vs[1]), v[1] = F2(vs[2], vs[3]);
-            pack<T, kHalves>(u, v, turned);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (!kNorm && pair0 + i >= (p.rotated >> 1)) continue;
-                constexpr int kA = kHalves ? 1 : 2, kB = kHalves ? 4 : 1;
-                b.e[j].v[kA * i] = turned.v[kA * i];
-                b.e[j].v[kA * i + kB] = turned.v[kA * i + kB];
+            for (int i = 0; i < 2; ++i) {
+                float a0, a1, b0, b1;
+                xc[i].split(a0, a1), yc[i].split(b0, b1);
+                const bool s0 = stays<kHalves, kVec>(m.stay, 2 * i), s1 = stays<kHalves, kVec>(m.stay, 2 * i + 1);
+                xc[i] = F2(s0 ? 0.0f : a0, s1 ? 0.0f : a1), yc[i] = F2(s0 ? 0.0f : b0, s1 ? 0.0f : b1);
             }
         }
-        if (j * per_iter < live) store8<T, kHalves, kVec>(p, out + j * step, pair0, first, second, b.e[j]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            u[i] = fma2(x[i], m.aa[i], mul2(yc[i], m.ab[i]));
+            v[i] = fma2(y[i], m.bb[i], mul2(xc[i], m.ba[i]));
+            if constexpr (kNorm) u[i] = mul2(u[i], rr), v[i] = mul2(v[i], rr);
+        }
+        if constexpr (kWhole || kNorm) {
+            pack<T, kHalves>(u, v, b.e[j]);
+        } else {
+            // (without the norm not touched at all)
+            Eight<T> turned;
+            pack<T, kHalves>(u, v, turned);
+            constexpr int kA = kHalves ? 1 : 2, kB = kHalves ? 4 : 1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (!stays<kHalves, kVec>(m.stay, i)) {
+                    b.e[j].v[kA * i] = turned.v[kA * i];
+                    b.e[j].v[kA * i + kB] = turned.v[kA * i + kB];
+                }
+        }
+        if (j * per_iter < live) store8<T, kHalves, kVec, kGroup>(p, out + j * step, lane, first, second, b.e[j]);
     }
 }
 
@@ -340,8 +360,8 @@ __device__ __forceinline__ void fill_tables(const Params& p, Tables& tab) {
 
 template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole, int kGroup>
 __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const __grid_constant__ Params p) {
-    const int lane = threadIdx.x & 31;
-    const int pair0 = 4 * (lane & (kGroup - 1)), sub = lane / kGroup;
+    const int lane = threadIdx.x & 31, part = lane & (kGroup - 1), sub = lane / kGroup;
+    const int pair0 = pair_of<kVec, kGroup>(part, 0);
     const bool has_pairs = pair0 < (p.dim >> 1);
     const int first = has_pairs ? first_of<kHalves>(p, pair0) : 0, second = has_pairs ? second_of<kHalves>(p, pair0) : 0;
     const int per_iter = 32 / kGroup;
@@ -353,14 +373,14 @@ __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const _
         const int64_t row = u / p.chunks;
         const int chunk = static_cast<int>(u - row * p.chunks);
         const int64_t sample = row / p.tokens, token = row - sample * p.tokens;
-        Batch<T> b;
+        Batch<T, kVec> b;
         int h = chunk * p.t[0].per_unit;
         {
             const Heads& t = p.t[0];
             const int live = has_pairs ? min(h + t.per_unit, t.heads) - h - sub : 0;
             load_batch<T, kHalves, kVec, kGroup>(
                 p, static_cast<const T*>(t.in) + sample * t.in_sample + token * t.in_token + (h + sub) * t.in_head,
-                per_iter * t.in_head, pair0, first, second, live, b);
+                per_iter * t.in_head, part, first, second, live, b);
         }
         // revolutions in fp64, their fraction (at most half a turn) in fp32; each pair's by one lane
         __syncwarp();
@@ -374,16 +394,32 @@ __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const _
             angle[pair] = a;
         }
         __syncwarp();
-        const float4 a01 = *reinterpret_cast<const float4*>(&angle[pair0]), a23 = *reinterpret_cast<const float4*>(&angle[pair0 + 2]);
-        const float cs[4] = {a01.x, a01.z, a23.x, a23.z}, sn[4] = {a01.y, a01.w, a23.y, a23.w};
+        float cs[4], sn[4];
+        if constexpr (kVec) {
+            const float4 a01 = *reinterpret_cast<const float4*>(&angle[pair0]);
+            const float4 a23 = *reinterpret_cast<const float4*>(&angle[pair0 + 2]);
+            cs[0] = a01.x, cs[1] = a01.z, cs[2] = a23.x, cs[3] = a23.z;
+            sn[0] = a01.y, sn[1] = a01.w, sn[2] = a23.y, sn[3] = a23.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cs[i] = angle[pair_of<kVec, kGroup>(part, i)].x, sn[i] = angle[pair_of<kVec, kGroup>(part, i)].y;
+        }
+        uint32_t stay = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) stay |= (pair_of<kVec, kGroup>(part, i) >= (p.rotated >> 1) ? 1u : 0u) << i;
 #pragma unroll 1
         for (int k = 0; k < p.tensors; ++k) {
             const Heads& t = p.t[k];
             Turn m;
+            m.stay = stay;
             float w[2][4] = {{1.0f, 1.0f, 1.0f, 1.0f}, {1.0f, 1.0f, 1.0f, 1.0f}};
-            if constexpr (kNorm) {
+            if constexpr (kNorm && kVec) {
                 *reinterpret_cast<float4*>(w[0]) = *reinterpret_cast<const float4*>(&tab.weight[k][0][pair0]);
                 *reinterpret_cast<float4*>(w[1]) = *reinterpret_cast<const float4*>(&tab.weight[k][1][pair0]);
+            } else if constexpr (kNorm) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[0][i] = tab.weight[k][0][pair_of<kVec, kGroup>(part, i)], w[1][i] = tab.weight[k][1][pair_of<kVec, kGroup>(part, i)];
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -395,13 +431,13 @@ __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const _
             const int end = min(h + t.per_unit, t.heads);
             const T* in = static_cast<const T*>(t.in) + sample * t.in_sample + token * t.in_token + (h + sub) * t.in_head;
             T* out = static_cast<T*>(t.out) + sample * t.out_sample + token * t.out_token + (h + sub) * t.out_head;
-            for (; h < end; h += per_iter * kBatch) {
+            for (; h < end; h += per_iter * kBatch<T, kVec>) {
                 const int live = has_pairs ? end - h - sub : 0;
                 if (k > 0 || h > chunk * t.per_unit)
-                    load_batch<T, kHalves, kVec, kGroup>(p, in, per_iter * t.in_head, pair0, first, second, live, b);
-                turn_batch<T, kHalves, kVec, kNorm, kWhole, kGroup>(p, out, per_iter * t.out_head, pair0, first, second, live, m, b);
-                in += kBatch * per_iter * t.in_head;
-                out += kBatch * per_iter * t.out_head;
+                    load_batch<T, kHalves, kVec, kGroup>(p, in, per_iter * t.in_head, part, first, second, live, b);
+                turn_batch<T, kHalves, kVec, kNorm, kWhole, kGroup>(p, out, per_iter * t.out_head, part, first, second, live, m, b);
+                in += kBatch<T, kVec> * per_iter * t.in_head;
+                out += kBatch<T, kVec> * per_iter * t.out_head;
             }
         }
     }
@@ -421,18 +457,18 @@ int32_t launch(const Params& p, int sms, cudaStream_t st) {
 
 // The lanes of a head are a compile-time number: 8, 16 or 32 (with the norm 252 us for 14 x 4096 tokens against
 // 276 us with a run-time one, both at the power cap).
-template <typename T, bool kHalves, bool kNorm, bool kWhole>
+template <typename T, bool kHalves, bool kVec, bool kNorm, bool kWhole>
 int32_t launch_group(const Params& p, int sms, cudaStream_t st) {
-    if (p.group == 8) return launch<T, kHalves, true, kNorm, kWhole, 8>(p, sms, st);
-    if (p.group == 16) return launch<T, kHalves, true, kNorm, kWhole, 16>(p, sms, st);
-    return launch<T, kHalves, true, kNorm, kWhole, 32>(p, sms, st);
+    if (p.group == 8) return launch<T, kHalves, kVec, kNorm, kWhole, 8>(p, sms, st);
+    if (p.group == 16) return launch<T, kHalves, kVec, kNorm, kWhole, 16>(p, sms, st);
+    return launch<T, kHalves, kVec, kNorm, kWhole, 32>(p, sms, st);
 }
 
 template <typename T, bool kNorm, bool kHalves>
 int32_t launch_vec(const Params& p, bool vec, int sms, cudaStream_t st) {
-    if (!vec) return launch<T, kHalves, false, kNorm, false, 32>(p, sms, st);
-    return p.rotated == p.dim ? launch_group<T, kHalves, kNorm, true>(p, sms, st)
-                              : launch_group<T, kHalves, kNorm, false>(p, sms, st);
+    if (!vec) return launch_group<T, kHalves, false, kNorm, false>(p, sms, st);
+    return p.rotated == p.dim ? launch_group<T, kHalves, true, kNorm, true>(p, sms, st)
+                              : launch_group<T, kHalves, true, kNorm, false>(p, sms, st);
 }
 
 template <typename T, bool kNorm>
@@ -534,7 +570,7 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
     // A token's heads are split over warps while that leaves the SMs room: more units than resident
     // warps pay their angles for nothing (1024 tokens of 24 heads: 5.9 us on 4 chunks, 13 us on 8).
     // Lanes that share a head: 4 pairs each, a power of two for the norm's shuffles.
-    p.group = !vec || dim > 128 ? 32 : dim > 64 ? 16 : 8;
+    p.group = dim > 128 ? 32 : dim > 64 ? 16 : 8;
     const int per_iter = 32 / p.group;
     const int most_chunks = (most_heads + per_iter - 1) / per_iter;
     const int64_t rows = static_cast<int64_t>(batch) * tokens;
