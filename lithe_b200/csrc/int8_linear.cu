@@ -32,7 +32,8 @@ constexpr int kMostRows = 0x7fffffff - 1024;   // rows and channels of whole til
 // there are many rows (57344 x 3072: 80 us, 6.6 TB/s; four a row 102 us), four where there are few and
 // their latency counts (one row 1.8 us; 3.0 us).  A longer row is read twice, the second time from L2
 // (20000 x 18432: 216 us, 5.1 TB/s).  Rows that do not start on 16-byte boundaries are put together out of
-// aligned pieces (20000 x 1001: 18 us, value by value 29 us; 1237 x 1898: 3.8 and 6.1 us).
+// aligned pieces (15488 x 5591: 77 us, 102 us with both granules of a piece loaded by its lane; 20000 x 1001:
+// 18 us, value by value 29 us; 1237 x 1898: 4.0 and 6.1 us).
 // The quotients of a piece are checked for nearness to halfway together, with a bound (2^-13) above every
 // 2^-21 |t|; the few pieces it stops are done value by value.
 // ------------------------------------------------------------------------------------------
@@ -102,53 +103,86 @@ __device__ __forceinline__ uint2 quantize8(const uint4& v, float pre, float r) {
     return make_uint2(__byte_perm(a0, a1, 0x5410), __byte_perm(a2, a3, 0x5410));
 }
 
-// A lane's kPieces pieces of a row of k values, the first one's number at0 and the rest kLanes apart: piece
-// `at` is the values 8 at to 8 at + 7, zeros from k on.  kWhole: rows are whole pieces on 16-byte
-// boundaries.  Else a piece is shifted together out of the two 16-byte granules it lies in, all of them
-// loaded before the first is used; those that reach beyond the row are read value by value then.
-template <bool kWhole, int kLanes, int kPieces>
-__device__ __forceinline__ void load_pieces(const uint16_t* row, int at0, int k, uint4 (&v)[kPieces]) {
-    if constexpr (kWhole) {
+__device__ __forceinline__ uint32_t max_of(uint32_t m, const uint4& v) {
+    return __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)),
+                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+}
+
+// A lane's kPieces pieces of a row of k values, piece `at` being the values 8 at to 8 at + 7, zeros from k on.
+// kWhole: rows are whole pieces on 16-byte boundaries.  Else a piece is shifted together out of two of the
+// 16-byte granules that the row lies in, one the lane's own and one its neighbour's: a warp holds 32 kPieces
+// granules in a row and the one behind them (lane 31).  The granules that reach beyond the row are read value
+// by value, after the others have been loaded.
+template <bool kWhole, int kPieces>
+struct Pieces {
+    uint4 g[kPieces];
+    uint4 behind;
+    int shift;
+
+    // The lane's piece c: row pieces `first` on, kLanes lanes side by side.
+    template <int kLanes>
+    static __device__ __forceinline__ int at(int first, int c) {
+        if constexpr (kWhole) return first + c * kLanes + static_cast<int>(threadIdx.x) % kLanes;
+        const int t = static_cast<int>(threadIdx.x) % kLanes;
+        return first + (t / 32 * kPieces + c) * 32 + t % 32;
+    }
+
+    static __device__ __forceinline__ uint4 edge(const uint16_t* row, int value, int k) {
+        uint32_t x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = value + i >= 0 && value + i < k ? __ldg(row + value + i) : 0u;
+        return make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
+    }
+
+    template <int kLanes>
+    __device__ __forceinline__ void load(const uint16_t* row, int first, int k) {
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+        shift = kWhole ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 7;
 #pragma unroll
         for (int c = 0; c < kPieces; ++c) {
-            const int at = c * kLanes + at0;
-            v[c] = 8 * at < k ? __ldg(reinterpret_cast<const uint4*>(row) + at) : make_uint4(0, 0, 0, 0);
+            const int value = 8 * at<kLanes>(first, c) - shift;
+            g[c] = value >= 0 && value + 8 <= k ? __ldg(reinterpret_cast<const uint4*>(row + value)) : zero;
         }
-    } else {
-        const int shift = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 7;
-        uint4 g[kPieces][2];
+        if constexpr (!kWhole) {
+            const int next = 8 * (at<kLanes>(first, kPieces - 1) + 1) - shift;
+            const bool last = (threadIdx.x & 31) == 31;
+            behind = last && next >= 0 && next + 8 <= k ? __ldg(reinterpret_cast<const uint4*>(row + next)) : zero;
 #pragma unroll
-        for (int c = 0; c < kPieces; ++c)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int first = 8 * (c * kLanes + at0 + e) - shift;          // the granule's first value
-                g[c][e] = first >= 0 && first + 8 <= k ? __ldg(reinterpret_cast<const uint4*>(row + first))
-                                                       : make_uint4(0, 0, 0, 0);
+            for (int c = 0; c < kPieces; ++c) {
+                const int value = 8 * at<kLanes>(first, c) - shift;
+                if (value < k && (value < 0 || value + 8 > k)) g[c] = edge(row, value, k);
             }
-#pragma unroll
-        for (int c = 0; c < kPieces; ++c) {
-            uint32_t w[8];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int first = 8 * (c * kLanes + at0 + e) - shift;
-                if (first < k && (first < 0 || first + 8 > k)) {
-                    uint32_t x[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = first + i >= 0 && first + i < k ? __ldg(row + first + i) : 0u;
-                    g[c][e] = make_uint4(x[0] | x[1] << 16, x[2] | x[3] << 16, x[4] | x[5] << 16, x[6] | x[7] << 16);
-                }
-                w[4 * e] = g[c][e].x, w[4 * e + 1] = g[c][e].y, w[4 * e + 2] = g[c][e].z, w[4 * e + 3] = g[c][e].w;
-            }
-#pragma unroll
-            for (int i = 0; i < 6; ++i) w[i] = shift & 4 ? w[i + 2] : w[i];
-#pragma unroll
-            for (int i = 0; i < 5; ++i) w[i] = shift & 2 ? w[i + 1] : w[i];
-            const int half = 16 * (shift & 1);
-            v[c] = make_uint4(__funnelshift_r(w[0], w[1], half), __funnelshift_r(w[1], w[2], half),
-                              __funnelshift_r(w[2], w[3], half), __funnelshift_r(w[3], w[4], half));
+            if (last && next < k && next + 8 > k) behind = edge(row, next, k);
         }
     }
-}
+
+    __device__ __forceinline__ uint32_t most(uint32_t m) const {
+#pragma unroll
+        for (int c = 0; c < kPieces; ++c) m = max_of(m, g[c]);
+        return kWhole ? m : max_of(m, behind);
+    }
+
+    // The lane's piece c, in the order of c; every lane of the warp takes part.
+    __device__ __forceinline__ uint4 piece(int c) {
+        if constexpr (kWhole) return g[c];
+        const int lane = threadIdx.x & 31;
+        // lane 31's neighbour is lane 0's next granule, and behind the last the one that lane 31 holds
+        const uint4 wrap = c + 1 < kPieces ? g[c + 1 < kPieces ? c + 1 : 0] : behind;
+        const bool hand_on = c + 1 < kPieces && lane == 0;
+        uint32_t w[8] = {g[c].x, g[c].y, g[c].z, g[c].w, hand_on ? wrap.x : g[c].x, hand_on ? wrap.y : g[c].y,
+                         hand_on ? wrap.z : g[c].z, hand_on ? wrap.w : g[c].w};
+#pragma unroll
+        for (int i = 4; i < 8; ++i) w[i] = __shfl_sync(0xffffffffu, w[i], (lane + 1) & 31);
+        if (c + 1 == kPieces && lane == 31) w[4] = behind.x, w[5] = behind.y, w[6] = behind.z, w[7] = behind.w;
+#pragma unroll
+        for (int i = 0; i < 6; ++i) w[i] = shift & 4 ? w[i + 2] : w[i];
+#pragma unroll
+        for (int i = 0; i < 5; ++i) w[i] = shift & 2 ? w[i + 1] : w[i];
+        const int half = 16 * (shift & 1);
+        return make_uint4(__funnelshift_r(w[0], w[1], half), __funnelshift_r(w[1], w[2], half),
+                          __funnelshift_r(w[2], w[3], half), __funnelshift_r(w[3], w[4], half));
+    }
+};
 
 // Its bytes to q's row (which starts on a 16-byte boundary); those from k on are left as they are.
 template <bool kWhole>
@@ -161,26 +195,18 @@ __device__ __forceinline__ void store_piece(int8_t* row, int at, int k, const ui
     }
 }
 
-__device__ __forceinline__ uint32_t max_of(uint32_t m, const uint4& v) {
-    return __vmaxu2(__vmaxu2(m, __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu)),
-                    __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
-}
-
 template <bool kF16, bool kWhole, int kWarps, int kPieces>
 __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     constexpr int kLanes = 32 * kWarps, kRowsCta = kThreadsQ / kLanes;
     __shared__ uint32_t part[kThreadsQ / 32];
-    const int warp = threadIdx.x >> 5, at0 = threadIdx.x % kLanes;
+    const int warp = threadIdx.x >> 5;
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kRowsCta + threadIdx.x / kLanes;
     const bool live = row < p.rows;
-    const uint16_t* x = p.x + row * p.x_stride;
-    const int pieces = live ? (p.k + 7) >> 3 : 0;
-    uint4 v[kPieces];
-    load_pieces<kWhole, kLanes>(x, at0, live ? p.k : 0, v);
-    uint32_t m = 0;
-#pragma unroll
-    for (int c = 0; c < kPieces; ++c) m = max_of(m, v[c]);
+    const int k = live ? p.k : 0, pieces = (k + 7) >> 3;
+    Pieces<kWhole, kPieces> v;
+    v.template load<kLanes>(p.x + row * p.x_stride, 0, k);
+    uint32_t m = v.most(0);
     m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
     if constexpr (kWarps > 1) {
         if ((threadIdx.x & 31) == 0) part[warp] = m;
@@ -188,15 +214,16 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_kernel(const QuantParams p
 #pragma unroll
         for (int i = 0; i < kWarps; ++i) m = max(m, part[warp / kWarps * kWarps + i]);
     }
-    if (!live) return;
+    if (!live) return;                         // (whole warps: they share a row)
     float pre, r;
-    row_factors<kF16>(m, at0 == 0, p.scale + row, pre, r);
+    row_factors<kF16>(m, threadIdx.x % kLanes == 0, p.scale + row, pre, r);
     int8_t* q = p.q + row * p.q_stride;
 #pragma unroll
     for (int c = 0; c < kPieces; ++c) {
-        const int at = c * kLanes + at0;
+        const int at = v.template at<kLanes>(0, c);
+        const uint4 x = v.piece(c);
         if (at < pieces)
-            store_piece<kWhole>(q, at, p.k, pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r));
+            store_piece<kWhole>(q, at, p.k, pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(x, pre, r));
     }
 }
 
@@ -236,11 +263,11 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_long_kernel(const QuantPar
     constexpr int kPieces = 4;
     const int pieces = (p.k + 7) >> 3;
     uint32_t m = 0;
-    uint4 v[kPieces];
-    for (int at = threadIdx.x; at < pieces; at += kPieces * kThreadsQ) {
-        load_pieces<kWhole, kThreadsQ>(x, at, p.k, v);
-#pragma unroll
-        for (int c = 0; c < kPieces; ++c) m = max_of(m, v[c]);
+    Pieces<kWhole, kPieces> v;
+    // (every warp goes round as often: the pieces are put together across its lanes)
+    for (int first = 0; first < pieces; first += kPieces * kThreadsQ) {
+        v.template load<kThreadsQ>(x, first, p.k);
+        m = v.most(m);
     }
     m = __reduce_max_sync(0xffffffffu, max(m & 0xffffu, m >> 16));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
@@ -249,13 +276,15 @@ __global__ void __launch_bounds__(kThreadsQ) quantize_long_kernel(const QuantPar
     for (int i = 0; i < kThreadsQ / 32; ++i) m = max(m, part[i]);
     float pre, r;
     row_factors<kF16>(m, threadIdx.x == 0, p.scale + row, pre, r);
-    for (int at = threadIdx.x; at < pieces; at += kPieces * kThreadsQ) {
-        load_pieces<kWhole, kThreadsQ>(x, at, p.k, v);
+    for (int first = 0; first < pieces; first += kPieces * kThreadsQ) {
+        v.template load<kThreadsQ>(x, first, p.k);
 #pragma unroll
-        for (int c = 0; c < kPieces; ++c)
-            if (at + c * kThreadsQ < pieces)
-                store_piece<kWhole>(q, at + c * kThreadsQ, p.k,
-                                    pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(v[c], pre, r));
+        for (int c = 0; c < kPieces; ++c) {
+            const int at = v.template at<kThreadsQ>(first, c);
+            const uint4 piece = v.piece(c);
+            if (at < pieces)
+                store_piece<kWhole>(q, at, p.k, pre == 0.0f ? make_uint2(0, 0) : quantize8<kF16>(piece, pre, r));
+        }
     }
 }
 
