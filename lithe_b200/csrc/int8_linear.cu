@@ -801,24 +801,37 @@ __device__ __forceinline__ void add_expand(const Params& p, int n0, int c0, int 
         }
         return;
     }
+    // sample s's factors of channel block j
+    const auto factors_of = [&](int s, int j) {
+        if (s == staged) return factors[(c0 + 8 * j + g) * 4 + q];
+        const int n = min(n0 + c0 + 8 * j + g, p.n - 1);
+        return __ldg(reinterpret_cast<const uint2*>(p.b_dec + (static_cast<int64_t>(s) * p.n + n) * kRank) + q);
+    };
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        // the samples of the 16 rows, one after the other
         const int first = __shfl_sync(0xffffffffu, rows.sample[2 * half], 0);
         const int last = __shfl_sync(0xffffffffu, rows.sample[2 * half + 1], 31);
+        const uint32_t a[4] = {rows.h[2 * half].x, rows.h[2 * half + 1].x, rows.h[2 * half].y, rows.h[2 * half + 1].y};
+        if (first == last) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint2 b = factors_of(first, j);
+                mma_bf16_16816(y[half][j], a, b.x, b.y, y[half][j]);
+            }
+            continue;
+        }
+        // the samples of the 16 rows, one after the other; a row takes the sum with its own sample's factors
+        // (zeros in place of the other rows' h would not do: times a factor that is not finite they are NaN)
 #pragma unroll 1
         for (int s = first; s <= last; ++s) {
             const bool lo = rows.sample[2 * half] == s, hi = rows.sample[2 * half + 1] == s;
-            const uint32_t a[4] = {lo ? rows.h[2 * half].x : 0u, hi ? rows.h[2 * half + 1].x : 0u,
-                                   lo ? rows.h[2 * half].y : 0u, hi ? rows.h[2 * half + 1].y : 0u};
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                uint2 b = factors[(c0 + 8 * j + g) * 4 + q];
-                if (s != staged) {
-                    const int n = min(n0 + c0 + 8 * j + g, p.n - 1);
-                    b = __ldg(reinterpret_cast<const uint2*>(p.b_dec + (static_cast<int64_t>(s) * p.n + n) * kRank) + q);
-                }
-                mma_bf16_16816(y[half][j], a, b.x, b.y, y[half][j]);
+                const uint2 b = factors_of(s, j);
+                float sum[4];
+                mma_bf16_16816(sum, a, b.x, b.y, y[half][j]);
+                if (lo) y[half][j][0] = sum[0], y[half][j][1] = sum[1];
+                if (hi) y[half][j][2] = sum[2], y[half][j][3] = sum[3];
             }
         }
     }

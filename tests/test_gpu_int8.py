@@ -299,3 +299,25 @@ def test_one_pass_of_pairs(samples, rps, n, k):
         if dtype == torch.bfloat16:
             h, b_dec = make((samples * rps, 16), dtype, 4), make((samples, n, 16), dtype, 5, 0.1)
             check(int8_linear(x, w, ws, bias, h=h, b_dec=b_dec), *exact_linear(x, w, ws, bias, h, b_dec))
+
+
+@pytest.mark.parametrize("samples,rps,n,k", [(7, 2, 40, 96), (7, 5, 72, 64), (7, 37, 256, 320), (3, 100, 520, 256), (5, 20, 264, 4096),
+                                             (20, 300, 1096, 1000), (5, 1000, 2000, 136), (4, 256, 512, 128),
+                                             (5, 1280, 3000, 136)])
+def test_bad_factors_stay_with_their_sample(samples, rps, n, k):
+    """A sample's decoded factors with infinities and NaN: its own rows have them in those channels, and every
+    other value keeps its bits, on each of the kernel's paths (samples that end inside a tile among them)."""
+    bf = torch.bfloat16
+    x = make((samples, rps, k), bf, 1)
+    w, ws = quantize_weight(make((n, k), bf, 2, 0.02))
+    h, b_dec = make((samples * rps, 16), bf, 4), make((samples, n, 16), bf, 5, 0.1)
+    clean = int8_linear(x, w, ws, h=h, b_dec=b_dec)
+    for s in (0, samples // 2, samples - 1):
+        b = b_dec.clone()
+        b[s, 3, 7], b[s, 8], b[s, n - 1, 0] = INF, NAN, -INF
+        got = int8_linear(x, w, ws, h=h, b_dec=b)
+        bad = torch.zeros(samples, 1, n, dtype=torch.bool, device=DEV)
+        bad[s, 0, [3, 8, n - 1]] = True
+        bad = bad.expand_as(got)
+        assert not got[bad].isfinite().any()
+        assert torch.equal(got[~bad], clean[~bad]), s
