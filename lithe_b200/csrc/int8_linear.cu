@@ -316,11 +316,13 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes of a row at k0; bytes from k on are zeros.  kStream: read once, kept out of L1.
-template <bool kStream>
+// 16 bytes of a row at k0; bytes from k on are zeros.  kWeights: read once and kept out of L1, as memory that
+// nobody writes while the kernel runs.  The activations are read by ordinary loads: their quantisation may
+// still be writing them when the kernel starts (see grid_dependency_wait).
+template <bool kWeights>
 __device__ __forceinline__ uint4 load16(const int8_t* row, int k0, int k) {
     if (k0 + 16 <= k) {
-        if (!kStream) return __ldg(reinterpret_cast<const uint4*>(row + k0));
+        if (!kWeights) return *reinterpret_cast<const uint4*>(row + k0);
         uint4 v;
         asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
@@ -350,6 +352,8 @@ __device__ __forceinline__ float expand_of(const Params& p, int r, int n, float 
 // The linear's kernels may start while the quantisation of their activations runs (it lets them at its
 // start): they wait here before they read what it writes.  What ran before it has completed by then,
 // since it was launched in stream order.  Returns at once in a launch that depends on nothing so.
+// q and x_scale are read by ordinary loads behind it: they are written in the kernel's lifetime, which the
+// loads of __ldg (ld.global.nc) rule out and which would let the compiler move them over the wait.
 __device__ __forceinline__ void grid_dependency_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 struct Launch {
@@ -701,7 +705,7 @@ struct RowRegs {
         for (int i = 0; i < 4; ++i) {
             const int r = row0 + (lane >> 2) + 8 * i;
             const bool in = r < p.rows;
-            sx[i] = in ? __ldg(p.x_scale + r) : 0.0f;
+            sx[i] = in ? p.x_scale[r] : 0.0f;
             if constexpr (kExpand == kExpandMma) {
                 h[i] = in ? __ldg(reinterpret_cast<const uint2*>(p.h + static_cast<int64_t>(r) * kRank) + (lane & 3))
                           : make_uint2(0, 0);
@@ -880,7 +884,7 @@ __device__ __forceinline__ void finish_sums(const TileParams& tp, const uint8_t*
         const int in = e / (kSize / 8), c = 8 * (e % (kSize / 8));             // row of the tile, first column
         const int r = m0 + in, n = n0 + c;
         if (n >= p.n) continue;
-        const float sx = __ldg(p.x_scale + r);
+        const float sx = p.x_scale[r];
         uint4 a[kSplits][2];
 #pragma unroll
         for (int s = 0; s < kSplits; ++s) {

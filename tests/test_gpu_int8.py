@@ -10,7 +10,7 @@ magnitudes of what is added: c = 40.
 import pytest
 import torch
 
-from lithe_b200 import device_errors
+from lithe_b200 import _lib, device_errors
 from lithe_b200.kernels import _launch, int8_linear, quantize_rows, quantize_weight
 
 pytestmark = pytest.mark.gpu
@@ -321,3 +321,26 @@ def test_bad_factors_stay_with_their_sample(samples, rps, n, k):
         bad = bad.expand_as(got)
         assert not got[bad].isfinite().any()
         assert torch.equal(got[~bad], clean[~bad]), s
+
+
+@pytest.mark.parametrize("rows,n,k", [(2, 1091, 3072), (14, 264, 1000), (32, 256, 12288), (200, 520, 640), (3000, 1536, 512)])
+def test_one_workspace_many_calls(rows, n, k):
+    """Calls of other activations one behind the other through one workspace: each reads what its own
+    quantisation has written, not what stood there."""
+    xs = [make((rows, k), torch.bfloat16, i, 1.0 + i) for i in range(3)]
+    w, ws = quantize_weight(make((n, k), torch.bfloat16, 9, 0.02))
+    want = []
+    for x in xs:
+        q = quantize_rows(x)
+        out = torch.empty(rows, n, dtype=torch.bfloat16, device=DEV)
+        want.append(_launch.int8_linear_(q.q, q.scale, w, ws, None, out))
+    space = torch.empty(_lib.lib().lithe_int8_workspace_bytes(rows, k), dtype=torch.uint8, device=DEV)
+    got = [torch.empty_like(want[0]) for _ in range(30)]
+    for i, out in enumerate(got):
+        rc = _lib.lib().lithe_int8_linear_dynamic(
+            xs[i % 3].data_ptr(), k, w.data_ptr(), w.stride(0), ws.data_ptr(), None, out.data_ptr(), _lib.DTYPE_BF16,
+            rows, n, k, None, None, 0, 0, _launch.error_word(space.device).data_ptr(), space.data_ptr(),
+            space.numel(), torch.cuda.current_stream().cuda_stream)
+        assert rc == 0
+    assert all(torch.equal(out, want[i % 3]) for i, out in enumerate(got))
+    assert device_errors() == 0

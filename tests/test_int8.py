@@ -1,4 +1,7 @@
 """8-bit linear: what the entry points refuse, without a GPU."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
@@ -161,3 +164,14 @@ def test_ops_know_their_shapes():
         assert tuple(y.shape) == (2, 3, 3) and y.dtype == torch.float16
         y = torch.ops.lithe_b200.int8_linear(q, scale, q[:3], scale[:3], None, None, None, True)
         assert tuple(y.shape) == (6, 3) and y.dtype == torch.float16
+
+
+def test_what_the_quantisation_writes_is_read_by_ordinary_loads():
+    """The linear may start while q and the scales are being written, so it must not read them as memory
+    that is constant for its lifetime (__ldg)."""
+    source = (Path(_lib.__file__).parent / "csrc" / "int8_linear.cu").read_text()
+    body = source[source.index("struct Params {"):source.index("extern \"C\"")]         # the linear's kernels
+    constant = re.findall(r"__ldg\(((?:[^()]|\((?:[^()]|\([^()]*\))*\))*)\)", body)
+    assert constant and not [c for c in constant if re.search(r"\bx_scale\b|\bp\.q\b|\brow\b", c)], constant
+    load = body[body.index("uint4 load16("):]
+    assert "return *reinterpret_cast<const uint4*>(row + k0)" in load[:load.index("\n}\n")]
