@@ -79,6 +79,7 @@ def int8_linear(x: Union[torch.Tensor, QuantizedRows], weight: torch.Tensor, wei
     add h . b_dec[sample]^T; every sample has rows / samples consecutive rows (bfloat16 x only).
     Any number of rows, n >= 1, k up to 131072.
     """
+    _inference_only(bias, weight_scale, h, b_dec, *((x.scale,) if isinstance(x, QuantizedRows) else (x,)))
     if isinstance(x, QuantizedRows):
         n = weight.shape[0]
         if torch.compiler.is_compiling():
@@ -88,7 +89,6 @@ def int8_linear(x: Union[torch.Tensor, QuantizedRows], weight: torch.Tensor, wei
             out = torch.empty(x.q.shape[0], n, dtype=x.dtype, device=x.q.device)
             _launch.int8_linear_(x.q, x.scale, weight, weight_scale, bias, out, h, b_dec)
         return out.view(*x.shape, n)
-    _inference_only(x, bias)
     if torch.compiler.is_compiling():
         return torch.ops.lithe_b200.int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec)
     return _launch.int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec)

@@ -66,7 +66,7 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     projection).  The result is a new tensor, or ``out`` (x itself to rotate in place).
     """
     _launch._check_heads(x, "x")
-    _inference_only(x, out)
+    _inference_only(x, positions, out)
     compiling = torch.compiler.is_compiling()
     axes, theta, code = (_rotation.__wrapped__ if compiling else _rotation)(x.shape[3], tuple(axes), theta, pairing)
     fresh = out is None
@@ -101,7 +101,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     """
     _launch._check_heads(q, "q")
     _launch._check_heads(k, "k", q)
-    _inference_only(q, k, weight_q, weight_k, out_q, out_k)
+    _inference_only(q, k, weight_q, weight_k, positions, out_q, out_k)
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")

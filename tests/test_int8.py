@@ -7,7 +7,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from lithe_b200 import _lib
-from lithe_b200.kernels import _launch, int8_linear, quantize_rows, quantize_weight
+from lithe_b200.kernels import QuantizedRows, _launch, int8_linear, quantize_rows, quantize_weight
 
 
 def _linear(q=0x10000, q_stride=128, xs=0x20000, w=0x30000, w_stride=128, ws=0x40000, bias=None, out=0x50000,
@@ -175,3 +175,19 @@ def test_what_the_quantisation_writes_is_read_by_ordinary_loads():
     assert constant and not [c for c in constant if re.search(r"\bx_scale\b|\bp\.q\b|\brow\b", c)], constant
     load = body[body.index("uint4 load16("):]
     assert "return *reinterpret_cast<const uint4*>(row + k0)" in load[:load.index("\n}\n")]
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("which", ["x", "bias", "weight_scale", "h", "b_dec"])
+def test_every_operand_is_inference_only(which, quantized):
+    """No operand's gradient is lost silently: with grad mode on, one that requires a gradient is refused."""
+    bf = torch.bfloat16
+    with FakeTensorMode():
+        ops = dict(x=torch.empty(6, 32, dtype=bf, device="cuda"), weight=torch.empty(4, 32, dtype=torch.int8, device="cuda"),
+                   weight_scale=torch.empty(4, device="cuda"), bias=torch.empty(4, dtype=bf, device="cuda"),
+                   h=torch.empty(6, 16, dtype=bf, device="cuda"), b_dec=torch.empty(2, 4, 16, dtype=bf, device="cuda"))
+        if quantized:
+            ops["x"] = QuantizedRows(torch.empty(6, 32, dtype=torch.int8, device="cuda"), torch.empty(6, device="cuda"), (6,), bf)
+        (ops["x"].scale if which == "x" and quantized else ops[which]).requires_grad_()
+        with pytest.raises(RuntimeError, match="inference-only"):
+            int8_linear(**ops)

@@ -152,3 +152,17 @@ def test_ops_are_registered():
         assert torch.ops.lithe_b200.rotate_axes_(torch.empty_like(x), x, pos, [32, 32], 1e4, 0) is None
         assert torch.ops.lithe_b200.qk_norm_rotate_(torch.empty_like(x), torch.empty_like(x), x, x, None, None, pos,
                                                     [32, 32], 1e4, 1e-6, 0) is None
+
+
+@pytest.mark.parametrize("which", ["positions", "weight_q", "weight_k", "q", "k"])
+def test_every_operand_is_inference_only(which):
+    with FakeTensorMode():
+        ops = dict(q=torch.empty(2, 4, 3, 64, device="cuda"), k=torch.empty(2, 4, 3, 64, device="cuda"),
+                   weight_q=torch.empty(64, device="cuda"), weight_k=torch.empty(64, device="cuda"),
+                   positions=torch.empty(4, 2, device="cuda"))
+        ops[which].requires_grad_()
+        with pytest.raises(RuntimeError, match="inference-only"):
+            qk_norm_rotate(*ops.values(), (32, 32))
+        if which == "positions":
+            with pytest.raises(RuntimeError, match="inference-only"):
+                rotate_axes(ops["k"], ops["positions"], (32, 32))
