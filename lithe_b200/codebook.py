@@ -129,10 +129,10 @@ def level_lut(pools: torch.Tensor) -> np.ndarray:
     global _PC
     if pools.dim() != 3 or tuple(pools.shape[1:]) != (K, BLOCK_SIZE):
         raise ValueError(f"pools must be (L, {K}, {BLOCK_SIZE}), got {tuple(pools.shape)}")
-    key = id(pools)
+    key, version = id(pools), None if pools.is_inference() else pools._version     # (None: not counted, not kept)
     with _lut_lock:
         hit = _lut_cache.get(key)
-    if hit is not None and hit[0] == pools._version:
+    if hit is not None and hit[0] == version:
         return hit[1]
     if _PC is None:
         _PC = popcount_table()
@@ -143,9 +143,11 @@ def level_lut(pools: torch.Tensor) -> np.ndarray:
             lut[level, n] = host[level, (1 << n) - 1, 0]          # P(0) = 0 -> popcount(k) = n
         if not np.array_equal(lut[level][_PC].view(np.uint32), host[level].view(np.uint32)):
             raise ValueError(f"pools level {level} is not a Hadamard-9bit codebook level")
+    if version is None:
+        return lut
     with _lut_lock:
         fresh = key not in _lut_cache
-        _lut_cache[key] = (pools._version, lut)
+        _lut_cache[key] = (version, lut)
     if fresh:
         weakref.finalize(pools, _forget, key)
     return lut

@@ -23,7 +23,7 @@ from . import codebook as cb
 from . import quant
 from .fileio import LitheAdapter
 from .kernels import _launch, ops
-from .kernels.layers import FUSED_GEMM_MAX_K, _inference_only, _InputKey, _RouteKey, shared_input_sets
+from .kernels.layers import FUSED_GEMM_MAX_K, _inference_only, _InputKey, _RouteKey, _tracked, shared_input_sets
 
 Route = Sequence[Tuple[int, float]]
 
@@ -44,6 +44,7 @@ class Router:
         self._key = None
         self._serial = 0
 
+    @torch.inference_mode(False)        # (tables that count their versions, whatever the caller's mode)
     def set(self, routes: Sequence[Route]) -> None:
         routes = [list(r) for r in routes]
         width = max([1] + [len(r) for r in routes])
@@ -59,14 +60,17 @@ class Router:
         self.weights = torch.from_numpy(w_rows)
         self._serial += 1
 
+    @torch.inference_mode(False)
     def columns(self, device: torch.device, scales: Tuple[float, ...]) -> List[Tuple[torch.Tensor, torch.Tensor]]:
         """Device tables per route column: (slot ids int32 (b,), w * alpha/r float32 (b,)).
 
         Built on the host once per (routing, device, adapter scales) and shared by all layers;
-        columns without any live entry are omitted.
+        columns without any live entry are omitted.  Tables of the caller's own that were made under
+        inference_mode count no versions: the device tables are then built anew in every call.
         """
-        key = (self._serial, id(self.ids), id(self.weights), self.ids._version, self.weights._version)
-        if key != self._key:
+        key = (None if not _tracked(self.ids, self.weights) else
+               (self._serial, id(self.ids), id(self.weights), self.ids._version, self.weights._version))
+        if key is None or key != self._key:
             self._tables.clear()
             self._key = key
         tkey = (str(device), scales)
@@ -156,17 +160,17 @@ class MultiAdapterLinear(nn.Module):
         else:
             va, vb = self._view_params()
             # the B factors of this route column, decoded once while it and the banks are unchanged
-            bank_key = (self._n_added, self.idx_a._version, self.idx_b._version)
-            compiling = torch.compiler.is_compiling()
+            keep = not torch.compiler.is_compiling() and _tracked(slot_ids, self.idx_a, self.idx_b)
+            bank_key = (self._n_added, self.idx_a._version, self.idx_b._version) if keep else None
             cache = self._bdec_cache
-            if not compiling and cache is not None and cache[0].matches(slot_ids, bank_key):
+            if keep and cache is not None and cache[0].matches(slot_ids, bank_key):
                 b_dec = cache[1]
                 h = torch.ops.lithe_b200.lora_prep_h(xs, self.idx_a, self.idx_b, va, vb, self.idx_a.shape[0], slot_ids,
                                                      w, d_out, self._lut, 1.0)
             else:
                 h, b_dec = torch.ops.lithe_b200.lora_prep(xs, self.idx_a, self.idx_b, va, vb, self.idx_a.shape[0],
                                                           slot_ids, w, d_out, self._lut, 1.0, True)
-                if not compiling:
+                if keep:
                     self._bdec_cache = (_RouteKey(slot_ids, bank_key), b_dec)
         out = torch.ops.lithe_b200.lora_gemm(xs.view(bsz * m, d_in), self.base.weight, self.base.bias, h, b_dec, m)
         return out.view(*x.shape[:-1], d_out)
@@ -221,6 +225,8 @@ class _RoutePrepGroup:
 
     def prep(self, layer: "MultiAdapterLinear", x: torch.Tensor, xs: torch.Tensor, ids: torch.Tensor,
              w: torch.Tensor) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
+        if not _tracked(x, ids, w):
+            return None
         if self._key is not None:
             if self._key.matches(x, ids, w, None):
                 got = self._ready.pop(id(layer), None)

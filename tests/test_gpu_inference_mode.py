@@ -1,0 +1,53 @@
+"""The layers under torch.inference_mode, whose tensors count no versions: nothing that depends on one is
+kept, nothing raises, and the results are those of no_grad, bit for bit."""
+import pytest
+import torch
+
+from lithe_b200 import device_errors, serve
+from lithe_b200.flux_model import FluxConfig, FluxShapedTransformer, lora_targets
+from tests.helpers import random_adapter
+
+pytestmark = pytest.mark.gpu
+
+
+def served(seed, attach):
+    """(model, its inputs, what `attach(model, targets)` gives), seeded."""
+    torch.manual_seed(seed)
+    cfg = FluxConfig.tiny()
+    model = FluxShapedTransformer(cfg).cuda().bfloat16().eval()
+    got = attach(model, lora_targets(model))
+    lat = torch.randn(2, 256, cfg.in_channels, device="cuda").bfloat16()
+    txt = torch.randn(2, 256, cfg.text_dim, device="cuda").bfloat16()
+    pooled = torch.randn(2, cfg.pooled_dim, device="cuda").bfloat16()
+    return model, (lat, txt, pooled, torch.full((2,), 0.5, device="cuda")), got
+
+
+@pytest.mark.parametrize("fused_gemm", [False, True])
+@pytest.mark.parametrize("attached_inside", [False, True])
+def test_attached_adapters(fused_gemm, attached_inside):
+    def attach(model, targets):
+        ads = [random_adapter([(n, m.in_features, m.out_features) for n, m in targets], rank=16, seed=30 + s)
+               for s in range(3)]
+        with torch.inference_mode(attached_inside):
+            return serve.attach_adapters(model, ads, fused_gemm=fused_gemm)
+
+    model, args, (router, _) = served(9, attach)
+    routes = [[[(2, 1.0)], [(0, 0.5)]], [[(1, 1.0)], [(0, 0.5)]], [[(1, 0.25)], []]]
+    want = []
+    with torch.no_grad():
+        for route in routes:
+            router.set(route)
+            want.append(model(*args))
+    with torch.inference_mode():
+        for _ in range(2):
+            for route, w in zip(routes, want):
+                router.set(route)
+                assert torch.equal(model(*args), w) and torch.equal(model(*args), w)
+        router.set(routes[0])
+        model(*args)
+        router.ids[0, 0] = 1                         # an in-place change of the routing is seen
+        assert torch.equal(model(*args), want[1])
+    with torch.no_grad():
+        router.set(routes[2])
+        assert torch.equal(model(*args), want[2])
+    assert device_errors() == 0

@@ -468,3 +468,31 @@ def test_cpu_arm_runs_the_reference_when_installed(monkeypatch):
     monkeypatch.setattr(bench, "CPU_SAMPLE_TOKENS", 64)
     rec = bench.cpu_reference_passes(2, warmup=1)
     assert rec["kind"] == "reference" and "MultiAdapterLinear" in rec["path"]
+
+
+def test_router_under_inference_mode():
+    """The device tables are kept while the routing is unchanged; tables of the caller's own that count no
+    versions (made under inference_mode) are looked at anew in every call."""
+    cpu = torch.device("cpu")
+    r = serve.Router()
+    with torch.inference_mode():
+        r.set([[(0, 1.0)], [(1, 0.5)]])
+        cols = r.columns(cpu, (2.0, 0.5))
+        assert r.columns(cpu, (2.0, 0.5)) is cols and not any(t.is_inference() for t in cols[0])
+        r.ids[0, 0] = 1
+        assert r.columns(cpu, (2.0, 0.5))[0][0].tolist() == [1, 1]
+        r.ids, r.weights = torch.tensor([[0], [1]]), torch.tensor([[1.0], [0.5]])
+        assert r.columns(cpu, (2.0, 0.5))[0][0].tolist() == [0, 1]
+        r.ids[0, 0] = 1
+        cols = r.columns(cpu, (2.0, 0.5))
+        assert cols[0][0].tolist() == [1, 1] and cols[0][1].tolist() == [0.5, 0.25]
+
+
+def test_level_lut_of_pools_made_under_inference_mode():
+    with torch.inference_mode():
+        pools = cb.build_pools([0.5, 0.25])
+        lut = cb.level_lut(pools)
+        assert np.array_equal(lut, cb.level_lut(pools))
+        pools.mul_(2)
+        assert np.array_equal(cb.level_lut(pools), 2 * lut)
+    assert np.array_equal(cb.level_lut(cb.build_pools([0.5, 0.25])), lut)
