@@ -237,7 +237,7 @@ class SharedInputPrep:
     def prep(self, layer: "PackedLoRALinear", x3: torch.Tensor, ids: torch.Tensor,
              w: Optional[torch.Tensor]) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
         """(h, b_dec) of ``layer`` for this call, or None when the group does not apply."""
-        if not _tracked(x3, ids, w):
+        if not _tracked(x3, ids, w, layer.bank.words):
             return None
         if self._key is not None:
             if self._key.matches(x3, ids, w, None):
@@ -445,14 +445,14 @@ class PackedLoRALinear(nn.Module):
             h, b_dec = got
         else:
             share = self.rows is not None and not compiling and _tracked(x3, ids, w)
-            keep = not compiling and _tracked(ids)
+            keep = not compiling and _tracked(ids, self.bank.words)
             h = self._shared_h(x3, ids, w) if share else None
             fresh = h is None
             words = self.bank.words
             # B factor of this routing: decoded once and kept while the routing and the bank's
             # contents are unchanged (a denoise loop's steps); traced graphs decode every call
             b_dec = None
-            bank_key = self.bank.contents_key()
+            bank_key = self.bank.contents_key() if keep else None
             if keep and self._bdec_cache is not None and self._bdec_cache[0].matches(ids, bank_key):
                 b_dec = self._bdec_cache[1]
             if b_dec is None:

@@ -3,8 +3,9 @@ kept, nothing raises, and the results are those of no_grad, bit for bit."""
 import pytest
 import torch
 
-from lithe_b200 import device_errors, serve
+from lithe_b200 import device_errors, kohya, serve
 from lithe_b200.flux_model import FluxConfig, FluxShapedTransformer, lora_targets
+from lithe_b200.kernels import PackedBank, PackedLayout, wrap_packed
 from tests.helpers import random_adapter
 
 pytestmark = pytest.mark.gpu
@@ -50,4 +51,40 @@ def test_attached_adapters(fused_gemm, attached_inside):
     with torch.no_grad():
         router.set(routes[2])
         assert torch.equal(model(*args), want[2])
+    assert device_errors() == 0
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("key_format", ["diffusers", "kohya"])
+def test_a_bank_made_under_inference_mode(key_format, int8):
+    def attach(model, targets):
+        if key_format == "kohya":
+            cfg = model.cfg
+            mods = kohya.kohya_flux_modules(rank=16, double_blocks=cfg.double_blocks, single_blocks=cfg.single_blocks,
+                                            hidden=cfg.hidden, mlp_ratio=cfg.mlp_ratio)
+        else:
+            mods = [{"name": n, "shape_a": [16, m.in_features], "shape_b": [m.out_features, 16]} for n, m in targets]
+        lay = PackedLayout.from_modules(mods)
+        with torch.inference_mode():
+            bank = PackedBank(lay, 4, "cuda")
+            bank.fill_random(seed=5)
+            wrapped = wrap_packed(model, bank, key_format, scaling=20.0, fused_gemm=not int8, int8_base=int8)
+        return bank, wrapped
+
+    model, args, (bank, wrapped) = served(11, attach)
+    for m in wrapped.values():
+        m.assign = torch.tensor([1, 3], dtype=torch.int32, device="cuda")
+    other = PackedBank(bank.layout, 4, "cuda")
+    other.words.copy_(bank.words)
+    with torch.inference_mode():
+        got = model(*args)
+        bank.fill_random(seed=6)                     # new adapters in the same slots
+        moved = model(*args)
+        bank.words.copy_(other.words)
+        assert torch.equal(model(*args), got) and not torch.equal(moved, got)
+    with torch.no_grad():
+        assert torch.equal(model(*args), got)
+        for m in wrapped.values():                   # a bank that counts versions gives the same
+            m.bank = other
+        assert torch.equal(model(*args), got) and torch.equal(model(*args), got)
     assert device_errors() == 0
