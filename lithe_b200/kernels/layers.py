@@ -161,13 +161,14 @@ def _tracked(*tensors: Optional[torch.Tensor]) -> bool:
 
 class _InputKey:
     """Identifies one call's input, routing and weights by tensor identity and version, through
-    weak references: a key does not keep the activation it names alive.  It names the stream and the
+    weak references: a key does not keep the activation it names alive.  ``extra`` is a tuple of what
+    else the results depend on (the index banks' contents, the scalings).  It names the stream and the
     graph capture too: on another stream the results may not be there yet, and a captured call whose
     replays see new values in the same tensors needs its own, made in that capture."""
 
-    def __init__(self, x3, ids, w, scaling):
+    def __init__(self, x3, ids, w, extra):
         self._refs = (weakref.ref(x3), weakref.ref(ids), None if w is None else weakref.ref(w))
-        self._vals = (x3._version, ids._version, None if w is None else w._version, scaling)
+        self._vals = (x3._version, ids._version, None if w is None else w._version, extra)
         self._where = _launch.ordered_after(x3.device)
 
     def alive(self) -> bool:
@@ -178,11 +179,11 @@ class _InputKey:
         """The key was made on the current stream, inside the same capture or outside of any."""
         return self._where == _launch.ordered_after(device)
 
-    def matches(self, x3, ids, w, scaling) -> bool:
+    def matches(self, x3, ids, w, extra) -> bool:
         rx, ri, rw = self._refs
         if rx() is not x3 or ri() is not ids or (rw is None) != (w is None) or (rw is not None and rw() is not w):
             return False
-        return (self._vals == (x3._version, ids._version, None if w is None else w._version, scaling)
+        return (self._vals == (x3._version, ids._version, None if w is None else w._version, extra)
                 and self._where is not None and self._where == _launch.ordered_after(x3.device))
 
 
@@ -239,8 +240,9 @@ class SharedInputPrep:
         """(h, b_dec) of ``layer`` for this call, or None when the group does not apply."""
         if not _tracked(x3, ids, w, layer.bank.words):
             return None
+        extra = (layer.bank.contents_key(), tuple(m.scaling for m in self.members))
         if self._key is not None:
-            if self._key.matches(x3, ids, w, None):
+            if self._key.matches(x3, ids, w, extra):
                 got = self._ready.pop(id(layer), None)
                 if not self._ready:
                     self._key = None
@@ -255,8 +257,8 @@ class SharedInputPrep:
         if layer not in members or len(members) < 2:
             return None
         words = [layer.bank.words] * len(members)
-        extra = (layer.bank.contents_key(), tuple(id(m) for m in members))
-        cached = self._bdec_key is not None and self._bdec_key.matches(ids, extra)
+        route = (extra[0], tuple(id(m) for m in members))
+        cached = self._bdec_key is not None and self._bdec_key.matches(ids, route)
         outs = torch.ops.lithe_b200.lora_prep_multi(
             x3, words, words, [v for m in members for v in m._va], [v for m in members for v in m._vb],
             layer.bank.n_slots, ids, w, [m.base.out_features for m in members], layer._lut,
@@ -264,10 +266,10 @@ class SharedInputPrep:
         n = len(members)
         if not cached:
             self._bdecs = outs[n:]
-            self._bdec_key = _RouteKey(ids, extra)
+            self._bdec_key = _RouteKey(ids, route)
         bds = self._bdecs
         self._ready = {id(m): (outs[i], bds[i]) for i, m in enumerate(members) if m is not layer}
-        self._key = _InputKey(x3, ids, w, None)
+        self._key = _InputKey(x3, ids, w, extra)
         i = members.index(layer)
         return outs[i], bds[i]
 
@@ -400,22 +402,22 @@ class PackedLoRALinear(nn.Module):
             return None
         return self.weights.to(device=x3.device, dtype=torch.float32).contiguous()
 
-    def _h_key(self, x3, ids, w):
-        return _InputKey(x3, ids, w, self.scaling)
+    def _h_depends(self) -> tuple:
+        return (self.scaling, self.bank.contents_key())
 
     def _shared_h(self, x3, ids, w) -> Optional[torch.Tensor]:
         """The h a sibling split target computed for the same input, routing and scale, if any
-        (the very same, unmodified tensor objects)."""
+        (the very same, unmodified tensor objects, and no slot of the bank written since)."""
         entry = getattr(self.bank, "_shared_h", {}).get(self.name)
         if entry is None:
             return None
         key, h = entry
-        return h if key.matches(x3, ids, w, self.scaling) else None
+        return h if key.matches(x3, ids, w, self._h_depends()) else None
 
     def _store_h(self, x3, ids, w, h) -> None:
         if not hasattr(self.bank, "_shared_h"):
             self.bank._shared_h = {}
-        self.bank._shared_h[self.name] = (self._h_key(x3, ids, w), h)      # one entry per fused module
+        self.bank._shared_h[self.name] = (_InputKey(x3, ids, w, self._h_depends()), h)      # one entry per fused module
 
     def _forward_fused_gemm(self, x: torch.Tensor, x3: torch.Tensor) -> torch.Tensor:
         bsz, m, d_in = x3.shape
@@ -444,7 +446,7 @@ class PackedLoRALinear(nn.Module):
         if got is not None:
             h, b_dec = got
         else:
-            share = self.rows is not None and not compiling and _tracked(x3, ids, w)
+            share = self.rows is not None and not compiling and _tracked(x3, ids, w, self.bank.words)
             keep = not compiling and _tracked(ids, self.bank.words)
             h = self._shared_h(x3, ids, w) if share else None
             fresh = h is None

@@ -225,10 +225,11 @@ class _RoutePrepGroup:
 
     def prep(self, layer: "MultiAdapterLinear", x: torch.Tensor, xs: torch.Tensor, ids: torch.Tensor,
              w: torch.Tensor) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
-        if not _tracked(x, ids, w):
+        if not _tracked(x, ids, w, *(t for m in self.members for t in (m.idx_a, m.idx_b))):
             return None
+        extra = tuple((m._n_added, m.idx_a._version, m.idx_b._version) for m in self.members)
         if self._key is not None:
-            if self._key.matches(x, ids, w, None):
+            if self._key.matches(x, ids, w, extra):
                 got = self._ready.pop(id(layer), None)
                 if not self._ready:
                     self._key = None
@@ -248,7 +249,7 @@ class _RoutePrepGroup:
             layer._lut, [1.0] * len(members), True)
         n = len(members)
         self._ready = {id(m): (outs[i], outs[n + i]) for i, m in enumerate(members) if m is not layer}
-        self._key = _InputKey(x, ids, w, None)
+        self._key = _InputKey(x, ids, w, extra)
         i = members.index(layer)
         return outs[i], outs[n + i]
 

@@ -145,3 +145,68 @@ def test_decoded_b_factors_are_reused_while_routing_and_bank_are_unchanged():
                 m.prep_group._bdec_key = None
         fresh = model(*args)
     assert torch.equal(after, fresh)
+
+
+@pytest.mark.parametrize("int8", [False, True])
+@pytest.mark.parametrize("key_format", ["diffusers", "kohya"])
+def test_a_bank_written_between_siblings_is_seen(key_format, int8):
+    """q runs on an input, its bank's slots get other adapters, k and v run on the same input: they use the
+    new ones (what q prepared for them, or their shared h, is of the old)."""
+    from lithe_b200 import kohya
+    torch.manual_seed(21)
+    cfg = FluxConfig.tiny()
+    model = FluxShapedTransformer(cfg).cuda().bfloat16().eval()
+    if key_format == "kohya":
+        mods = kohya.kohya_flux_modules(rank=16, double_blocks=cfg.double_blocks, single_blocks=cfg.single_blocks,
+                                        hidden=cfg.hidden, mlp_ratio=cfg.mlp_ratio)
+    else:
+        mods = [{"name": n, "shape_a": [16, m.in_features], "shape_b": [m.out_features, 16]}
+                for n, m in lora_targets(model)]
+    bank = PackedBank(PackedLayout.from_modules(mods), 4, "cuda")
+    bank.fill_random(seed=3)
+    wrapped = wrap_packed(model, bank, key_format, scaling=20.0, fused_gemm=not int8, int8_base=int8)
+    ids = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    for m in wrapped.values():
+        m.assign = ids
+    q, k, v = (wrapped[f"transformer_blocks.0.attn.to_{c}"] for c in "qkv")
+    x = torch.randn(2, 256, cfg.hidden, device="cuda").bfloat16()
+    raw = torch.randint(0, 512, (bank.layout.num_indices,), dtype=torch.int16, device="cuda")
+    with torch.no_grad():
+        q(x)
+        bank.load_raw(1, raw)
+        got_k = k(x)
+        bank.words[2].copy_(bank.words[1])
+        got_v = v(x)
+        for m in (q, k, v):                          # against calls with nothing shared or kept
+            m.prep_group = m._bdec_cache = None
+        bank._shared_h = {}
+        want_v = v(x)
+        k._bdec_cache, bank._shared_h = None, {}
+        torch.random.manual_seed(0)
+        bank.fill_random(seed=3)
+        bank.load_raw(1, raw)
+        want_k = k(x.clone())
+    assert torch.equal(got_k, want_k) and torch.equal(got_v, want_v)
+
+
+def test_attached_banks_written_between_siblings_are_seen():
+    from lithe_b200 import serve
+    from tests.helpers import random_adapter
+
+    torch.manual_seed(22)
+    cfg = FluxConfig.tiny()
+    model = FluxShapedTransformer(cfg).cuda().bfloat16().eval()
+    ads = [random_adapter([(n, m.in_features, m.out_features) for n, m in lora_targets(model)], rank=16, seed=40 + s)
+           for s in range(2)]
+    router, layers = serve.attach_adapters(model, ads, fused_gemm=True)
+    router.set([[(1, 1.0)], [(0, 0.5)]])
+    q, k = (next(l for n, l in layers.items() if n.endswith(f"transformer_blocks.0.attn.to_{c}") and "single" not in n)
+            for c in "qk")
+    assert q.prep_group is k.prep_group is not None
+    x = torch.randn(2, 256, cfg.hidden, device="cuda").bfloat16()
+    with torch.no_grad():
+        q(x)
+        k.idx_a[1].copy_(k.idx_a[0])
+        got = k(x)
+        k.prep_group = k._bdec_cache = None
+        assert torch.equal(got, k(x))
