@@ -94,6 +94,16 @@ def ordered_after(device: torch.device) -> Optional[Tuple[int, int]]:
     return None if capture < 0 else (stream, capture)
 
 
+_dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+
+
+def recorded(t: torch.Tensor) -> bool:
+    """Whether a call on ``t`` is recorded or interpreted instead of only run -- torch.compile, jit.trace, a
+    dispatch mode (make_fx, FakeTensorMode), a tensor subclass -- so that it must reach its kernel as a torch op."""
+    return (torch.compiler.is_compiling() or torch.jit.is_tracing() or _dispatch_modes() > 0
+            or type(t) not in (torch.Tensor, torch.nn.Parameter))
+
+
 _lut_cache: dict = {}
 
 

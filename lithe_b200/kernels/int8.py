@@ -49,7 +49,7 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     if k > 1 and x2.stride(1) != 1:
         x2 = x2.contiguous()
-    if torch.compiler.is_compiling():
+    if _launch.recorded(x):
         q, scale = torch.ops.lithe_b200.quantize_rows(x2)
     else:
         q = torch.empty(x2.shape[0], _launch.padded(k), dtype=torch.int8, device=x.device)[:, :k]
@@ -82,13 +82,13 @@ def int8_linear(x: Union[torch.Tensor, QuantizedRows], weight: torch.Tensor, wei
     _inference_only(bias, weight_scale, h, b_dec, *((x.scale,) if isinstance(x, QuantizedRows) else (x,)))
     if isinstance(x, QuantizedRows):
         n = weight.shape[0]
-        if torch.compiler.is_compiling():
+        if _launch.recorded(x.q):
             out = torch.ops.lithe_b200.int8_linear(x.q, x.scale, weight, weight_scale, bias, h, b_dec,
                                                    x.dtype == torch.float16)
         else:
             out = torch.empty(x.q.shape[0], n, dtype=x.dtype, device=x.q.device)
             _launch.int8_linear_(x.q, x.scale, weight, weight_scale, bias, out, h, b_dec)
         return out.view(*x.shape, n)
-    if torch.compiler.is_compiling():
+    if _launch.recorded(x):
         return torch.ops.lithe_b200.int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec)
     return _launch.int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec)

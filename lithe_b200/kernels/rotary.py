@@ -67,13 +67,13 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     """
     _launch._check_heads(x, "x")
     _inference_only(x, positions, out)
-    compiling = torch.compiler.is_compiling()
-    axes, theta, code = (_rotation.__wrapped__ if compiling else _rotation)(x.shape[3], tuple(axes), theta, pairing)
+    as_op = _launch.recorded(x)
+    axes, theta, code = (_rotation.__wrapped__ if as_op else _rotation)(x.shape[3], tuple(axes), theta, pairing)
     fresh = out is None
     if fresh:
         out = x.new_empty(x.shape)
     positions = positions.contiguous()
-    if compiling:
+    if as_op:
         if out is x:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
             torch.ops.lithe_b200.rotate_axes_(out, x, positions, list(axes), theta, code)
@@ -105,15 +105,15 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
-    compiling = torch.compiler.is_compiling()
-    axes, theta, code = (_rotation.__wrapped__ if compiling else _rotation)(q.shape[3], tuple(axes), theta, pairing)
+    as_op = _launch.recorded(q)
+    axes, theta, code = (_rotation.__wrapped__ if as_op else _rotation)(q.shape[3], tuple(axes), theta, pairing)
     fresh = out_q is None and out_k is None
     if out_q is None:
         out_q = q.new_empty(q.shape)
     if out_k is None:
         out_k = k.new_empty(k.shape)
     positions = positions.contiguous()
-    if compiling:
+    if as_op:
         oq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is q else out_q
         ok = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is k else out_k
         torch.ops.lithe_b200.qk_norm_rotate_(oq, ok, q, k, weight_q, weight_k, positions, list(axes), theta, eps, code)
