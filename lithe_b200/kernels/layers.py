@@ -209,8 +209,8 @@ class SharedInputPrep:
     instead of once per linear) and hands the others theirs; results are bit-identical to
     each member's own lithe_lora_prep.  A member called on another input while results for a
     live input are pending, called again on an input it already took, on the cuBLAS path, or
-    under torch.compile (the hand-over keys on tensor identity, which a traced graph does not
-    have), computes its own.  Pending results for an input that has been freed, or that were
+    under torch.compile or another tracer (the hand-over keys on tensor identity, which a traced
+    graph does not have), computes its own.  Pending results for an input that has been freed, or that were
     made on another stream or in another graph capture, are dropped.
     Members must share one ``assign`` tensor (int32, on the device) for the hand-over to
     apply.  The members' decoded B factors are kept for the last routing (see
@@ -435,19 +435,19 @@ class PackedLoRALinear(nn.Module):
         w = self._weights(x3)
         # Split targets of one fused module (Kohya q/k/v, q/k/v/proj_mlp) share its A factor and are
         # called with the same input, so h = x . A^T is computed once and reused by the others.  The
-        # reuse keys on tensor identity, which a traced graph does not have: under torch.compile
-        # every target computes its own h (the same values).
+        # reuse keys on tensor identity, which a traced graph does not have: under torch.compile or
+        # another tracer every target computes its own h (the same values).
         # Linears with their own A that read the same input (q, k, v of one attention) take
         # their h and b_dec from one multi-target prep when grouped (SharedInputPrep).
-        compiling = torch.compiler.is_compiling()
+        recorded = _launch.recorded(x3)
         got = None
-        if self.prep_group is not None and self.rows is None and not compiling:
+        if self.prep_group is not None and self.rows is None and not recorded:
             got = self.prep_group.prep(self, x3, ids, w)
         if got is not None:
             h, b_dec = got
         else:
-            share = self.rows is not None and not compiling and _tracked(x3, ids, w, self.bank.words)
-            keep = not compiling and _tracked(ids, self.bank.words)
+            share = self.rows is not None and not recorded and _tracked(x3, ids, w, self.bank.words)
+            keep = not recorded and _tracked(ids, self.bank.words)
             h = self._shared_h(x3, ids, w) if share else None
             fresh = h is None
             words = self.bank.words

@@ -153,14 +153,15 @@ class MultiAdapterLinear(nn.Module):
         bsz, m, d_in = xs.shape
         d_out = self.base.out_features
         got = None
-        if self.prep_group is not None and not torch.compiler.is_compiling():
+        recorded = _launch.recorded(xs)
+        if self.prep_group is not None and not recorded:
             got = self.prep_group.prep(self, x, xs, slot_ids, w)
         if got is not None:
             h, b_dec = got
         else:
             va, vb = self._view_params()
             # the B factors of this route column, decoded once while it and the banks are unchanged
-            keep = not torch.compiler.is_compiling() and _tracked(slot_ids, self.idx_a, self.idx_b)
+            keep = not recorded and _tracked(slot_ids, self.idx_a, self.idx_b)
             bank_key = (self._n_added, self.idx_a._version, self.idx_b._version) if keep else None
             cache = self._bdec_cache
             if keep and cache is not None and cache[0].matches(slot_ids, bank_key):

@@ -5,7 +5,8 @@ import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 
 from lithe_b200 import device_errors
-from lithe_b200.kernels import Int8Linear, int8_linear, qk_norm_rotate, quantize_rows, quantize_weight, rotate_axes
+from lithe_b200.kernels import (Int8Linear, PackedBank, PackedLayout, int8_linear, qk_norm_rotate, quantize_rows,
+                                quantize_weight, rotate_axes, wrap_packed)
 from tests.test_gpu_int8 import make
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +62,38 @@ def test_layer(how):
         g = traced(how, layer, (make((3, 5, 96), BF, 1),))
         x = make((3, 5, 96), BF, 2)
         assert torch.equal(g(x), layer(x))
+
+
+@pytest.mark.parametrize("how", ["jit", "fx"])
+@pytest.mark.parametrize("int8", [False, True])
+def test_layers_keep_nothing_in_a_trace(how, int8):
+    """q, k and v of a block traced after eager calls have left a B factor and a shared preparation behind: the
+    trace has its own, so that it follows the routing tensor and the bank."""
+    names = ["b.attn.to_q", "b.attn.to_k", "b.attn.to_v"]
+    bank = PackedBank(PackedLayout.from_modules([{"name": n, "shape_a": [16, 256], "shape_b": [256, 16]} for n in names]),
+                      8, DEV)
+    bank.fill_random(seed=1)
+    block = torch.nn.Module()
+    block.b = torch.nn.Module()
+    block.b.attn = torch.nn.Module()
+    for n in names:
+        setattr(block.b.attn, n.split(".")[-1], torch.nn.Linear(256, 256, device=DEV, dtype=BF).requires_grad_(False))
+    layers = list(wrap_packed(block, bank, scaling=2.0, int8_base=int8, fused_gemm=not int8).values())
+    ids = torch.tensor([1, 4], dtype=torch.int32, device=DEV)
+    for m in layers:
+        m.assign = ids
+
+    def f(x):
+        return tuple(m(x) for m in layers)
+
+    with torch.no_grad():
+        x = make((2, 128, 256), BF, 1)
+        f(x)
+        layers[0](x)                                 # leaves the other two's results pending
+        g = traced(how, f, (x,))
+        ids.copy_(torch.tensor([3, 0], dtype=torch.int32))
+        y = make((2, 128, 256), BF, 2)
+        assert all(torch.equal(a, b) for a, b in zip(g(y), f(y)))
+        bank.fill_random(seed=7)
+        assert all(torch.equal(a, b) for a, b in zip(g(x), f(x)))
+    assert device_errors() == 0
