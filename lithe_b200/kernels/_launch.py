@@ -15,6 +15,7 @@ from typing import Optional, Sequence, Tuple
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
@@ -102,6 +103,17 @@ def recorded(t: torch.Tensor) -> bool:
     dispatch mode (make_fx, FakeTensorMode), a tensor subclass -- so that it must reach its kernel as a torch op."""
     return (torch.compiler.is_compiling() or torch.jit.is_tracing() or _dispatch_modes() > 0
             or type(t) not in (torch.Tensor, torch.nn.Parameter))
+
+
+def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether a derivative through one of the tensors is being recorded: it requires a gradient while grad mode
+    is on, or carries a forward-mode tangent.  The kernels have none to give."""
+    grad = torch.is_grad_enabled()
+    forward = getattr(forward_ad, "_current_level", -1) >= 0
+    if not (grad or forward):
+        return False
+    return any(t is not None and ((grad and t.requires_grad)
+                                  or (forward and forward_ad.unpack_dual(t).tangent is not None)) for t in tensors)
 
 
 _lut_cache: dict = {}

@@ -31,7 +31,7 @@ from .shared import _check
 
 
 def _inference_only(out: torch.Tensor) -> None:
-    if out.requires_grad and torch.is_grad_enabled():
+    if _launch.differentiated(out):
         raise RuntimeError("lithe_b200 layers are inference-only: run them under torch.no_grad()")
 
 
@@ -385,7 +385,7 @@ class PackedLoRALinear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         x3 = x.unsqueeze(1) if x.dim() == 2 else x
         if x3.dim() == 3 and self._takes_expand(x3):
-            if torch.is_grad_enabled() and (x.requires_grad or self.base.weight.requires_grad):
+            if _launch.differentiated(x, self.base.weight):
                 raise RuntimeError("lithe_b200 layers are inference-only (run under torch.no_grad())")
             return self._forward_fused_gemm(x, x3.contiguous())
         out = self.base(x)

@@ -29,9 +29,8 @@ from . import _launch
 
 
 def _inference_only(*tensors: Optional[torch.Tensor]) -> None:
-    for t in tensors:
-        if t is not None and t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
+    if _launch.differentiated(*tensors):
+        raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
 
 
 def _written(*tensors: torch.Tensor) -> None:

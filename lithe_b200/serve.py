@@ -188,7 +188,7 @@ class MultiAdapterLinear(nn.Module):
                 xs = x.reshape(bsz, -1, x.shape[-1]).contiguous()
                 cols = self.router.columns(x.device, tuple(self.scales))
                 if len(cols) == 1 and self._gemm_ok(xs):
-                    if torch.is_grad_enabled() and (x.requires_grad or self.base.weight.requires_grad):
+                    if _launch.differentiated(x, self.base.weight):
                         raise RuntimeError("lithe_b200 layers are inference-only (run under torch.no_grad())")
                     return self._forward_fused_gemm(x, xs, *cols[0])
         out = self.base(x)
