@@ -1075,8 +1075,6 @@ class _DenoiseSetup:
         fused_qk = kind.endswith("_qk")
         kind = kind[:-3] if fused_qk else kind
         self.model.cfg.fused_qk = fused_qk
-        for blk in (*self.model.transformer_blocks, *self.model.single_transformer_blocks):
-            blk.fused_qk = fused_qk
         if kind == "lithe_int8" and kind not in self.tables:
             self.tables[kind] = self._on_int8()
         for m in self.packed.values():

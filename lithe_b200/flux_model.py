@@ -213,7 +213,6 @@ class DoubleBlock(nn.Module):
         d = cfg.hidden
         self.norm1, self.norm1_context = AdaNorm(d, 6), AdaNorm(d, 6)
         self.attn = JointAttention(d, cfg.heads, context=True)
-        self.fused_qk = cfg.fused_qk
         self.ff = FeedForward(d, d * cfg.mlp_ratio)
         self.ff_context = FeedForward(d, d * cfg.mlp_ratio)
 
@@ -223,7 +222,7 @@ class DoubleBlock(nn.Module):
         a = self.attn
         xi = _mod(_ln(img), sh, sc)
         xt = _mod(_ln(txt), csh, csc)
-        if self.fused_qk:
+        if torch.is_tensor(rope):
             o = _attend_joint([(a.add_q_proj(xt), a.add_k_proj(xt), a.add_v_proj(xt), a.norm_added_q, a.norm_added_k),
                                (a.to_q(xi), a.to_k(xi), a.to_v(xi), a.norm_q, a.norm_k)], a.heads, rope)
         else:
@@ -244,7 +243,6 @@ class SingleBlock(nn.Module):
         d = cfg.hidden
         self.norm = AdaNorm(d, 3)
         self.attn = JointAttention(d, cfg.heads, context=False)
-        self.fused_qk = cfg.fused_qk
         self.proj_mlp = nn.Linear(d, d * cfg.mlp_ratio)
         self.proj_out = nn.Linear(d + d * cfg.mlp_ratio, d)
 
@@ -252,7 +250,7 @@ class SingleBlock(nn.Module):
         sh, sc, g = self.norm(temb)
         h = _mod(_ln(x), sh, sc)
         a = self.attn
-        if self.fused_qk:
+        if torch.is_tensor(rope):
             o = _attend_joint([(a.to_q(h), a.to_k(h), a.to_v(h), a.norm_q, a.norm_k)], a.heads, rope)
         else:
             q, k, v = a._qkv(h, a.to_q, a.to_k, a.to_v, a.norm_q, a.norm_k)
@@ -290,6 +288,7 @@ class FluxShapedTransformer(nn.Module):
         temb = self.time_in(self.timestep_embedding(t).to(dtype)) + self.pooled_in(pooled)
         img = self.x_embedder(latents)
         txt = self.context_embedder(text)
+        # what rope is tells every block which form to take: positions (qk_norm_rotate) or tables (plain torch)
         if self.cfg.fused_qk:
             rope = rope_positions(txt.shape[1], img.shape[1], img.device)
         else:
