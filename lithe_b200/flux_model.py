@@ -159,31 +159,39 @@ def _rotate(t, cos_f, sin_f):
     return torch.addcmul(t * cos_f, swapped, sin_f)
 
 
+def _sdpa(q, k, v):
+    """Attention of (b, heads, s, hd) to (b, s, heads * hd).  (An empty batch is answered here: on CUDA torch's
+    attention has no answer to one.)"""
+    b, heads, s, hd = q.shape
+    if b == 0:
+        return q.new_empty(0, s, heads * hd)
+    return F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(b, s, heads * hd)
+
+
 def _attend(q, k, v, heads, rope=None):
     b, s, d = q.shape
     hd = d // heads
     q, k, v = (t.view(b, s, heads, hd).transpose(1, 2) for t in (q, k, v))
     if rope is not None:
         q, k = _rotate(q, *rope), _rotate(k, *rope)
-    o = F.scaled_dot_product_attention(q, k, v)
-    return o.transpose(1, 2).reshape(b, s, d)
+    return _sdpa(q, k, v)
 
 
 def _attend_joint(parts, heads, positions):
     """Attention over the joint sequence of ``parts``, each (q, k, v, norm of q, norm of k) of one stream
     straight from its projections: ``qk_norm_rotate`` writes every stream's q and k into its place."""
     b, d = parts[0][0].shape[0], parts[0][0].shape[2]
-    hd = d // heads
-    q, k = (parts[0][0].new_empty(b, positions.shape[0], heads, hd) for _ in range(2))
+    s, hd = positions.shape[0], d // heads
+    q, k = (parts[0][0].new_empty(b, s, heads, hd) for _ in range(2))
     at = 0
     for sq, sk, _, nq, nk in parts:
         end = at + sq.shape[1]
-        qk_norm_rotate(sq.view(b, -1, heads, hd), sk.view(b, -1, heads, hd), nq.weight, nk.weight, positions[at:end],
-                       rope_axes(hd), out_q=q[:, at:end], out_k=k[:, at:end])
+        qk_norm_rotate(sq.view(b, end - at, heads, hd), sk.view(b, end - at, heads, hd), nq.weight, nk.weight,
+                       positions[at:end], rope_axes(hd), out_q=q[:, at:end], out_k=k[:, at:end])
         at = end
     v = parts[0][2] if len(parts) == 1 else torch.cat([p[2] for p in parts], 1)
-    q, k, v = (t.transpose(1, 2) for t in (q, k, v.view(b, -1, heads, hd)))
-    return F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(b, -1, d)
+    q, k, v = (t.transpose(1, 2) for t in (q, k, v.view(b, s, heads, hd)))
+    return _sdpa(q, k, v)
 
 
 class JointAttention(nn.Module):

@@ -36,3 +36,13 @@ def test_fused_qk_is_one_switch(built):
             calls = [n for n in graph.nodes if "qk_norm_rotate_" in str(n.target)]
             assert len(calls) == (2 * cfg.double_blocks + cfg.single_blocks if fused else 0)
             assert model(*args).shape == (2, 9, cfg.in_channels)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+@pytest.mark.parametrize("batch,n_img,n_txt", [(0, 9, 5), (2, 9, 0), (2, 0, 5), (1, 1, 1)])
+def test_empty_batches_and_streams(batch, n_img, n_txt, fused):
+    with FakeTensorMode(), torch.no_grad():
+        cfg = FluxConfig.tiny()
+        cfg.fused_qk = fused
+        got = fake_model(cfg)(*inputs(cfg, batch, n_img, n_txt))
+    assert got.shape == (batch, n_img, cfg.in_channels)

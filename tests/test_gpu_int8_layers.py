@@ -323,3 +323,14 @@ def test_results_shared_on_one_stream_alone():
             assert layer._bdec_cache[1] is not kept
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("batch,n_img,n_txt", [(0, 9, 5), (2, 9, 0), (2, 0, 5), (1, 1, 1)])
+def test_model_on_empty_batches_and_streams(batch, n_img, n_txt):
+    model, (lat, txt, pooled, t) = tiny(5, False)
+    fused, _ = tiny(5, True, model.state_dict())
+    args = (lat[:batch, :n_img], txt[:batch, :n_txt], pooled[:batch], t[:batch])
+    with torch.no_grad():
+        want, got = model(*args), fused(*args)
+    assert got.shape == want.shape == (batch, n_img, 16)
+    assert got.numel() == 0 or rel_fro(got.float(), want.float()) < 2e-2
