@@ -292,7 +292,9 @@ class FluxShapedTransformer(nn.Module):
         return torch.cat([torch.cos(args), torch.sin(args)], dim=-1)
 
     def forward(self, latents, text, pooled, t):
-        dtype = latents.dtype
+        # the model's type is its weights'; an 8-bit embedder has none, there it is the latents'
+        w = getattr(self.x_embedder, "weight", None)
+        dtype = w.dtype if w is not None and w.is_floating_point() else latents.dtype
         temb = self.time_in(self.timestep_embedding(t).to(dtype)) + self.pooled_in(pooled)
         img = self.x_embedder(latents)
         txt = self.context_embedder(text)

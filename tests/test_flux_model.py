@@ -46,3 +46,32 @@ def test_empty_batches_and_streams(batch, n_img, n_txt, fused):
         cfg.fused_qk = fused
         got = fake_model(cfg)(*inputs(cfg, batch, n_img, n_txt))
     assert got.shape == (batch, n_img, cfg.in_channels)
+
+
+@pytest.mark.parametrize("weights,latents", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16),
+                                             (torch.bfloat16, torch.bfloat16)])
+def test_the_time_embedding_has_the_weights_type(weights, latents):
+    """Under autocast the latents may have another type than the weights; the embedding goes by the weights."""
+    cfg = FluxConfig.tiny()
+    model = FluxShapedTransformer(cfg).to(weights)
+    seen = []
+    model.time_in.register_forward_pre_hook(lambda mod, args: seen.append(args[0].dtype))
+    with torch.no_grad(), torch.autocast("cpu", torch.bfloat16):
+        model(*inputs(cfg, device="cpu", dtype=latents))
+    assert seen == [weights]
+
+
+def test_the_time_embedding_of_an_8_bit_embedder():
+    class Wrapped(torch.nn.Module):                  # an embedder without a weight of its own
+        def __init__(self, base):
+            super().__init__()
+            self.base = base
+
+        def forward(self, x):
+            return self.base(x)
+
+    cfg = FluxConfig.tiny()
+    model = FluxShapedTransformer(cfg).to(torch.bfloat16)
+    model.x_embedder = Wrapped(model.x_embedder)
+    with torch.no_grad():
+        assert model(*inputs(cfg, device="cpu")).dtype == torch.bfloat16
