@@ -40,18 +40,25 @@ def _written(*tensors: torch.Tensor) -> None:
 
 
 @functools.lru_cache(maxsize=256)
-def _rotation(dim: int, axes: Tuple[int, ...], theta: float, pairing: str) -> Tuple[Tuple[int, ...], float, int]:
-    axes = tuple(operator.index(a) for a in axes)
+def _checked_rotation(dim: int, axes: Tuple[int, ...], theta: float, pairing: str) -> int:
     if pairing not in _launch.PAIRINGS:
         raise ValueError(f"pairing must be one of {tuple(_launch.PAIRINGS)}, got {pairing!r}")
     if not 1 <= len(axes) <= _lib.MAX_AXES:
         raise ValueError(f"1 to {_lib.MAX_AXES} axes, got {len(axes)}")
     if any(a < 0 or a % 2 for a in axes) or sum(axes) > dim:
         raise ValueError(f"the axes' dims {axes} must be even, not negative and sum to at most the head dim {dim}")
-    theta = float(theta)
     if not (theta > 0.0 and math.isfinite(theta)):
         raise ValueError(f"theta must be positive and finite, got {theta}")
-    return axes, theta, _launch.PAIRINGS[pairing]
+    return _launch.PAIRINGS[pairing]
+
+
+def _rotation(dim: int, axes: Sequence[int], theta: float, pairing: str,
+              recorded: bool) -> Tuple[Tuple[int, ...], float, int]:
+    """(axes, theta, the pairing's code), plain numbers, checked.  (They are made plain before the lookup: an
+    object that can change, a tensor say, is one key with its old value.)"""
+    axes, theta = tuple(operator.index(a) for a in axes), float(theta)
+    check = _checked_rotation.__wrapped__ if recorded else _checked_rotation
+    return axes, theta, check(dim, axes, theta, pairing)
 
 
 def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *, theta: float = 10000.0,
@@ -67,7 +74,7 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     _launch._check_heads(x, "x")
     _inference_only(x, positions, out)
     as_op = _launch.recorded(x)
-    axes, theta, code = (_rotation.__wrapped__ if as_op else _rotation)(x.shape[3], tuple(axes), theta, pairing)
+    axes, theta, code = _rotation(x.shape[3], axes, theta, pairing, as_op)
     fresh = out is None
     if fresh:
         out = x.new_empty(x.shape)
@@ -105,7 +112,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
     as_op = _launch.recorded(q)
-    axes, theta, code = (_rotation.__wrapped__ if as_op else _rotation)(q.shape[3], tuple(axes), theta, pairing)
+    axes, theta, code = _rotation(q.shape[3], axes, theta, pairing, as_op)
     fresh = out_q is None and out_k is None
     if out_q is None:
         out_q = q.new_empty(q.shape)

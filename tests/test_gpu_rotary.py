@@ -260,3 +260,14 @@ def test_compiled_calls():
     want = both(q, k)
     got = torch.compile(both, fullgraph=True, backend="aot_eager")(q, k)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_theta_and_axes_are_read_in_every_call():
+    x, pos = make((1, 9, 2, 64), torch.float32, 1), torch.arange(18, device=DEV).view(9, 2)
+    theta, axis = torch.tensor(1e4), torch.tensor(16)
+    for t, a in ((1e4, 16), (256.0, 16), (256.0, 40)):
+        theta.fill_(t)
+        axis.fill_(a)
+        assert torch.equal(rotate_axes(x, pos, (axis, 24), theta=theta), rotate_axes(x, pos, (a, 24), theta=t))
+        q, _ = qk_norm_rotate(x, x, None, None, pos, (axis, 24), theta=theta)
+        assert torch.equal(q, qk_norm_rotate(x, x, None, None, pos, (a, 24), theta=t)[0])

@@ -6,7 +6,7 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from lithe_b200 import _lib
-from lithe_b200.kernels import _launch, qk_norm_rotate, rotate_axes
+from lithe_b200.kernels import _launch, qk_norm_rotate, rotary, rotate_axes
 
 
 def _view(**over):
@@ -166,3 +166,20 @@ def test_every_operand_is_inference_only(which):
         if which == "positions":
             with pytest.raises(RuntimeError, match="inference-only"):
                 rotate_axes(ops["k"], ops["positions"], (32, 32))
+
+
+def test_no_answer_is_kept_for_an_object_that_can_change():
+    """axes and theta may come as tensors or arrays: each call takes the numbers that they hold then."""
+    rotation = rotary._rotation
+    theta, axis = torch.tensor(1e4), torch.tensor(16)
+    assert rotation(64, (axis, 24), theta, "interleaved", False) == ((16, 24), 1e4, 0)
+    theta.fill_(256.0)
+    axis.fill_(8)
+    assert rotation(64, (axis, 24), theta, "interleaved", False) == ((8, 24), 256.0, 0)
+    assert rotation(64, [8, 24], 256, "halves", False) == ((8, 24), 256.0, 1)
+    assert all(type(a) is int for a in rotation(64, (True + 7, axis), 1, "halves", False)[0])
+    with pytest.raises(TypeError):
+        rotation(64, (8.0, 24), 256, "halves", False)       # though (8, 24) is known
+    axis.fill_(7)
+    with pytest.raises(ValueError, match="even"):
+        rotation(64, (axis, 24), theta, "interleaved", False)
