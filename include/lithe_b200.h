@@ -362,7 +362,7 @@ typedef struct lithe_heads_view {
  *   (u, v) -> (u cos - v sin, v cos + u sin), in fp32 with the revolution count in fp64, rounded
  *   once.  The values from R = sum(axis_dims) on are copied.
  *   dtype      LITHE_DTYPE_BF16, _F16 or _F32 of x and out; out may be x itself (the same view),
- *              any other overlap of the two is undefined
+ *              any other overlap with x or the positions is undefined
  *   positions  device (tokens, n_axes), or (batch, tokens, n_axes) when per_sample != 0, contiguous,
  *              of pos_type; integers beyond 2^53 are rounded
  *   axis_dims  HOST (n_axes) even, >= 0, sum R at most dim; n_axes 1..LITHE_MAX_AXES
@@ -380,7 +380,7 @@ LITHE_API int32_t lithe_rotate_axes(const lithe_heads_view* x, const lithe_heads
  *   n = x * rsqrt(mean(x^2) + eps) * weight   over the head's dim, in fp32; then turned; one rounding.
  * q and k may have different head counts (grouped heads); out_q / out_k may be slices of larger
  * buffers (a joint [text; image] sequence) or q / k themselves; any other overlap of an output
- * with an input or the other output is undefined.
+ * with what the call reads or with the other output is undefined.
  *   weight_q, weight_k   device (dim) of weight_dtype (dtype or LITHE_DTYPE_F32), or NULL for ones
  */
 LITHE_API int32_t lithe_qk_norm_rotate(const lithe_heads_view* q, const lithe_heads_view* k,

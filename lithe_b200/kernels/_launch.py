@@ -631,6 +631,18 @@ def _check_outputs(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], na
                 raise ValueError(f"{names[i]} overlaps an input (it may be its own input's very view)")
 
 
+def _check_not_written(outs: Sequence[tuple], names: Sequence[str], **read: Optional[torch.Tensor]) -> None:
+    """No output (their _heads_layout) reaches over a contiguous tensor that every token reads."""
+    for what, t in read.items():
+        if t is None:
+            continue
+        first = t.data_ptr()
+        behind = first + t.numel() * t.element_size()
+        for name, (_, o0, o1, _) in zip(names, outs):
+            if first < o1 and o0 < behind:
+                raise ValueError(f"{name} overlaps {what}")
+
+
 def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta: float, pairing: int) -> tuple:
     code = _POS_CODE.get(positions.dtype)
     if code is None:
@@ -661,6 +673,7 @@ def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, ax
     of_x, of_out = _heads_layout(x), _heads_layout(out)
     if not fresh:
         _check_outputs((x,), (out,), ("out",), (of_x, of_out))
+        _check_not_written((of_out,), ("out",), positions=positions)
     b, s, _, d = x.shape
     args = (of_x[0], of_out[0], _DTYPE_CODE[x.dtype], b, s, d,
             *_rotation_args(x, positions, tuple(axes), theta, pairing))
@@ -689,6 +702,7 @@ def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k
     layouts = [_heads_layout(t) for t in (q, k, out_q, out_k)]
     if not fresh:
         _check_outputs((q, k), (out_q, out_k), ("out_q", "out_k"), layouts)
+        _check_not_written(layouts[2:], ("out_q", "out_k"), positions=positions, weight_q=weight_q, weight_k=weight_k)
     b, s, _, d = q.shape
     if k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch, tokens and dim")

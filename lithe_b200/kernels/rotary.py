@@ -69,7 +69,8 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     sample's own; int32, int64 or float32, on x's device.  ``axes``: the head's values each axis
     turns (even, summing to at most dim); dim even, at most 256.  x is bfloat16, float16 or
     float32, with any strides over samples, tokens and heads (a slice of a fused q / k / v
-    projection).  The result is a new tensor, or ``out`` (x itself to rotate in place).
+    projection).  The result is a new tensor, or ``out``: x itself to rotate in place, or memory
+    apart from x and the positions.
     """
     _launch._check_heads(x, "x")
     _inference_only(x, positions, out)
@@ -103,7 +104,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     first three dimensions.  ``weight_q`` / ``weight_k`` (dim,) of q's type or float32, or None
     for a norm without weights.  ``positions``, ``axes``, ``theta`` and ``pairing`` as in
     ``rotate_axes``.  The results are new tensors, or ``out_q`` / ``out_k``: slices of a joint
-    [text; image] buffer, or q and k themselves.
+    [text; image] buffer, or q and k themselves (apart from all else that the call reads).
     """
     _launch._check_heads(q, "q")
     _launch._check_heads(k, "k", q)

@@ -183,3 +183,23 @@ def test_no_answer_is_kept_for_an_object_that_can_change():
     axis.fill_(7)
     with pytest.raises(ValueError, match="even"):
         rotation(64, (axis, 24), theta, "interleaved", False)
+
+
+def test_outputs_apart_from_what_every_token_reads(monkeypatch):
+    """An output that reaches over the positions or the norms' weights is refused: tokens would read each
+    other's results there."""
+    monkeypatch.setattr(_launch, "_require_cuda", lambda t, what: None)
+    buf = torch.zeros(2 * 3 * 2 * 8 + 64)
+    out = buf[:96].view(2, 3, 2, 8)
+    x, k = torch.ones(2, 3, 2, 8), torch.ones(2, 3, 2, 8)
+    for pos in (buf[80:86].view(3, 2), buf[95:101].view(3, 2), buf[:12].view(2, 3, 2)):
+        with pytest.raises(ValueError, match="out overlaps positions"):
+            _launch.rotate_axes_(x, out, pos, (4, 4), 1e4, 0)
+        with pytest.raises(ValueError, match="out_k overlaps positions"):
+            _launch.qk_norm_rotate_(x, k, x, out, None, None, pos, (4, 4), 1e4, 1e-6, 0)
+    pos = torch.zeros(3, 2)
+    with pytest.raises(ValueError, match="out_q overlaps weight_k"):
+        _launch.qk_norm_rotate_(x, k, out, k, None, buf[89:97], pos, (4, 4), 1e4, 1e-6, 0)
+    layouts = [_launch._heads_layout(out)]
+    _launch._check_not_written(layouts, ("out",), positions=buf[96:102], weight_q=None, weight_k=buf[102:110])
+    _launch._check_not_written([_launch._heads_layout(buf[:0].view(0, 3, 2, 8))], ("out",), positions=buf[:6])
