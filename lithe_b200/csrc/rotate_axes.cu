@@ -6,8 +6,8 @@
 //   (a, b) -> (a cos - b sin, b cos + a sin) for pair p's two values: neighbours 2p, 2p + 1
 //   ("interleaved") or p, p + R/2 ("halves"), R = sum of d_axis; values from R on stay.
 //   With the norm: a, b are first x * rsqrt(mean(x^2) + eps) * weight over the head's dim.
-//   Everything in fp32 (the angle's revolution count in fp64, so that far positions keep their
-//   phase), one rounding at the store.
+//   Everything in fp32 (the angle in fp64 up to the fraction of its last turn, so that far positions
+//   keep their phase), one rounding at the store.
 //
 // Bound: HBM (each value is read once and written once; about 3 to 7 operations a value), with the
 // issue rate close behind: the first form, 19 instructions a value, took 380 us for 14 x 4096 tokens
@@ -382,14 +382,21 @@ __global__ void __launch_bounds__(32 * kWarps, kMinBlocks) rotate_kernel(const _
                 p, static_cast<const T*>(t.in) + sample * t.in_sample + token * t.in_token + (h + sub) * t.in_head,
                 per_iter * t.in_head, part, first, second, live, b);
         }
-        // revolutions in fp64, their fraction (at most half a turn) in fp32; each pair's by one lane
+        // revolutions in fp64; their fraction f, in half turns, as an fp32 number and what is left of it, an angle
+        // of at most 2^-25 pi whose sine and cosine are itself and 1 (to 1e-14): the values are within 1.5 units in
+        // their last place, near zero too, where f alone in fp32 would leave 2^-26 pi.  Each pair's by one lane
         __syncwarp();
         for (int pair = lane; pair < (4 * kGroup); pair += 32) {
             float2 a = make_float2(1.0f, 0.0f);
             if (pair < (p.rotated >> 1)) {
                 const double r =
                     position_of(p, sample * p.pos_sample + token * p.axes + tab.axis[pair]) * tab.turn[pair];
-                sincospif(static_cast<float>(2.0 * (r - rint(r))), &a.y, &a.x);
+                const double f = 2.0 * (r - rint(r));
+                const float near = static_cast<float>(f);
+                const float rest = static_cast<float>(f - near) * 3.14159265f;
+                float s, c;
+                sincospif(near, &s, &c);
+                a = make_float2(fmaf(-s, rest, c), fmaf(c, rest, s));
             }
             angle[pair] = a;
         }

@@ -271,3 +271,22 @@ def test_theta_and_axes_are_read_in_every_call():
         assert torch.equal(rotate_axes(x, pos, (axis, 24), theta=theta), rotate_axes(x, pos, (a, 24), theta=t))
         q, _ = qk_norm_rotate(x, x, None, None, pos, (axis, 24), theta=theta)
         assert torch.equal(q, qk_norm_rotate(x, x, None, None, pos, (a, 24), theta=t)[0])
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.float32])
+@pytest.mark.parametrize("far", [3, 1000, 10 ** 5])
+def test_sines_and_cosines_hold_their_last_places(kind, far):
+    """The pair (1, 0) gives the angle's cosine and sine.  They are within 3 half steps of fp32 of the value,
+    also where they are near zero: the sine and cosine of the fraction's fp32 part (2 half steps, a unit in the
+    last place), the sum with its rest (1); the fp64 angles of both sides (frequency, product, reduction: 4 half
+    steps of 2^-53 of the angle each); and 1e-14 for the rest's squares."""
+    g = torch.Generator(device=DEV).manual_seed(far)
+    dim, theta, s = 256, 1e4, 20000
+    pos = (torch.rand(s, 1, generator=g, device=DEV, dtype=torch.float64) * far).to(kind)
+    x = torch.tensor([1.0, 0.0], device=DEV).repeat(dim // 2).expand(1, s, 1, dim)
+    got = rotate_axes(x, pos, (dim,), theta=theta)[0, :, 0].double().view(s, dim // 2, 2)
+    freq = torch.tensor([theta ** (-2.0 * i / dim) for i in range(dim // 2)], dtype=torch.float64, device=DEV)
+    angle = pos.double() * freq
+    for part, want in ((0, angle.cos()), (1, angle.sin())):
+        tol = 3 * 2.0 ** -24 * want.abs() + 8 * 2.0 ** -53 * angle.abs() + 1e-14
+        assert ((got[..., part] - want).abs() <= tol).all()
