@@ -95,25 +95,35 @@ def ordered_after(device: torch.device) -> Optional[Tuple[int, int]]:
     return None if capture < 0 else (stream, capture)
 
 
+_tracing_state = getattr(torch._C, "_get_tracing_state", lambda: None)
 _dispatch_modes = getattr(torch._C, "_len_torch_dispatch_stack", lambda: 0)
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
 
 
 def recorded(t: torch.Tensor) -> bool:
     """Whether a call on ``t`` is recorded or interpreted instead of only run -- torch.compile, jit.trace, a
     dispatch mode (make_fx, FakeTensorMode), a tensor subclass -- so that it must reach its kernel as a torch op."""
-    return (torch.compiler.is_compiling() or torch.jit.is_tracing() or _dispatch_modes() > 0
-            or type(t) not in (torch.Tensor, torch.nn.Parameter))
+    return (torch.compiler.is_compiling() or _tracing_state() is not None or _dispatch_modes() > 0
+            or type(t) not in _PLAIN)
 
 
 def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a derivative through one of the tensors is being recorded: it requires a gradient while grad mode
     is on, or carries a forward-mode tangent.  The kernels have none to give."""
-    grad = torch.is_grad_enabled()
-    forward = getattr(forward_ad, "_current_level", -1) >= 0
-    if not (grad or forward):
-        return False
-    return any(t is not None and ((grad and t.requires_grad)
-                                  or (forward and forward_ad.unpack_dual(t).tangent is not None)) for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if getattr(forward_ad, "_current_level", -1) >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return False
+
+
+def inference_only(*tensors: Optional[torch.Tensor]) -> None:
+    if (torch.is_grad_enabled() or getattr(forward_ad, "_current_level", -1) >= 0) and differentiated(*tensors):
+        raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
 
 
 _lut_cache: dict = {}
@@ -523,11 +533,12 @@ def _heads_strides(t: torch.Tensor) -> tuple:
 _pack_view = struct.Struct("PqqqiI").pack
 
 
-def _heads_layout(t: torch.Tensor) -> tuple:
+def _heads_layout(t: torch.Tensor, shape: Optional[Sequence[int]] = None,
+                  strides: Optional[Sequence[int]] = None) -> tuple:
     """(lithe_heads_view of ``t``, the address of its first byte, the one behind its last, whether its heads,
-    tokens and samples follow one another without meeting)."""
-    b, s, h, d = t.shape
-    sb, ss, sh, _ = t.stride()
+    tokens and samples follow one another without meeting).  ``shape``, ``strides``: t's, where they are at hand."""
+    b, s, h, d = t.shape if shape is None else shape
+    sb, ss, sh, _ = t.stride() if strides is None else strides
     apart = True
     inner = d
     if h == 1:
@@ -549,14 +560,26 @@ def _heads_layout(t: torch.Tensor) -> tuple:
     return _pack_view(first, sb, ss, sh, h, 0), first, first + inner * t.element_size(), apart
 
 
+def _output_layout(t: torch.Tensor, name: str, like: torch.Tensor) -> tuple:
+    """_heads_layout of an output that the caller gave, checked against the input it belongs to."""
+    shape, strides = t.shape, t.stride()
+    if not t.is_cuda or t.dtype != like.dtype or t.device != like.device or len(shape) != 4 or strides[3] != 1:
+        _check_heads(t, name, like)
+    if shape != like.shape:
+        raise ValueError(f"{name} must be {tuple(like.shape)}, got {tuple(shape)}")
+    return _heads_layout(t, shape, strides)
+
+
 def _check_heads(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None) -> None:
-    _require_cuda(t, name)
+    if not t.is_cuda:
+        _require_cuda(t, name)
     if t.dtype not in _DTYPE_CODE:
         raise TypeError(f"{name} must be bfloat16, float16 or float32, got {t.dtype}")
     shape = t.shape
     if len(shape) != 4:
         raise ValueError(f"{name} must be (batch, tokens, heads, dim), got {tuple(shape)}")
-    _check_sizes(t, name)
+    if t.numel() > _MOST:
+        _check_sizes(t, name)
     if t.stride()[3] != 1 and shape[3] > 1:
         raise ValueError(f"{name}: the values of a head must be contiguous (stride 1), got stride {t.stride(3)}")
     if like is not None and (t.dtype != like.dtype or t.device != like.device):
@@ -631,18 +654,6 @@ def _check_outputs(ins: Sequence[torch.Tensor], outs: Sequence[torch.Tensor], na
                 raise ValueError(f"{names[i]} overlaps an input (it may be its own input's very view)")
 
 
-def _check_not_written(outs: Sequence[tuple], names: Sequence[str], **read: Optional[torch.Tensor]) -> None:
-    """No output (their _heads_layout) reaches over a contiguous tensor that every token reads."""
-    for what, t in read.items():
-        if t is None:
-            continue
-        first = t.data_ptr()
-        behind = first + t.numel() * t.element_size()
-        for name, (_, o0, o1, _) in zip(names, outs):
-            if first < o1 and o0 < behind:
-                raise ValueError(f"{name} overlaps {what}")
-
-
 def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta: float, pairing: int) -> tuple:
     code = _POS_CODE.get(positions.dtype)
     if code is None:
@@ -659,21 +670,23 @@ def _rotation_args(x: torch.Tensor, positions: torch.Tensor, axes: tuple, theta:
     return positions.data_ptr(), code, len(shape) - 2, dims, n, freqs, pairing, stream_handle(x.device)
 
 
+def _check_read(first: int, size: int, what: str, out: tuple, name: str) -> None:
+    """The output (its _heads_layout) does not reach over ``size`` bytes from ``first`` on, which every token reads."""
+    if first < out[2] and out[1] < first + size:
+        raise ValueError(f"{name} overlaps {what}")
+
+
 def rotate_axes_(x: torch.Tensor, out: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], theta: float,
                  pairing: int, checked: bool = False, fresh: bool = False) -> torch.Tensor:
     """lithe_rotate_axes on torch tensors: ``out`` (batch, tokens, heads, dim) is written.  ``checked``: the
     caller has checked x; ``fresh``: and made ``out`` for this call."""
     if not checked:
         _check_heads(x, "x")
-    if not fresh:
-        if out is not x:
-            _check_heads(out, "out", x)
-            if out.shape != x.shape:
-                raise ValueError(f"out must be {tuple(x.shape)}, got {tuple(out.shape)}")
-    of_x, of_out = _heads_layout(x), _heads_layout(out)
+    of_x = _heads_layout(x)
+    of_out = _heads_layout(out) if fresh else of_x if out is x else _output_layout(out, "out", x)
     if not fresh:
         _check_outputs((x,), (out,), ("out",), (of_x, of_out))
-        _check_not_written((of_out,), ("out",), positions=positions)
+        _check_read(positions.data_ptr(), positions.nbytes, "positions", of_out, "out")
     b, s, _, d = x.shape
     args = (of_x[0], of_out[0], _DTYPE_CODE[x.dtype], b, s, d,
             *_rotation_args(x, positions, tuple(axes), theta, pairing))
@@ -693,18 +706,14 @@ def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k
     if not checked:
         _check_heads(q, "q")
         _check_heads(k, "k", q)
-    if not fresh:
-        _check_heads(out_q, "out_q", q)
-        _check_heads(out_k, "out_k", q)
-        if out_q.shape != q.shape or out_k.shape != k.shape:
-            raise ValueError(f"out_q and out_k must be {tuple(q.shape)} and {tuple(k.shape)}, got "
-                             f"{tuple(out_q.shape)} and {tuple(out_k.shape)}")
-    layouts = [_heads_layout(t) for t in (q, k, out_q, out_k)]
-    if not fresh:
+    if fresh:
+        layouts = [_heads_layout(t) for t in (q, k, out_q, out_k)]
+    else:
+        layouts = [_heads_layout(q), _heads_layout(k), _output_layout(out_q, "out_q", q), _output_layout(out_k, "out_k", k)]
         _check_outputs((q, k), (out_q, out_k), ("out_q", "out_k"), layouts)
-        _check_not_written(layouts[2:], ("out_q", "out_k"), positions=positions, weight_q=weight_q, weight_k=weight_k)
     b, s, _, d = q.shape
-    if k.shape[0] != b or k.shape[1] != s or k.shape[3] != d:
+    kb, ks, _, kd = k.shape
+    if kb != b or ks != s or kd != d:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} must agree in batch, tokens and dim")
     dtype = weight_dtype = q.dtype
     for w, name in ((weight_q, "weight_q"), (weight_k, "weight_k")):
@@ -717,8 +726,17 @@ def qk_norm_rotate_(q: torch.Tensor, k: torch.Tensor, out_q: torch.Tensor, out_k
         weight_dtype = w.dtype
     if weight_q is not None and weight_k is not None and weight_q.dtype != weight_k.dtype:
         raise TypeError(f"weight_q and weight_k must have one type, got {weight_q.dtype} and {weight_k.dtype}")
-    args = (*(t[0] for t in layouts), weight_q.data_ptr() if weight_q is not None else None,
-            weight_k.data_ptr() if weight_k is not None else None, _DTYPE_CODE[weight_dtype], eps,
+    of_q, of_k, of_out_q, of_out_k = layouts
+    at_q = weight_q.data_ptr() if weight_q is not None else None
+    at_k = weight_k.data_ptr() if weight_k is not None else None
+    if not fresh:
+        lo, hi = min(of_out_q[1], of_out_k[1]), max(of_out_q[2], of_out_k[2])
+        for t, first, what in ((positions, positions.data_ptr(), "positions"), (weight_q, at_q, "weight_q"), (weight_k, at_k, "weight_k")):
+            if first is None or first >= hi or first + t.nbytes <= lo:
+                continue
+            _check_read(first, t.nbytes, what, of_out_q, "out_q")
+            _check_read(first, t.nbytes, what, of_out_k, "out_k")
+    args = (of_q[0], of_k[0], of_out_q[0], of_out_k[0], at_q, at_k, _DTYPE_CODE[weight_dtype], eps,
             _DTYPE_CODE[dtype], b, s, d, *_rotation_args(q, positions, tuple(axes), theta, pairing))
     with device_ctx(q.device):
         rc = _lib.lib().lithe_qk_norm_rotate(*args)
@@ -763,7 +781,8 @@ def _int8_weight(weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optiona
         raise TypeError(f"weight must be int8 on {dev}, got {weight.dtype} on {weight.device}")
     if weight.dim() != 2 or weight.shape[1] != k:
         raise ValueError(f"weight must be (n, {k}), got {tuple(weight.shape)}")
-    _check_sizes(weight, "weight")
+    if weight.numel() > _MOST:
+        _check_sizes(weight, "weight")
     n = weight.shape[0]
     stride, inner = weight.stride()
     if n == 1:
@@ -780,11 +799,14 @@ def _int8_weight(weight: torch.Tensor, weight_scale: torch.Tensor, bias: Optiona
     return n, stride
 
 
+_NO_EXPAND = (None, None, 0, 0)
+
+
 def _int8_expand(h: Optional[torch.Tensor], b_dec: Optional[torch.Tensor], rows: int, n: int,
                  dev: torch.device) -> tuple:
     """The checks of the expand's operands; their (h, b_dec, rows per sample, rank) arguments."""
     if h is None and b_dec is None:
-        return None, None, 0, 0
+        return _NO_EXPAND
     if h is None or b_dec is None:
         raise ValueError("h and b_dec come together")
     for t, name in ((h, "h"), (b_dec, "b_dec")):
@@ -856,7 +878,7 @@ def int8_linear_dynamic(x: torch.Tensor, weight: torch.Tensor, weight_scale: tor
     if rows > _MOST:
         raise NotImplementedError(f"x: {rows} rows are above {_MOST}")
     n, w_stride = _int8_weight(weight, weight_scale, bias, dtype, dev, k)
-    expand = _int8_expand(h, b_dec, rows, n, dev)
+    expand = _NO_EXPAND if h is None and b_dec is None else _int8_expand(h, b_dec, rows, n, dev)
     out = x.new_empty((*shape[:-1], n))
     if rows == 0:
         return out

@@ -19,7 +19,6 @@ from typing import NamedTuple, Optional, Tuple, Union
 import torch
 
 from . import _launch
-from .rotary import _inference_only
 
 
 class QuantizedRows(NamedTuple):
@@ -42,7 +41,7 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
         raise TypeError(f"x must be one of {_launch.ACTIVATION_DTYPES}, got {x.dtype}")
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must be (..., k) with k >= 1, got {tuple(x.shape)}")
-    _inference_only(x)
+    _launch.inference_only(x)
     k = x.shape[-1]
     if x.numel() // k > _launch._MOST:
         raise NotImplementedError(f"x: {x.numel() // k} rows are above {_launch._MOST}")
@@ -79,8 +78,8 @@ def int8_linear(x: Union[torch.Tensor, QuantizedRows], weight: torch.Tensor, wei
     add h . b_dec[sample]^T; every sample has rows / samples consecutive rows (bfloat16 x only).
     Any number of rows, n >= 1, k up to 131072.
     """
-    _inference_only(bias, weight_scale, h, b_dec, *((x.scale,) if isinstance(x, QuantizedRows) else (x,)))
     if isinstance(x, QuantizedRows):
+        _launch.inference_only(x.scale, bias, weight_scale, h, b_dec)
         n = weight.shape[0]
         if _launch.recorded(x.q):
             out = torch.ops.lithe_b200.int8_linear(x.q, x.scale, weight, weight_scale, bias, h, b_dec,
@@ -89,6 +88,7 @@ def int8_linear(x: Union[torch.Tensor, QuantizedRows], weight: torch.Tensor, wei
             out = torch.empty(x.q.shape[0], n, dtype=x.dtype, device=x.q.device)
             _launch.int8_linear_(x.q, x.scale, weight, weight_scale, bias, out, h, b_dec)
         return out.view(*x.shape, n)
+    _launch.inference_only(x, bias, weight_scale, h, b_dec)
     if _launch.recorded(x):
         return torch.ops.lithe_b200.int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec)
     return _launch.int8_linear_dynamic(x, weight, weight_scale, bias, h, b_dec)

@@ -28,11 +28,6 @@ from .. import _lib
 from . import _launch
 
 
-def _inference_only(*tensors: Optional[torch.Tensor]) -> None:
-    if _launch.differentiated(*tensors):
-        raise RuntimeError("lithe_b200 operators are inference-only: run them under torch.no_grad()")
-
-
 def _written(*tensors: torch.Tensor) -> None:
     """Move the version counters of tensors written behind torch's back, as an in-place op does (tensors
     of inference_mode have none and are passed over)."""
@@ -56,7 +51,7 @@ def _rotation(dim: int, axes: Sequence[int], theta: float, pairing: str,
               recorded: bool) -> Tuple[Tuple[int, ...], float, int]:
     """(axes, theta, the pairing's code), plain numbers, checked.  (They are made plain before the lookup: an
     object that can change, a tensor say, is one key with its old value.)"""
-    axes, theta = tuple(operator.index(a) for a in axes), float(theta)
+    axes, theta = tuple(map(operator.index, axes)), float(theta)
     check = _checked_rotation.__wrapped__ if recorded else _checked_rotation
     return axes, theta, check(dim, axes, theta, pairing)
 
@@ -73,13 +68,14 @@ def rotate_axes(x: torch.Tensor, positions: torch.Tensor, axes: Sequence[int], *
     apart from x and the positions.
     """
     _launch._check_heads(x, "x")
-    _inference_only(x, positions, out)
+    _launch.inference_only(x, positions, out)
     as_op = _launch.recorded(x)
     axes, theta, code = _rotation(x.shape[3], axes, theta, pairing, as_op)
     fresh = out is None
     if fresh:
         out = x.new_empty(x.shape)
-    positions = positions.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     if as_op:
         if out is x:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
@@ -108,7 +104,7 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
     """
     _launch._check_heads(q, "q")
     _launch._check_heads(k, "k", q)
-    _inference_only(q, k, weight_q, weight_k, positions, out_q, out_k)
+    _launch.inference_only(q, k, weight_q, weight_k, positions, out_q, out_k)
     eps = float(eps)
     if not (eps >= 0.0 and math.isfinite(eps)):
         raise ValueError(f"eps must be finite and not negative, got {eps}")
@@ -119,7 +115,8 @@ def qk_norm_rotate(q: torch.Tensor, k: torch.Tensor, weight_q: Optional[torch.Te
         out_q = q.new_empty(q.shape)
     if out_k is None:
         out_k = k.new_empty(k.shape)
-    positions = positions.contiguous()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     if as_op:
         oq = torch.empty(q.shape, dtype=q.dtype, device=q.device) if out_q is q else out_q
         ok = torch.empty(k.shape, dtype=k.dtype, device=k.device) if out_k is k else out_k

@@ -200,6 +200,6 @@ def test_outputs_apart_from_what_every_token_reads(monkeypatch):
     pos = torch.zeros(3, 2)
     with pytest.raises(ValueError, match="out_q overlaps weight_k"):
         _launch.qk_norm_rotate_(x, k, out, k, None, buf[89:97], pos, (4, 4), 1e4, 1e-6, 0)
-    layouts = [_launch._heads_layout(out)]
-    _launch._check_not_written(layouts, ("out",), positions=buf[96:102], weight_q=None, weight_k=buf[102:110])
-    _launch._check_not_written([_launch._heads_layout(buf[:0].view(0, 3, 2, 8))], ("out",), positions=buf[:6])
+    behind, none = _launch._heads_layout(out), _launch._heads_layout(buf[:0].view(0, 3, 2, 8))
+    for view in (behind, none):                             # next to an output, and an output without elements
+        _launch._check_read(buf[96:].data_ptr(), 24, "positions", view, "out")
