@@ -344,3 +344,17 @@ def test_one_workspace_many_calls(rows, n, k):
         assert rc == 0
     assert all(torch.equal(out, want[i % 3]) for i, out in enumerate(got))
     assert device_errors() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,k", [(64, 128), (1091, 1000), (3072, 320), (264, 4104), (1290, 12288)])
+def test_a_row_has_the_same_bits_among_any_others(n, k, dtype):
+    """The sums are exact and what follows is one expression everywhere, so a row does not depend on how many
+    there are, that is on which kernel, tile or split takes it."""
+    x = make((2300, k), dtype, 1)
+    w, ws = quantize_weight(make((n, k), dtype, 2, 0.02))
+    bias = make((n,), dtype, 3)
+    whole = int8_linear(x, w, ws, bias)
+    for rows in (1, 2, 8, 9, 16, 17, 40, 128, 129, 255, 600, 1100, 2048, 2299):
+        assert torch.equal(int8_linear(x[:rows], w, ws, bias), whole[:rows]), rows
+    assert torch.equal(int8_linear(x[1000:1003], w, ws, bias), whole[1000:1003])
