@@ -1128,6 +1128,7 @@ __device__ __forceinline__ void tile_kernel_body(const CUtensorMap& tm_q, const 
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
+                // (relaxed: wait::st and the fences, this one and the issuer's, order the sums before its product)
                 if (lane == 0) mbar_arrive_remote_relaxed(ereq);
                 if (!mbar_wait(&bars->efull, tile & 1u, abort, err)) break;
                 tc_fence_after();

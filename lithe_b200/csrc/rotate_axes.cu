@@ -490,13 +490,12 @@ bool aligned(const Heads& t, int size) {
            (s * size) % 16 == 0;
 }
 
-int32_t check_heads(const lithe_heads_view& v, const char* name, int32_t batch, int32_t tokens, int64_t* elements) {
+int32_t check_heads(const lithe_heads_view& v, const char* name) {
     if (v.heads <= 0) return fail_arg("%s: heads must be positive, got %d", name, v.heads);
     if (v.heads > kMostHeads) return fail_unsupported("%s: %d heads above %d", name, v.heads, kMostHeads);
     if (!v.base) return fail_arg("%s must be non-NULL", name);
     if (v.sample_stride < 0 || v.token_stride < 0 || v.head_stride < 0)
         return fail_arg("%s: strides must not be negative", name);
-    *elements = static_cast<int64_t>(batch) * tokens * v.heads;
     return LITHE_OK;
 }
 
@@ -544,9 +543,8 @@ int32_t run(const lithe_heads_view* in, const lithe_heads_view* out, const void*
     if (batch == 0 || tokens == 0) return LITHE_OK;
     if (!positions) return fail_arg("positions must be non-NULL");
     for (int i = 0; i < tensors; ++i) {
-        int64_t n;
-        int32_t rc = check_heads(in[i], i ? "k" : "x", batch, tokens, &n);
-        if (rc == LITHE_OK) rc = check_heads(out[i], i ? "out_k" : "out", batch, tokens, &n);
+        int32_t rc = check_heads(in[i], i ? "k" : "x");
+        if (rc == LITHE_OK) rc = check_heads(out[i], i ? "out_k" : "out");
         if (rc != LITHE_OK) return rc;
         if (in[i].heads != out[i].heads) return fail_arg("an output's heads differ from its input's");
         Heads& t = p.t[i];

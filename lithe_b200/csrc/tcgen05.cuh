@@ -100,8 +100,11 @@ __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
-// The same without release: for an arrival that hands on no memory the thread has written (an
-// accumulator it has read and waited for), where a release would wait for its global stores.
+// The same without release (which would wait for the thread's global stores): for handing TMEM over, read
+// (tcgen05.wait::ld) or written (tcgen05.wait::st), to another thread's tcgen05 instructions.  The order of
+// those accesses comes from the wait, tcgen05.fence::before_thread_sync in front of the arrival and
+// fence::after_thread_sync behind the other thread's wait on the barrier; leave none of them out, and hand no
+// shared or global memory over this way.
 __device__ __forceinline__ void mbar_arrive_remote_relaxed(uint32_t cluster_addr) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
