@@ -537,9 +537,11 @@ int32_t launch_rows(const Params& p, int sms, bool after_quantize, cudaStream_t 
 // Too few 128 x 128 tiles for the SMs: a cluster of `split` CTAs takes one, each a run of its k's.  Their
 // int32 sums go through shared memory, where each CTA adds the others' for its share of the rows (an
 // exact sum, so the split does not show in the result) and finishes them.  A CTA takes in about 60
-// bytes a cycle, 0.3 us a stage of a 128 x 128 tile, and the exchange costs 4 us: 32 x 12288 -> 3072
-// takes 15.2 us on clusters of 4 and 31.0 us on single CTAs, 128 x 3072 -> 3072 (24 stages) 11.7 and 11.6,
-// 256 x 1024 -> 1024 (8 stages) 9.4 and 6.4; clusters of 8 took 4 us more to start.
+// bytes a cycle, 0.3 us a stage of a 128 x 128 tile, and the exchange costs 4 us; clusters of 8 took 4 us more
+// to start.  From 24 stages on a cluster was as fast as a single CTA or faster at every size tried (us, clusters
+// and single CTAs: 32 x 12288 -> 3072 14.7 and 30.8; at 24 stages, -> 3072, 128 rows 11.8 and 11.8, 32 rows 9.3
+// and 11.4, 256 rows -> 1024 10.9 and 11.5; at 16 stages 11.2 and 9.7, 8.6 and 9.3, 10.0 and 9.2; at 8 10.4 and
+// 7.4, 7.5 and 6.9, 8.9 and 6.5).
 // Every mbarrier wait is bounded (4 s, LITHE_DEVERR_TIMEOUT, shared abort flag).
 enum Expand { kExpandNone, kExpandMma, kExpandTmem };
 
@@ -1298,8 +1300,11 @@ template <bool kF16, bool kWhole>
 int32_t launch_quantize(const QuantParams& p, cudaStream_t st) {
     const int pieces = (p.k + 7) / 8;
     const int short_ctas = static_cast<int>((static_cast<int64_t>(p.rows) + kThreadsQ / 32 - 1) / (kThreadsQ / 32));
-    // (3072 values: four warps a row are faster up to 1024 rows, and one from 4096 on)
-    const bool few = p.rows <= 2048 && pieces > 32 * 2;
+    // Four warps a row where there are few: up to 2048 rows, up to 1024 of at most 1024 values (us, four warps and
+    // one: 256 x 3072 2.3 and 3.4, 2048 x 3072 6.3 and 6.9, 4096 x 3072 9.6 and 9.5, 8192 x 3072 16.8 and 14.9;
+    // 2048 x 1536 4.2 and 4.5, 4096 x 1536 6.5 and 6.1; 512 x 1001 2.5 and 2.8, 1024 x 1001 3.1 and 3.0,
+    // 2048 x 1001 5.3 and 4.3; 1024 x 576 2.2 and 2.2, 2048 x 576 2.9 and 2.6).
+    const bool few = p.rows <= (pieces > 128 ? 2048 : 1024) && pieces > 32 * 2;
     if (!kWhole && p.k <= 32 * 4) quantize_short_kernel<kF16, 4><<<short_ctas, kThreadsQ, 0, st>>>(p);
     else if (!kWhole && p.k <= 32 * kShortMost) quantize_short_kernel<kF16, kShortMost><<<short_ctas, kThreadsQ, 0, st>>>(p);
     else if (few && pieces <= 128 * 2) launch_quantize_rows<kF16, kWhole, 4, 2>(p, st);
