@@ -422,7 +422,7 @@ __device__ __forceinline__ void quantize_here(const Params& p, int8_t* q, float*
 
 template <bool kF16, int kTiles, bool kDirect>
 __global__ void __launch_bounds__(32 * kMaxSplit, 2) int8_rows_kernel(const Params p) {
-    extern __shared__ int part_raw[];
+    extern __shared__ __align__(16) int part_raw[];          // (kDirect reads its row from it in 16-byte pieces)
     __shared__ float scale;
     __shared__ uint32_t row_max[kMaxSplit];
     int(*part)[8 * kTiles][17] = reinterpret_cast<int(*)[8 * kTiles][17]>(part_raw);   // [warp][row][channel]
