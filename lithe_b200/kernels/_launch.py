@@ -35,7 +35,7 @@ def error_word(device: torch.device) -> torch.Tensor:
     device = torch.device(device)
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    with _err_lock:
+    with _err_lock, torch.inference_mode(False):         # (device_errors clears it in any mode)
         t = _err_words.get(device.index)
         if t is None:
             t = torch.zeros(1, dtype=torch.int32, device=device)

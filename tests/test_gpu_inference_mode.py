@@ -88,3 +88,29 @@ def test_a_bank_made_under_inference_mode(key_format, int8):
             m.bank = other
         assert torch.equal(model(*args), got) and torch.equal(model(*args), got)
     assert device_errors() == 0
+
+
+def in_a_new_process(code):
+    """What a first call leaves behind needs a process without earlier ones."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    got = subprocess.run([sys.executable, "-c", "import torch\n" + code], cwd=Path(__file__).resolve().parents[1],
+                         capture_output=True, text=True, timeout=300)
+    assert got.returncode == 0 and got.stdout.strip().endswith("ok"), got.stderr[-2000:]
+
+
+def test_errors_of_a_first_call_under_inference_mode_can_be_cleared():
+    in_a_new_process("""
+from lithe_b200 import device_errors
+from lithe_b200.kernels import PackedBank, PackedLayout, wrap_packed, PackedLoRALinear
+lay = PackedLayout.from_modules([{"name": "m", "shape_a": [16, 128], "shape_b": [128, 16]}])
+with torch.inference_mode():
+    bank = PackedBank(lay, 2, "cuda")
+    layer = PackedLoRALinear(torch.nn.Linear(128, 128, device="cuda", dtype=torch.bfloat16), bank, "m", 16, 1.0)
+    layer.assign = torch.tensor([7], dtype=torch.int32, device="cuda")       # out of range: reported, not followed
+    layer(torch.zeros(1, 4, 128, device="cuda", dtype=torch.bfloat16))
+assert device_errors() != 0
+assert device_errors() == 0
+print("ok")
+""")
