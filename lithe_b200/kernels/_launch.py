@@ -107,6 +107,13 @@ def recorded(t: torch.Tensor) -> bool:
             or type(t) not in _PLAIN)
 
 
+def laid_out(t: torch.Tensor) -> None:
+    """Called where weights or banks are laid out: ``t``'s device gets its error word, so that no graph capture is
+    the first to need it.  A word made inside one is zeroed, with the errors in it, by every replay."""
+    if t.is_cuda and not recorded(t):
+        error_word(t.device)
+
+
 def differentiated(*tensors: Optional[torch.Tensor]) -> bool:
     """Whether a derivative through one of the tensors is being recorded: it requires a gradient while grad mode
     is on, or carries a forward-mode tangent.  The kernels have none to give."""

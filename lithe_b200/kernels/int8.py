@@ -63,6 +63,7 @@ def quantize_weight(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if weight.dim() != 2:
         raise ValueError(f"weight must be (n, k), got {tuple(weight.shape)}")
     got = quantize_rows(weight.detach())
+    _launch.laid_out(got.q)
     return got.q, got.scale
 
 

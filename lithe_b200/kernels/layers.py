@@ -73,6 +73,7 @@ class Int8Linear(nn.Module):
         self.register_buffer("weight_q", weight_q.contiguous())
         self.register_buffer("weight_scale", weight_scale.float().contiguous())
         self.register_buffer("bias", None if bias is None else bias.detach().contiguous())
+        _launch.laid_out(self.weight_q)
 
     @classmethod
     def from_linear(cls, linear: nn.Linear) -> "Int8Linear":
@@ -88,6 +89,7 @@ class Int8Linear(nn.Module):
         super()._apply(fn, recurse)
         if self.weight_scale.dtype != torch.float32:
             self.weight_scale = scale.to(self.weight_scale.device)
+        _launch.laid_out(self.weight_q)
         return self
 
     @property
@@ -115,6 +117,7 @@ class IndexLoRALinear(nn.Module):
         dev = base.weight.device
         self.register_buffer("idx_a", idx_a.to(device=dev, dtype=torch.int32).contiguous(), persistent=False)
         self.register_buffer("idx_b", idx_b.to(device=dev, dtype=torch.int32).contiguous(), persistent=False)
+        _launch.laid_out(self.idx_a)
         self.register_buffer("pool_a", pool_a.to(dev), persistent=False)
         self.register_buffer("pool_b", pool_b.to(dev), persistent=False)
         self.rank = int(rank)

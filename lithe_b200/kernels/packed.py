@@ -221,6 +221,7 @@ class PackedBank:
         self.device = torch.device(device)
         self.slot_stride = layout.num_words + (layout.num_words & 1)
         self.words = torch.zeros((n_slots, self.slot_stride), dtype=torch.int64, device=self.device)
+        _launch.laid_out(self.words)
         self._kernel_writes = 0          # slot writes by the pack kernels (not seen by words._version)
         pa, pb = pools if pools is not None else cb.twin_pools()
         self.pool_a, self.pool_b = pa, pb

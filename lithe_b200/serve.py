@@ -138,6 +138,7 @@ class MultiAdapterLinear(nn.Module):
             raise ValueError("adapter index shapes do not match this layer")
         self.idx_a = torch.cat([self.idx_a, ia]).contiguous()
         self.idx_b = torch.cat([self.idx_b, ib]).contiguous()
+        _launch.laid_out(self.idx_a)
         self.scales.append(float(scale))
         self._n_added += 1
 

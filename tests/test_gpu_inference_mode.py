@@ -114,3 +114,43 @@ assert device_errors() != 0
 assert device_errors() == 0
 print("ok")
 """)
+
+
+@pytest.mark.parametrize("setup", ["int8", "int8 layer", "bank", "index"])
+def test_a_first_call_inside_a_capture_leaves_the_error_word_alone(setup):
+    """The error word is there before a graph is captured: replays do not clear the errors in it."""
+    in_a_new_process(f"""
+from lithe_b200 import device_errors
+from lithe_b200.kernels import (IndexLoRALinear, Int8Linear, PackedBank, PackedLayout, PackedLoRALinear, _launch, int8_linear,
+                                quantize_weight)
+from lithe_b200 import codebook as cb
+bf = torch.bfloat16
+x = torch.ones(1, 40, 128, device="cuda", dtype=bf)
+lin = torch.nn.Linear(128, 128, device="cuda", dtype=bf).requires_grad_(False)
+if {setup!r} == "int8":
+    w, ws = quantize_weight(lin.weight)
+    call = lambda: int8_linear(x, w, ws)
+elif {setup!r} == "int8 layer":         # as from a checkpoint: filled on the CPU, then moved
+    call = lambda: layer(x)
+    layer = Int8Linear(128, 128, torch.ones(128, 128, dtype=torch.int8), torch.ones(128)).cuda()
+elif {setup!r} == "bank":
+    lay = PackedLayout.from_modules([{{"name": "m", "shape_a": [16, 128], "shape_b": [128, 16]}}])
+    layer = PackedLoRALinear(lin, PackedBank(lay, 2, "cuda"), "m", 16, 1.0)
+    layer.assign = torch.zeros(1, dtype=torch.int32, device="cuda")
+    call = lambda: layer(x)
+else:
+    idx = torch.zeros(2, 3, 32, dtype=torch.int32, device="cuda")
+    layer = IndexLoRALinear(lin, idx, idx, *cb.twin_pools(), 16, 1.0)
+    layer.assign = torch.zeros(1, dtype=torch.int32, device="cuda")
+    call = lambda: layer(x)
+lin(x)                                  # (cuBLAS lays out its own before a capture)
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.no_grad(), torch.cuda.graph(graph):
+    out = call()
+assert device_errors() == 0             # before any replay
+_launch.error_word(torch.device("cuda", 0)).fill_(4)
+graph.replay()
+assert device_errors() == 4
+print("ok")
+""")
