@@ -528,9 +528,9 @@ int32_t launch_rows(const Params& p, int sms, bool after_quantize, cudaStream_t 
 //                 TMEM in place of the int32 ones; one tcgen05.mma (kind::f16, K = 16) adds the expand
 //                 of the whole tile there, issued by a warp of its own (polled for by the products'
 //                 issuer it cost 10%), and the epilogue reads the result.  Warp MMAs share the
-//                 tensor pipe with tcgen05.mma and slow it: 57344 x 3072 -> 12288 takes 1.71 ms
-//                 this way, 2.1 ms with them and 1.6 ms without an expand (1.46 ms: the products
-//                 alone; all of it under the 1 kW cap, at 1.3 to 1.5 GHz).
+//                 tensor pipe with tcgen05.mma and slow it: 57344 x 3072 -> 12288 takes 1.42 ms
+//                 this way, 1.69 ms with them and 1.38 ms without an expand, calls 30 ms apart; with
+//                 the quantisation and in a row, under the 1 kW cap, 1.75, 2.01 and 1.67 ms.
 // Measured without an expand: 14336 x 3072 -> 12288 2.8 POP/s, x 768 -> 12288 130 us (an epilogue of 4
 // warps with a TMA store of 64-byte rows: 257 us).  In a tile the stages' bytes (64 KB a pair and
 // 128 k's) keep shared memory as busy as the products keep the tensor pipe.

@@ -18,9 +18,9 @@
 // pair costs four products two at a time (f32x2), the norm's factor two more.  The sum of squares is
 // a shuffle inside the lanes of a head.  kBatch heads are loaded before the first is used, the
 // token's first ones before its angles.
-// Measured on B200: 14 x 4096 tokens of 24 + 24 heads of 128, norm and rotation, 242 us (5.8 TB/s, 0.90 of
-// the measured copy rate; 250 us back to back, at the 1 kW cap); 32760 tokens of 24 heads, rotation, 64 us
-// (6.3 TB/s, 0.98); one token 3.2 us.
+// Measured on B200: 14 x 4096 tokens of 24 + 24 heads of 128, norm and rotation, 245 us (5.75 TB/s, 0.89 of
+// the measured copy rate; 251 us back to back, at the 1 kW cap); 32760 tokens of 24 heads, rotation, 63 us
+// (6.4 TB/s, 0.98); one token 2.9 us.
 // A second batch of heads on its way while one is turned took registers that cost more (306 us).
 #include <cmath>
 #include <type_traits>
