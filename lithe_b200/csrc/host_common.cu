@@ -77,6 +77,17 @@ static int32_t get_encoder(PFN_cuTensorMapEncodeTiled_v12000* out) {
     return LITHE_OK;
 }
 
+// The encoder wants a current context, which a thread has only once a runtime call of its own has bound one: the
+// first call that a thread makes here may come before that.  (cudaSetDevice binds it, also during a capture.)
+template <typename... Args>
+static CUresult encode(PFN_cuTensorMapEncodeTiled_v12000 enc, Args... args) {
+    CUresult r = enc(args...);
+    int device = 0;
+    if (r == CUDA_ERROR_INVALID_CONTEXT && cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess)
+        r = enc(args...);
+    return r;
+}
+
 int32_t encode_bf16_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
                        uint32_t b0, uint32_t b1) {
     PFN_cuTensorMapEncodeTiled_v12000 enc;
@@ -86,7 +97,7 @@ int32_t encode_bf16_3d(CUtensorMap* map, const void* base, uint64_t d0, uint64_t
     const cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};   // bytes, dims 1 and 2
     const cuuint32_t box[3] = {b0, b1, 1};
     const cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides,
+    CUresult r = encode(enc, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides,
                      box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
@@ -109,7 +120,7 @@ int32_t encode_bf16_chunked(CUtensorMap* map, const void* base, uint64_t inner, 
     const cuuint64_t strides[2] = {inner * 2, 128};
     const cuuint32_t box[3] = {64, box_rows, chunks_per_box};
     const cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
+    CUresult r = encode(enc, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
@@ -131,7 +142,7 @@ int32_t encode_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint6
     const cuuint64_t strides[1] = {inner * 2};
     const cuuint32_t box[2] = {box_inner, box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
+    CUresult r = encode(enc, map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, sw, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
@@ -149,7 +160,7 @@ int32_t encode_u8_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_
     const cuuint64_t strides[1] = {pitch};
     const cuuint32_t box[2] = {box_inner, box_rows};
     const cuuint32_t estr[2] = {1, 1};
-    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+    CUresult r = encode(enc, map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
