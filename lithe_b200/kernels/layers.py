@@ -16,6 +16,7 @@ otherwise ``assign`` (B,) gives the slot of every sample, -1 for none.
 """
 from __future__ import annotations
 
+import threading
 import weakref
 from typing import Callable, Dict, Iterable, List, Optional, Tuple
 
@@ -205,6 +206,11 @@ class _RouteKey:
                 and self._where is not None and self._where == _launch.ordered_after(ids.device))
 
 
+# Held while a group looks at and changes what it keeps (a few fields that belong together), so that threads
+# calling one model see whole states.  One for all groups: a lock of a group's own could not be copied with it.
+PREP_LOCK = threading.Lock()
+
+
 class SharedInputPrep:
     """Fused-GEMM linears with their own adapter modules that read the same input tensor -- the
     q, k and v projections of one attention block.  The first member to run on an input
@@ -243,6 +249,11 @@ class SharedInputPrep:
         """(h, b_dec) of ``layer`` for this call, or None when the group does not apply."""
         if not _tracked(x3, ids, w, layer.bank.words):
             return None
+        with PREP_LOCK:
+            return self._prep(layer, x3, ids, w)
+
+    def _prep(self, layer: "PackedLoRALinear", x3: torch.Tensor, ids: torch.Tensor,
+              w: Optional[torch.Tensor]) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
         extra = (layer.bank.contents_key(), tuple(m.scaling for m in self.members))
         if self._key is not None:
             if self._key.matches(x3, ids, w, extra):
@@ -458,8 +469,9 @@ class PackedLoRALinear(nn.Module):
             # contents are unchanged (a denoise loop's steps); traced graphs decode every call
             b_dec = None
             bank_key = self.bank.contents_key() if keep else None
-            if keep and self._bdec_cache is not None and self._bdec_cache[0].matches(ids, bank_key):
-                b_dec = self._bdec_cache[1]
+            cache = self._bdec_cache                 # (read once: another thread may replace it)
+            if keep and cache is not None and cache[0].matches(ids, bank_key):
+                b_dec = cache[1]
             if b_dec is None:
                 h_new, b_dec = torch.ops.lithe_b200.lora_prep(x3, words, words, self._va, self._vb, self.bank.n_slots,
                                                               ids, w, d_out, self._lut, self.scaling, fresh)

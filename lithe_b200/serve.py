@@ -23,7 +23,8 @@ from . import codebook as cb
 from . import quant
 from .fileio import LitheAdapter
 from .kernels import _launch, ops
-from .kernels.layers import FUSED_GEMM_MAX_K, _inference_only, _InputKey, _RouteKey, _tracked, shared_input_sets
+from .kernels.layers import (FUSED_GEMM_MAX_K, PREP_LOCK, _inference_only, _InputKey, _RouteKey, _tracked,
+                             shared_input_sets)
 
 Route = Sequence[Tuple[int, float]]
 
@@ -229,6 +230,11 @@ class _RoutePrepGroup:
              w: torch.Tensor) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
         if not _tracked(x, ids, w, *(t for m in self.members for t in (m.idx_a, m.idx_b))):
             return None
+        with PREP_LOCK:
+            return self._prep(layer, x, xs, ids, w)
+
+    def _prep(self, layer: "MultiAdapterLinear", x: torch.Tensor, xs: torch.Tensor, ids: torch.Tensor,
+              w: torch.Tensor) -> Optional[Tuple[torch.Tensor, torch.Tensor]]:
         extra = tuple((m._n_added, m.idx_a._version, m.idx_b._version) for m in self.members)
         if self._key is not None:
             if self._key.matches(x, ids, w, extra):
